@@ -47,6 +47,29 @@ class UViTBlockArgs(_c.Structure):
                 ("workspace", _P), ("workspace_bytes", _Z), ("y", _P), ("x_planes", _P), ("skip_planes", _P), ("y_planes", _P)]
 
 
+class SandwichNormArgs(_c.Structure):
+    _fields_ = [("x", _P), ("y", _P), ("dtype", _I), ("param_dtype", _I), ("rows", _L), ("D", _I), ("post", _I), ("pre", _I),
+                ("post_w", _P), ("post_b", _P), ("pre_w", _P), ("pre_b", _P), ("gate", _P), ("gate_rows", _L),
+                ("res_scale", _F), ("eps", _F), ("r", _P), ("z", _P), ("stats", _P), ("dr", _P), ("dz", _P), ("dx", _P), ("dy", _P),
+                ("dgate", _P), ("dpost_w", _P), ("dpost_b", _P), ("dpre_w", _P), ("dpre_b", _P), ("workspace", _P), ("workspace_bytes", _Z)]
+
+
+class RelAttentionArgs(_c.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("dtype", _I), ("B", _I), ("Tq", _I), ("Tk", _I), ("heads", _I), ("kv_heads", _I), ("ch", _I),
+                ("q_batch", _L), ("q_row", _L), ("k_batch", _L), ("k_row", _L), ("v_batch", _L), ("v_row", _L),
+                ("table", _P), ("table_dtype", _I), ("bucket_map", _P), ("radius", _I), ("num_buckets", _I), ("klen", _P), ("qstart", _P),
+                ("causal", _I), ("scale", _F), ("out", _P), ("out_batch", _L), ("out_row", _L), ("lse", _P),
+                ("dout", _P), ("dout_batch", _L), ("dout_row", _L), ("dq", _P), ("dk", _P), ("dv", _P),
+                ("dq_batch", _L), ("dq_row", _L), ("dk_batch", _L), ("dk_row", _L), ("dv_batch", _L), ("dv_row", _L),
+                ("dtable", _P), ("workspace", _P), ("workspace_bytes", _Z)]
+
+
+class TokenLogprobsArgs(_c.Structure):
+    _fields_ = [("logits", _P), ("dtype", _I), ("rows", _L), ("V", _L), ("ld", _L), ("ids", _P), ("k", _I), ("inv_temperature", _F),
+                ("logprob", _P), ("entropy", _P), ("lse", _P), ("top_ids", _P), ("top_logprobs", _P), ("stats", _P),
+                ("dlogprob", _P), ("dentropy", _P), ("dtop", _P), ("dlogits", _P), ("ldd", _L), ("workspace", _P), ("workspace_bytes", _Z)]
+
+
 # name -> (restype, argtypes); every symbol include/dua_hip.h declares
 SIGNATURES = {
     "dua_version": (_I, []),
@@ -168,6 +191,15 @@ SIGNATURES = {
     "dua_patchify": (_I, [_P, _P, _I, _I, _I, _I, _I, _P]),
     "dua_uvit_assemble": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P]),
     "dua_unpatchify": (_I, [_P, _P, _I, _I, _I, _I, _I, _P]),
+    "dua_sandwich_norm": (_I, [_c.POINTER(SandwichNormArgs), _P]),
+    "dua_sandwich_norm_bwd_workspace_bytes": (_Z, [_c.POINTER(SandwichNormArgs)]),
+    "dua_sandwich_norm_bwd": (_I, [_c.POINTER(SandwichNormArgs), _P]),
+    "dua_rel_attention_workspace_bytes": (_Z, [_c.POINTER(RelAttentionArgs), _I]),
+    "dua_rel_attention": (_I, [_c.POINTER(RelAttentionArgs), _P]),
+    "dua_rel_attention_bwd": (_I, [_c.POINTER(RelAttentionArgs), _P]),
+    "dua_token_logprobs_workspace_bytes": (_Z, [_c.POINTER(TokenLogprobsArgs)]),
+    "dua_token_logprobs": (_I, [_c.POINTER(TokenLogprobsArgs), _P]),
+    "dua_token_logprobs_bwd": (_I, [_c.POINTER(TokenLogprobsArgs), _P]),
 }
 
 _lib = None

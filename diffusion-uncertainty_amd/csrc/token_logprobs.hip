@@ -1,0 +1,495 @@
+// Log probabilities of given tokens with the entropy of each row's distribution and its k best alternatives, and their gradient.
+//   l = t x;  lse = log sum e^l;  logprob = l_id - lse;  H = -sum p l^  (l^ = l - lse, p = e^l^);  top k by (value descending, index ascending)
+//   dx = t [ glp (d_id - p) + sum_j gtop_j (d_top_j - p) - gH p (l^ + H) ]
+// Memory bound: the row is read once (backward: read once, written once).  One pass keeps, per thread, the running maximum m and the sums
+// s = sum e^(l-m), w = sum e^(l-m) (l-m), all fp32 and rescaled when m moves; lse = m + log s, H = log s - w / s.  Differences x - m are
+// formed BEFORE the temperature and the base change, so huge common offsets and masks of the type's lowest value keep their meaning.
+// The alternatives ride along: a thread remembers its best 16-byte group and the best value outside it.  The k-th largest of the threads'
+// maxima is a lower bound of the row's k-th largest value; only groups that reach it are read again (about k of them), a thread whose
+// second value reaches it too is re-read whole (about k^2 / 512 of them), and the few candidates are ranked exactly.  Rows with many equal
+// values, NaN or +inf take an ordered scan of the row in the same kernel (select_ordered).
+// Any alignment: a row is walked in aligned 16-byte groups, its first and last group element by element.
+#include <float.h>
+#include "elem.h"
+
+namespace {
+
+constexpr int NT = 256, NW = NT / 64;
+constexpr int KMAX = 64;                 // alternatives
+constexpr int CAP = 1024;                // candidates of the fast selection
+constexpr int RESCAN = 64;               // threads re-read whole before the ordered scan is cheaper
+constexpr int SMAX = 32;                 // parts of a row
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Soft { float m, s, w; };          // w in log2 units
+// moves a partial sum to a larger maximum; c = t log2 e.  The difference is clamped so that 0 * inf cannot arise (2^-1e4 = 0)
+__device__ __forceinline__ void soft_to(Soft& a, float m, float c) {
+    const float d = fmaxf((a.m - m) * c, -1e4f), f = __builtin_amdgcn_exp2f(d);
+    a.w = f * (a.w + a.s * d);
+    a.s *= f;
+    a.m = m;
+}
+__device__ __forceinline__ Soft soft_join(Soft a, Soft b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    soft_to(a, m, c);
+    soft_to(b, m, c);
+    return Soft{m, a.s + b.s, a.w + b.w};
+}
+
+// total order of floats as whole numbers: -0 = +0, every NaN above +inf
+__device__ __forceinline__ uint32_t okey(float x) {
+    if (x != x) return 0xFFFFFFFFu;
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return (b >> 31) ? ~b : b | 0x80000000u;
+}
+
+struct LogpP {
+    const void* x;
+    const int64_t* ids;
+    float *logprob, *entropy, *lse, *stats;          // stats [rows][4]: m, log s, H, -
+    int64_t* top_ids;
+    float* top_lp;
+    long rows, ld, V;
+    int k, splits;
+    float t;
+    float* part;                                      // [rows][splits][4 + 2 k]: m, s, w, - ; values ; indices (as int32 bits, within V < 2^31)
+    // backward
+    const float *dlp, *dent, *dtop;
+    const int64_t* tids;
+    void* dx;
+    long ldd;
+};
+
+// The 16-byte groups of elements [v0, v1) of a row: group g holds elements first + g * VEC ... ; the first and last may stick out.
+template <typename T> struct Groups {
+    static constexpr int VEC = Elem<T>::VEC;
+    const T* row;
+    long first, v0, v1, n;
+    __device__ Groups(const T* r, long a, long b) : row(r), v0(a), v1(b) {
+        const long mis = (long)(((uintptr_t)(r + a) & 15) / sizeof(T));
+        first = a - mis;
+        n = (b - first + VEC - 1) / VEC;
+    }
+    __device__ __forceinline__ bool whole(long g) const { return first + g * VEC >= v0 && first + (g + 1) * VEC <= v1; }
+    __device__ __forceinline__ void load(long g, float* f) const {                       // elements outside [v0, v1): -inf
+        const long e = first + g * VEC;
+        if (whole(g)) {
+            ld_elems<T, VEC>(row + e, f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = e + j >= v0 && e + j < v1 ? (float)row[e + j] : -INFINITY;
+        }
+    }
+};
+
+struct Shared {
+    Soft soft[NW];
+    uint32_t key[NT];
+    uint32_t ck[CAP];                     // candidates: key, index
+    int ci[CAP];
+    int rescan[RESCAN];
+    uint32_t tau;
+    int ncand, nrescan, any;
+    uint32_t bk[2][KMAX];                 // running best of the ordered scan
+    int bi[2][KMAX];
+};
+
+// Number of entries of key[0, n) that beat (k, i); entries tie by the lower index.
+__device__ __forceinline__ int rank_of(const uint32_t* key, const int* idx, int n, uint32_t k, int i) {
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += key[j] > k || (key[j] == k && idx[j] < i);
+    return r;
+}
+__device__ __forceinline__ int rank_of_thread(const uint32_t* key, uint32_t k, int t) {
+    int r = 0;
+    for (int j = 0; j < NT; ++j) r += key[j] > k || (key[j] == k && j < t);
+    return r;
+}
+
+// Exact selection by one ordered scan: 256 groups at a time in index order; a chunk is looked at only if one of its values beats the k-th of
+// the best so far.  Of a chunk only the k threads with the best (largest, then leftmost) maxima can hold winners: every element of another
+// thread is beaten by those k maxima.  Leaves the k best, sorted, in sh.bk / sh.bi[return value].
+template <typename T>
+__device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
+    constexpr int VEC = Elem<T>::VEC;
+    const int tid = threadIdx.x;
+    int cur = 0;
+    long have = 0;
+    for (long g0 = 0; g0 < gr.n; g0 += NT) {
+        const long g = g0 + tid, e0 = gr.first + g * VEC;
+        float f[VEC];
+        uint32_t best = 0;                                     // 0: below every float's key
+        if (g < gr.n) {
+            gr.load(g, f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (e0 + j >= gr.v0 && e0 + j < gr.v1) best = max(best, okey(f[j]));
+        }
+        __syncthreads();
+        if (tid == 0) { sh.any = 0; sh.ncand = 0; }
+        sh.key[tid] = best;
+        __syncthreads();
+        const uint32_t bar = have >= k ? sh.bk[cur][k - 1] : 0;
+        if (best > bar) sh.any = 1;
+        __syncthreads();
+        if (!sh.any) continue;
+        if (best > bar && rank_of_thread(sh.key, best, tid) < k) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (e0 + j >= gr.v0 && e0 + j < gr.v1 && okey(f[j]) > bar) {
+                    const int at = atomicAdd(&sh.ncand, 1);     // at most k * VEC <= 512: fits
+                    sh.ck[at] = okey(f[j]);
+                    sh.ci[at] = (int)(e0 + j);
+                }
+        }
+        __syncthreads();
+        const int n = sh.ncand, old = (int)min((long)k, have);
+        // ranks within the union of the old best (all of them left of the chunk) and the new candidates
+        for (int i = tid; i < n + old; i += NT) {
+            const uint32_t kk = i < n ? sh.ck[i] : sh.bk[cur][i - n];
+            const int ii = i < n ? sh.ci[i] : sh.bi[cur][i - n];
+            const int r = rank_of(sh.ck, sh.ci, n, kk, ii) + rank_of(sh.bk[cur], sh.bi[cur], old, kk, ii);
+            if (r < k) { sh.bk[cur ^ 1][r] = kk; sh.bi[cur ^ 1][r] = ii; }
+        }
+        have += n;
+        cur ^= 1;
+        __syncthreads();
+    }
+    __syncthreads();
+    return cur;
+}
+
+// Soft sums and the k best (sorted, with their values) of elements [v0, v1) of one row by one workgroup; k <= v1 - v0.
+template <typename T>
+__device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared& sh, int& best_set) {
+    constexpr int VEC = Elem<T>::VEC;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Groups<T> gr(row, v0, v1);
+    Soft a{-FLT_MAX, 0.f, 0.f};
+    float b1 = -INFINITY, b2 = -INFINITY;                 // best value, best value outside the best group
+    long bg = -1;
+    auto eat = [&](const float* f, long g) {
+        float vm = f[0];
+#pragma unroll
+        for (int j = 1; j < VEC; ++j) vm = fmaxf(vm, f[j]);
+        b2 = fmaxf(b2, fminf(b1, vm));
+        if (vm > b1 || bg < 0) bg = g;
+        b1 = fmaxf(b1, vm);
+        const float m = fmaxf(a.m, vm);
+        if (m > a.m) soft_to(a, m, c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float d = (f[j] - m) * c, e = __builtin_amdgcn_exp2f(d);
+            a.s += e;
+            a.w += e * fmaxf(d, -150.f);                  // 2^-150 = 0: e is 0 wherever the clamp acts, and 0 * -inf does not arise
+        }
+    };
+    long g = tid;
+    for (; g + NT < gr.n; g += 2 * NT) {
+        float f0[VEC], f1[VEC];
+        gr.load(g, f0);
+        gr.load(g + NT, f1);
+        eat(f0, g);
+        eat(f1, g + NT);
+    }
+    if (g < gr.n) {
+        float f0[VEC];
+        gr.load(g, f0);
+        eat(f0, g);
+    }
+    Soft t = a;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const Soft u{__shfl_xor(t.m, o, 64), __shfl_xor(t.s, o, 64), __shfl_xor(t.w, o, 64)};
+        t = soft_join(t, u, c);
+    }
+    __syncthreads();
+    if (lane == 0) sh.soft[wave] = t;
+    sh.key[tid] = bg < 0 ? 0u : okey(b1);
+    if (tid == 0) { sh.ncand = 0; sh.nrescan = 0; sh.any = 0; }
+    __syncthreads();
+    t = sh.soft[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) t = soft_join(t, sh.soft[i], c);
+    best_set = 0;
+    if (k == 0) return t;
+
+    const bool odd = !(t.s < INFINITY);                    // NaN, or infinite: NaN / +inf among the logits
+    if (!odd) {
+        const uint32_t mine = sh.key[tid];
+        if (rank_of_thread(sh.key, mine, tid) == k - 1) sh.tau = mine;
+        __syncthreads();
+        const uint32_t tau = sh.tau;                       // 0: fewer than k threads hold elements - every element is a candidate
+        auto push = [&](long e, float x) {
+            if (e >= gr.v0 && e < gr.v1 && okey(x) >= tau) {
+                const int at = atomicAdd(&sh.ncand, 1);
+                if (at < CAP) { sh.ck[at] = okey(x); sh.ci[at] = (int)e; }
+            }
+        };
+        if (bg >= 0 && mine >= tau) {
+            if (tau && okey(b2) >= tau && b2 > -INFINITY) {
+                const int at = atomicAdd(&sh.nrescan, 1);
+                if (at < RESCAN) sh.rescan[at] = tid;
+            } else if (tau && okey(b2) >= tau) {
+                sh.any = 1;                                 // the bound itself is -inf: too few finite values
+            } else {
+                float f[VEC];
+                gr.load(bg, f);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) push(gr.first + bg * VEC + j, f[j]);
+            }
+        }
+        __syncthreads();
+        const int nr = sh.nrescan;
+        if (nr <= RESCAN && !sh.any) {
+            for (int i = wave; i < nr; i += NW)
+                for (long gg = sh.rescan[i] + (long)lane * NT; gg < gr.n; gg += 64L * NT) {
+                    float f[VEC];
+                    gr.load(gg, f);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) push(gr.first + gg * VEC + j, f[j]);
+                }
+            __syncthreads();
+            const int n = sh.ncand;
+            if (n <= CAP) {
+                for (int i = tid; i < n; i += NT) {
+                    const int r = rank_of(sh.ck, sh.ci, n, sh.ck[i], sh.ci[i]);
+                    if (r < k) { sh.bk[0][r] = sh.ck[i]; sh.bi[0][r] = sh.ci[i]; }
+                }
+                __syncthreads();
+                return t;
+            }
+        }
+    }
+    best_set = select_ordered(gr, k, sh);
+    return t;
+}
+
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return k == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((k >> 31) ? k & 0x7FFFFFFFu : ~k);
+}
+
+// log probability of a value; a row without any finite value has no distribution: -inf everywhere, entropy 0
+__device__ __forceinline__ float value_lp(float x, float m, float logs, float t) {
+    return logs == -INFINITY ? -INFINITY : (x - m) * t - logs;
+}
+
+template <typename T>
+__device__ void finish_row(const LogpP& p, long r, Soft a, const uint32_t* bk, const int* bi) {
+    const float logs = a.s > 0.f || a.s != a.s ? logf(a.s) : -INFINITY;
+    if (threadIdx.x == 0) {
+        const float H = logs == -INFINITY ? 0.f : logs - LN2 * a.w / a.s;
+        const int64_t id = p.ids ? p.ids[r] : -1;
+        const float xid = id >= 0 && id < p.V ? (float)((const T*)p.x)[r * p.ld + id] : 0.f;
+        p.logprob[r] = id >= 0 && id < p.V ? value_lp(xid, a.m, logs, p.t) : 0.f;
+        p.entropy[r] = H;
+        p.lse[r] = logs == -INFINITY ? -INFINITY : a.m * p.t + logs;
+        *(float4*)(p.stats + 4 * r) = make_float4(a.m, logs, H, 0.f);
+    }
+    for (int j = threadIdx.x; j < p.k; j += NT) {
+        p.top_ids[r * p.k + j] = bi[j];
+        p.top_lp[r * p.k + j] = value_lp(key_value(bk[j]), a.m, logs, p.t);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void k_token_logprobs(LogpP p) {
+    __shared__ Shared sh;
+    const long r = blockIdx.x;
+    int set;
+    const Soft a = scan_row((const T*)p.x + r * p.ld, 0, p.V, p.t * LOG2E, p.k, sh, set);
+    finish_row<T>(p, r, a, sh.bk[set], sh.bi[set]);
+}
+
+// Few rows: `splits` workgroups a row, each with its part's sums and its k best; k_token_logprobs_join puts them together.
+template <typename T>
+__global__ __launch_bounds__(NT) void k_token_logprobs_part(LogpP p) {
+    __shared__ Shared sh;
+    const long r = blockIdx.x / p.splits, i = blockIdx.x % p.splits;
+    const long v0 = p.V * i / p.splits, v1 = p.V * (i + 1) / p.splits;
+    int set;
+    const Soft a = scan_row((const T*)p.x + r * p.ld, v0, v1, p.t * LOG2E, p.k, sh, set);
+    float* o = p.part + (long)blockIdx.x * (4 + 2 * p.k);
+    if (threadIdx.x == 0) { o[0] = a.m; o[1] = a.s; o[2] = a.w; }
+    for (int j = threadIdx.x; j < p.k; j += NT) {
+        o[4 + j] = __uint_as_float(sh.bk[set][j]);
+        o[4 + p.k + j] = __int_as_float(sh.bi[set][j]);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void k_token_logprobs_join(LogpP p) {
+    __shared__ uint32_t ck[SMAX * KMAX];
+    __shared__ int ci[SMAX * KMAX];
+    __shared__ uint32_t bk[KMAX];
+    __shared__ int bi[KMAX];
+    __shared__ int n;
+    const long r = blockIdx.x;
+    const float* q = p.part + r * p.splits * (4 + 2 * p.k);
+    Soft a{q[0], q[1], q[2]};
+    uint32_t tau = 0;                                       // the best of the parts' k-th values bounds the row's k-th from below
+    for (int i = 0; i < p.splits; ++i) {
+        const float* o = q + i * (4 + 2 * p.k);
+        if (i) a = soft_join(a, Soft{o[0], o[1], o[2]}, p.t * LOG2E);
+        if (p.k) tau = max(tau, __float_as_uint(o[4 + p.k - 1]));
+    }
+    if (threadIdx.x == 0) n = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < p.splits * p.k; j += NT) {
+        const float* o = q + j / p.k * (4 + 2 * p.k);
+        const uint32_t kk = __float_as_uint(o[4 + j % p.k]);
+        if (kk >= tau) {
+            const int at = atomicAdd(&n, 1);
+            ck[at] = kk;
+            ci[at] = __float_as_int(o[4 + p.k + j % p.k]);
+        }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += NT) {
+        const int rk = rank_of(ck, ci, n, ck[j], ci[j]);
+        if (rk < p.k) { bk[rk] = ck[j]; bi[rk] = ci[j]; }
+    }
+    __syncthreads();
+    finish_row<T>(p, r, a, bk, bi);
+}
+
+// One pass: reads a part of a row, writes its gradient.  The tokens that carry gradients of their own (the given one, the alternatives) are read
+// before the pass and written after it by the part that holds them, each once with all it gets; so dx may be x itself.
+template <typename T>
+__global__ __launch_bounds__(NT) void k_token_logprobs_bwd(LogpP p) {
+    constexpr int VEC = Elem<T>::VEC;
+    __shared__ long sid[KMAX + 1];
+    __shared__ float sg[KMAX + 1];
+    __shared__ float gsum;
+    const int tid = threadIdx.x;
+    const long r = blockIdx.x / p.splits, i = blockIdx.x % p.splits;
+    const long v0 = p.V * i / p.splits, v1 = p.V * (i + 1) / p.splits;
+    const T* row = (const T*)p.x + r * p.ld;
+    T* out = (T*)p.dx + r * p.ldd;
+    const float4 st = *(const float4*)(p.stats + 4 * r);
+    const float m = st.x, logs = st.y, H = st.z, gH = p.dent ? p.dent[r] : 0.f;
+    if (tid <= p.k) {
+        const long id = tid == 0 ? (p.ids ? (long)p.ids[r] : -1) : (long)p.tids[r * p.k + tid - 1];
+        const bool in = id >= 0 && id < p.V;
+        const float* src = tid == 0 ? p.dlp : p.dtop;
+        sid[tid] = in ? id : -1;
+        sg[tid] = in && src ? (tid == 0 ? src[r] : src[r * p.k + tid - 1]) : 0.f;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        float s = 0.f;
+        for (int j = 0; j <= p.k; ++j) s += sg[j];
+        gsum = s;
+    }
+    // this thread's special token, if it is the first of its index and lies in this part
+    long mine = -1;
+    float xm = 0.f, gm = 0.f;
+    if (tid <= p.k && sid[tid] >= v0 && sid[tid] < v1) {
+        mine = sid[tid];
+        for (int j = 0; j <= p.k; ++j)
+            if (sid[j] == mine) {
+                if (j < tid) mine = -1;
+                gm += sg[j];
+                if (mine < 0) break;
+            }
+        if (mine >= 0) xm = (float)row[mine];
+    }
+    __syncthreads();
+    const float A = gsum;
+    const bool none = logs == -INFINITY;
+    auto grad = [&](float x, float g) {
+        const float lp = (x - m) * p.t - logs, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
+        return none ? 0.f : p.t * (g - pr * (A + gH * (fmaxf(lp, -200.f) + H)));     // e^-200 = 0 in fp32: no 0 * inf
+    };
+    const Groups<T> gr(row, v0, v1);
+    const bool same = (((uintptr_t)(out + v0) ^ (uintptr_t)(row + v0)) & 15) == 0;
+    for (long g = tid; g < gr.n; g += NT) {
+        float f[VEC];
+        gr.load(g, f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] = grad(f[j], 0.f);
+        const long e = gr.first + g * VEC;
+        if (same && gr.whole(g)) {
+            st_elems<T, VEC>(out + e, f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (e + j >= v0 && e + j < v1) out[e + j] = (T)f[j];
+        }
+    }
+    __syncthreads();                                        // (orders this workgroup's stores: the special tokens are written last)
+    if (mine >= 0) out[mine] = (T)grad(xm, gm);
+}
+
+int check_common(const dua_token_logprobs_args* a, const char* who) {
+    DUA_REQUIRE(a, "%s: null arguments", who);
+    DUA_REQUIRE(dua_dtype_ok(a->dtype), "%s: dtype must be fp32, bf16 or fp16", who);
+    DUA_REQUIRE(a->rows >= 0 && a->rows < (1L << 24) && a->V >= 1 && a->V < (1L << 31) - 64 && a->ld >= a->V, "%s: rows in [0, 2^24), V in [1, 2^31 - 64), ld >= V", who);
+    DUA_REQUIRE(a->k >= 0 && a->k <= KMAX && a->k <= a->V, "%s: k must be in [0, %d] and at most V", who, KMAX);
+    DUA_REQUIRE(a->inv_temperature > 0.f && a->inv_temperature < INFINITY, "%s: inv_temperature must be positive and finite", who);
+    DUA_REQUIRE(a->rows == 0 || (a->logits && a->stats && ((uintptr_t)a->stats & 15) == 0), "%s: null logits / stats, or stats not 16-byte aligned", who);
+    return DUA_OK;
+}
+
+// Parts of a row: enough workgroups for the chip, at least 4096 elements (more than k) each.
+int plan_splits(long rows, long V) {
+    if (rows >= 256 || rows == 0) return 1;
+    long s = (512 + rows - 1) / rows, most = V / 4096;
+    if (s > most) s = most;
+    if (s > SMAX) s = SMAX;
+    return s < 1 ? 1 : (int)s;
+}
+LogpP pack(const dua_token_logprobs_args* a) {
+    LogpP p{};
+    p.x = a->logits; p.ids = a->ids; p.logprob = a->logprob; p.entropy = a->entropy; p.lse = a->lse; p.stats = a->stats;
+    p.top_ids = a->top_ids; p.top_lp = a->top_logprobs; p.rows = a->rows; p.ld = a->ld; p.V = a->V; p.k = a->k; p.t = a->inv_temperature;
+    return p;
+}
+
+}  // namespace
+
+extern "C" size_t dua_token_logprobs_workspace_bytes(const dua_token_logprobs_args* a) {
+    if (!a || a->rows < 0 || a->V < 1 || a->k < 0) return 0;
+    const int s = plan_splits(a->rows, a->V);
+    return s > 1 ? (size_t)a->rows * s * (4 + 2 * a->k) * sizeof(float) : 0;
+}
+
+extern "C" int dua_token_logprobs(const dua_token_logprobs_args* a, void* stream) {
+    if (int rc = check_common(a, "dua_token_logprobs")) return rc;
+    if (a->rows == 0) return DUA_OK;
+    DUA_REQUIRE(a->logprob && a->entropy && a->lse && (a->k == 0 || (a->top_ids && a->top_logprobs)), "dua_token_logprobs: null output");
+    LogpP p = pack(a);
+    p.splits = plan_splits(a->rows, a->V);
+    p.part = (float*)a->workspace;
+    DUA_REQUIRE(p.splits == 1 || (a->workspace && a->workspace_bytes >= dua_token_logprobs_workspace_bytes(a)),
+                "dua_token_logprobs: workspace smaller than dua_token_logprobs_workspace_bytes");
+    hipStream_t st = as_stream(stream);
+#define GO(T)                                                                                                              \
+    if (p.splits == 1) hipLaunchKernelGGL(k_token_logprobs<T>, (unsigned)p.rows, NT, 0, st, p);                             \
+    else {                                                                                                                  \
+        hipLaunchKernelGGL(k_token_logprobs_part<T>, (unsigned)(p.rows * p.splits), NT, 0, st, p);                          \
+        hipLaunchKernelGGL(k_token_logprobs_join<T>, (unsigned)p.rows, NT, 0, st, p);                                       \
+    }
+    if (a->dtype == DUA_DTYPE_F32) { GO(float) } else if (a->dtype == DUA_DTYPE_BF16) { GO(bf16_t) } else { GO(f16_t) }
+#undef GO
+    return dua_check_launch("dua_token_logprobs");
+}
+
+extern "C" int dua_token_logprobs_bwd(const dua_token_logprobs_args* a, void* stream) {
+    if (int rc = check_common(a, "dua_token_logprobs_bwd")) return rc;
+    if (a->rows == 0) return DUA_OK;
+    DUA_REQUIRE(a->dlogits && a->ldd >= a->V && (!a->dlogprob || a->ids) && (a->k == 0 || (a->dtop && a->top_ids)),
+                "dua_token_logprobs_bwd: null operand (k > 0 needs dtop and top_ids, dlogprob needs ids)");
+    DUA_REQUIRE(a->dlogits != a->logits || a->ldd == a->ld, "dua_token_logprobs_bwd: in place needs one row stride");
+    LogpP p = pack(a);
+    p.dlp = a->dlogprob; p.dent = a->dentropy; p.dtop = a->dtop; p.tids = a->top_ids; p.dx = a->dlogits; p.ldd = a->ldd;
+    long s = (4096 + a->rows - 1) / a->rows;                 // parts of at least 4096 elements, about 4096 workgroups
+    if (s > a->V / 4096) s = a->V / 4096;
+    p.splits = s < 1 ? 1 : (s > 1024 ? 1024 : (int)s);
+    hipStream_t st = as_stream(stream);
+    const unsigned grid = (unsigned)(p.rows * p.splits);
+    if (a->dtype == DUA_DTYPE_F32) hipLaunchKernelGGL(k_token_logprobs_bwd<float>, grid, NT, 0, st, p);
+    else if (a->dtype == DUA_DTYPE_BF16) hipLaunchKernelGGL(k_token_logprobs_bwd<bf16_t>, grid, NT, 0, st, p);
+    else hipLaunchKernelGGL(k_token_logprobs_bwd<f16_t>, grid, NT, 0, st, p);
+    return dua_check_launch("dua_token_logprobs_bwd");
+}

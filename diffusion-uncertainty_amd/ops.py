@@ -1,8 +1,11 @@
 """Tensor-level wrappers over the C ABI (include/dua_hip.h).
 
 torch is used for device memory and the current HIP stream only; every arithmetic step runs in
-libdua_hip.so.  All tensors must be contiguous fp32 (or the stated integer type) on a HIP device.
+libdua_hip.so.  All tensors must be contiguous fp32 (or the stated integer type) on a HIP device; the token operators at the end
+also take bf16 and fp16, and strided views where they say so.
 """
+import collections
+import contextlib
 import ctypes
 import math
 
@@ -10,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import AttnBlockArgs, GemmArgs, ResBlockArgs, UViTBlockArgs, check
+from ._lib import (AttnBlockArgs, GemmArgs, RelAttentionArgs, ResBlockArgs, SandwichNormArgs, TokenLogprobsArgs, UViTBlockArgs, check)
 
 
 def _stream():
@@ -1199,3 +1202,294 @@ def uvit_block(x, skip, B, L, heads, w, precision="fp32", eps=1e-5, want_planes=
     if yp is not None:
         y._dua_planes = yp
     return y
+
+
+# ------------------------------------------------------------------ token operators
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORMS = {None: 0, "rms": 1, "layer": 2}
+
+
+def _token_tensor(t, name, dtypes, shape=None, device=None, contiguous=True):
+    """Checks of an operand of the token operators; contiguous=False asks only for unit stride along the last dimension."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name}: the HIP path needs a GPU tensor (got {getattr(t, 'device', type(t))}); "
+                           "there is no CPU fallback in this package")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name}: on {t.device}, the other operands on {device}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    if not contiguous and t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dimension must have unit stride")
+    return t
+
+
+def _on(device):
+    """The call's device as the current one (kernels launch on ITS current stream), whatever the caller's is."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _a(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+
+
+SandwichNormGrads = collections.namedtuple("SandwichNormGrads", "dx dy dgate dpost_w dpost_b dpre_w dpre_b")
+
+
+def _sandwich_args(x, y, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps):
+    if post not in _NORMS or pre not in _NORMS:
+        raise ValueError("post / pre: None, 'rms' or 'layer'")
+    _token_tensor(x, "x", tuple(_DTYPES))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x: expected [..., D], got {tuple(x.shape)}")
+    D = x.shape[-1]
+    rows = x.numel() // D
+    _token_tensor(y, "y", (x.dtype,), x.shape, x.device)
+    given = [(n, t) for n, t in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)) if t is not None]
+    pt = given[0][1].dtype if given else (gate.dtype if gate is not None else torch.float32)
+    if pt not in (torch.float32, x.dtype):
+        raise TypeError(f"parameters: expected torch.float32 or {x.dtype}, got {pt}")
+    for n, t in given:
+        if (post if n.startswith("post") else pre) is None:
+            raise ValueError(f"{n}: given for a norm that is off")
+        _token_tensor(t, n, (pt,), (D,), x.device)
+    gate_rows = 0
+    if gate is not None:
+        _token_tensor(gate, "gate", (pt,), None, x.device)
+        if gate.shape[-1:] != (D,):
+            raise ValueError(f"gate: expected [D] or [rows, D] with D = {D}, got {tuple(gate.shape)}")
+        gate_rows = gate.numel() // D
+        if gate_rows < 1 or rows % gate_rows:
+            raise ValueError(f"gate: its {gate_rows} rows must divide the {rows} rows of x")
+    return SandwichNormArgs(x=_a(x), y=_a(y), dtype=_DTYPES[x.dtype], param_dtype=_DTYPES[pt], rows=rows, D=D, post=_NORMS[post], pre=_NORMS[pre],
+                            post_w=_a(post_w), post_b=_a(post_b), pre_w=_a(pre_w), pre_b=_a(pre_b), gate=_a(gate), gate_rows=gate_rows,
+                            res_scale=float(res_scale), eps=float(eps))
+
+
+def sandwich_norm(x, y, post="rms", post_w=None, post_b=None, gate=None, res_scale=1.0, pre="rms", pre_w=None, pre_b=None, eps=1e-6,
+                  want_stats=False):
+    """The norms around a transformer block with its gate and residual scale, one pass:
+    r = res_scale * x + gate * post(y) (the stream after a block with output y), z = pre(r) (the next block's input) -> r, z.
+    x, y [..., D]; post / pre: None (post(y) = y; z is None), "rms" or "layer", with weights / shifts [D] or None; gate [D], or [G, D] for the G
+    equal runs of rows of x (a gate per sample, or per token).  Parameters in fp32 or x's type.  want_stats=True: also what the backward
+    pass needs."""
+    a = _sandwich_args(x, y, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps)
+    with _on(x.device):
+        r = torch.empty_like(x)
+        z = torch.empty_like(x) if pre is not None else None
+        stats = torch.empty((a.rows, 4), device=x.device, dtype=torch.float32) if want_stats else None
+        a.r, a.z, a.stats = _a(r), _a(z), _a(stats)
+        check(_lib.lib().dua_sandwich_norm(ctypes.byref(a), _stream()), "dua_sandwich_norm")
+    return (r, z, stats) if want_stats else (r, z)
+
+
+def sandwich_norm_bwd(x, y, stats, dr, dz, post="rms", post_w=None, post_b=None, gate=None, res_scale=1.0, pre="rms", pre_w=None, pre_b=None,
+                      eps=1e-6):
+    """Gradients of sandwich_norm (same arguments, `stats` of the forward call) given those of r and z (dz None without pre) ->
+    SandwichNormGrads; None for what was not given, parameters' gradients in their type."""
+    a = _sandwich_args(x, y, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps)
+    _token_tensor(stats, "stats", (torch.float32,), (a.rows, 4), x.device)
+    _token_tensor(dr, "dr", (x.dtype,), x.shape, x.device)
+    if pre is not None:
+        _token_tensor(dz, "dz", (x.dtype,), x.shape, x.device)
+    elif dz is not None:
+        raise ValueError("dz: given without a pre norm")
+    with _on(x.device):
+        like = lambda t: torch.empty_like(t) if t is not None else None
+        g = SandwichNormGrads(like(x), like(y), like(gate), like(post_w), like(post_b), like(pre_w), like(pre_b))
+        a.stats, a.dr, a.dz, a.dx, a.dy, a.dgate = _a(stats), _a(dr), _a(dz), _a(g.dx), _a(g.dy), _a(g.dgate)
+        a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = _a(g.dpost_w), _a(g.dpost_b), _a(g.dpre_w), _a(g.dpre_b)
+        L = _lib.lib()
+        a.workspace_bytes = L.dua_sandwich_norm_bwd_workspace_bytes(ctypes.byref(a))
+        ws = _workspace(a.workspace_bytes, x.device)
+        a.workspace = _a(ws)
+        check(L.dua_sandwich_norm_bwd(ctypes.byref(a), _stream()), "dua_sandwich_norm_bwd")
+    return g
+
+
+class RelativeBuckets:
+    """Buckets of the relative positions rel = key - query, clipped to [-max_distance, max_distance]: distances below half of a side's buckets have
+    one each, the rest share buckets that grow with the logarithm of the distance, the last one from max_distance on.  bidirectional: a
+    half of the buckets for keys at or before the query, the other half for later ones; otherwise later keys fall into bucket 0.
+    The borders are found by comparing whole numbers: bucket exact + i starts where (n / exact)^steps >= (max_distance / exact)^i."""
+
+    def __init__(self, num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
+        side = num_buckets // 2 if bidirectional else num_buckets
+        exact = side // 2
+        if exact < 1 or (bidirectional and num_buckets % 2) or not exact < max_distance <= 1024:
+            raise ValueError("RelativeBuckets: needs at least two buckets a side (an even number of both) and half a side < max_distance <= 1024")
+        steps, m = side - exact, []
+        for rel in range(-max_distance, max_distance + 1):
+            n = abs(rel) if bidirectional else max(-rel, 0)
+            b = min(n, exact)
+            while exact <= b < side - 1 and n ** steps * exact ** (b + 1 - exact) >= max_distance ** (b + 1 - exact) * exact ** steps:
+                b += 1
+            m.append(b + (side if bidirectional and rel > 0 else 0))
+        self._set(torch.tensor(m, dtype=torch.int32, device=device), num_buckets)
+
+    @classmethod
+    def from_map(cls, bucket_map, num_buckets):
+        """Any assignment: bucket_map int32 [2 R + 1] on the device, entry rel + R the bucket of rel clipped to [-R, R]; entries outside
+        [0, num_buckets) add no bias."""
+        self = cls.__new__(cls)
+        self._set(_token_tensor(bucket_map, "bucket_map", (torch.int32,)), num_buckets)
+        return self
+
+    def _set(self, bucket_map, num_buckets):
+        n = bucket_map.numel()
+        if bucket_map.dim() != 1 or n % 2 == 0 or not 3 <= n <= 2049 or num_buckets < 1:
+            raise ValueError("bucket_map: expected [2 R + 1] with 1 <= R <= 1024, and at least one bucket")
+        self.map, self.radius, self.num_buckets = bucket_map, n // 2, int(num_buckets)
+
+
+def _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart):
+    _token_tensor(q, "q", tuple(_DTYPES), contiguous=False)
+    kv_heads = heads if kv_heads is None else kv_heads
+    if q.dim() != 3 or heads < 1 or kv_heads < 1 or heads % kv_heads or q.shape[2] % heads:
+        raise ValueError(f"q: expected [B, Tq, heads * ch] and kv_heads dividing heads, got {tuple(q.shape)}, {heads}, {kv_heads}")
+    B, Tq, C = q.shape
+    ch = C // heads
+    _token_tensor(k, "k", (q.dtype,), None, q.device, contiguous=False)
+    if k.dim() != 3 or k.shape[0] != B or k.shape[2] != kv_heads * ch:
+        raise ValueError(f"k: expected [{B}, Tk, {kv_heads * ch}], got {tuple(k.shape)}")
+    _token_tensor(v, "v", (q.dtype,), k.shape, q.device, contiguous=False)
+    Tk = k.shape[1]
+    if not isinstance(buckets, RelativeBuckets) or buckets.map.device != q.device:
+        raise ValueError(f"buckets: expected RelativeBuckets on {q.device}")
+    _token_tensor(table, "table", (torch.float32, q.dtype), (buckets.num_buckets, heads), q.device)
+    for n, t in (("klen", klen), ("qstart", qstart)):
+        if t is not None:
+            _token_tensor(t, n, (torch.int32,), (B,), q.device)
+    a = RelAttentionArgs(q=_a(q), k=_a(k), v=_a(v), dtype=_DTYPES[q.dtype], B=B, Tq=Tq, Tk=Tk, heads=heads, kv_heads=kv_heads, ch=ch,
+                         q_batch=q.stride(0), q_row=q.stride(1), k_batch=k.stride(0), k_row=k.stride(1), v_batch=v.stride(0), v_row=v.stride(1),
+                         table=_a(table), table_dtype=_DTYPES[table.dtype], bucket_map=_a(buckets.map), radius=buckets.radius,
+                         num_buckets=buckets.num_buckets, klen=_a(klen), qstart=_a(qstart), causal=int(bool(causal)),
+                         scale=1.0 / math.sqrt(ch) if scale is None else float(scale))
+    return a
+
+
+def rel_attention(q, k, v, table, buckets, heads, kv_heads=None, causal=False, scale=None, klen=None, qstart=None, want_lse=False):
+    """Multi-head attention with a learned relative position bias, fused (neither scores nor bias in HBM):
+    softmax(scale q k^T + table[bucket(j - p_i), h]) v, p_i = qstart[b] + i, over keys j < klen[b] and, if causal, j <= p_i -> [B, Tq, heads * ch].
+    q [B, Tq, heads * ch], k / v [B, Tk, kv_heads * ch] (views with unit stride along the last dimension: thirds of a qkv projection, slots
+    of a cache), head widths up to 128; query head h attends to kv head h // (heads // kv_heads); table [num_buckets, heads] in fp32 or q's
+    type; klen / qstart int32 [B].  A query without keys gives zeros; keys behind klen are not read.  Tq = 1 with qstart = klen - 1
+    is decoding.  want_lse=True: also lse [B, heads, Tq], for the backward pass."""
+    a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
+    with _on(q.device):
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        lse = torch.empty((a.B, heads, a.Tq), device=q.device, dtype=torch.float32) if want_lse else None
+        a.out, a.out_batch, a.out_row, a.lse = _a(out), out.stride(0), out.stride(1), _a(lse)
+        L = _lib.lib()
+        a.workspace_bytes = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 0)
+        ws = _workspace(a.workspace_bytes, q.device)
+        a.workspace = _a(ws)
+        check(L.dua_rel_attention(ctypes.byref(a), _stream()), "dua_rel_attention")
+    return (out, lse) if want_lse else out
+
+
+def rel_attention_bwd(q, k, v, table, buckets, out, lse, dout, heads, kv_heads=None, causal=False, scale=None, klen=None, qstart=None):
+    """Gradients of rel_attention (same arguments, `out` and `lse` of the forward call) given that of out -> dq, dk, dv, dtable (in their
+    operands' types; shared kv heads and the table summed over all that read them; zeros for keys behind klen)."""
+    a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
+    _token_tensor(out, "out", (q.dtype,), q.shape, q.device, contiguous=False)
+    _token_tensor(dout, "dout", (q.dtype,), q.shape, q.device, contiguous=False)
+    _token_tensor(lse, "lse", (torch.float32,), (a.B, heads, a.Tq), q.device)
+    with _on(q.device):
+        new = lambda t: torch.empty(t.shape, device=q.device, dtype=t.dtype)
+        dq, dk, dv, dtable = new(q), new(k), new(v), new(table)
+        a.out, a.out_batch, a.out_row, a.lse = _a(out), out.stride(0), out.stride(1), _a(lse)
+        a.dout, a.dout_batch, a.dout_row = _a(dout), dout.stride(0), dout.stride(1)
+        a.dq, a.dk, a.dv, a.dtable = _a(dq), _a(dk), _a(dv), _a(dtable)
+        a.dq_batch, a.dq_row, a.dk_batch, a.dk_row, a.dv_batch, a.dv_row = (s for t in (dq, dk, dv) for s in t.stride()[:2])
+        L = _lib.lib()
+        a.workspace_bytes = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 1)
+        ws = _workspace(a.workspace_bytes, q.device)
+        a.workspace = _a(ws)
+        check(L.dua_rel_attention_bwd(ctypes.byref(a), _stream()), "dua_rel_attention_bwd")
+    return dq, dk, dv, dtable
+
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprob entropy lse top_ids top_logprobs stats")
+
+
+def _logprob_args(logits, ids, k, inv_temperature):
+    _token_tensor(logits, "logits", tuple(_DTYPES), contiguous=False)
+    if logits.dim() < 2 or logits.shape[-1] < 1:
+        raise ValueError(f"logits: expected [..., V], got {tuple(logits.shape)}")
+    V = logits.shape[-1]
+    try:
+        rows = logits.view(-1, V) if logits.numel() else logits.reshape(0, V)
+    except RuntimeError:
+        raise ValueError("logits: the rows must be evenly spaced") from None
+    ld = rows.stride(0) if rows.shape[0] > 1 else V
+    if rows.shape[0] > 1 and ld < V:
+        raise ValueError("logits: the rows must not overlap")
+    if ids is not None:
+        _token_tensor(ids, "ids", (torch.int64,), logits.shape[:-1], logits.device)
+    if not 0 <= k <= min(64, V):
+        raise ValueError(f"k: expected 0 to min(64, V), got {k}")
+    if not 0.0 < inv_temperature < math.inf:
+        raise ValueError(f"inv_temperature: must be positive and finite, got {inv_temperature}")
+    return TokenLogprobsArgs(logits=_a(logits), dtype=_DTYPES[logits.dtype], rows=rows.shape[0], V=V, ld=ld, ids=_a(ids), k=k,
+                             inv_temperature=float(inv_temperature))
+
+
+def token_logprobs(logits, ids=None, k=0, inv_temperature=1.0):
+    """What a categorical answer is worth, in one pass over the logits [..., V] (rows evenly spaced: a slice of a padded vocabulary is fine), with
+    l = inv_temperature * logits -> TokenLogprobs:
+      logprob [...]            log softmax(l) at ids (int64 [...]; an id outside [0, V), such as -100, gives 0; ids None: zeros)
+      entropy, lse [...]       -sum p log p (the token counterpart of the pixel-wise uncertainty map) and log sum e^l
+      top_ids, top_logprobs    [..., k] (k <= 64): the best alternatives, ties to the lowest index (None for k = 0)
+      stats                    for the backward pass.
+    All but the ids fp32.  A row without a finite logit: logprob = lse = -inf, entropy 0."""
+    a = _logprob_args(logits, ids, k, inv_temperature)
+    lead, dev = logits.shape[:-1], logits.device
+    with _on(dev):
+        new = lambda *s, dtype=torch.float32: torch.empty(s, device=dev, dtype=dtype)
+        o = TokenLogprobs(new(*lead), new(*lead), new(*lead), new(*lead, k, dtype=torch.int64) if k else None, new(*lead, k) if k else None,
+                          new(a.rows, 4))
+        a.logprob, a.entropy, a.lse, a.top_ids, a.top_logprobs, a.stats = (_a(t) for t in o)
+        L = _lib.lib()
+        a.workspace_bytes = L.dua_token_logprobs_workspace_bytes(ctypes.byref(a))
+        ws = _workspace(a.workspace_bytes, dev)
+        a.workspace = _a(ws)
+        check(L.dua_token_logprobs(ctypes.byref(a), _stream()), "dua_token_logprobs")
+    return o
+
+
+def token_logprobs_bwd(logits, ids, saved, dlogprob=None, dentropy=None, dtop=None, inv_temperature=1.0, out=None):
+    """Gradient of token_logprobs' logprob, entropy and top_logprobs (any of them None: no gradient) with respect to the logits; `saved`: the
+    forward call's TokenLogprobs.  out: where to (like logits; logits itself: in place).  Rows without a finite logit get zeros."""
+    k = saved.top_ids.shape[-1] if dtop is not None and saved.top_ids is not None else 0
+    if dtop is not None and not k:
+        raise ValueError("dtop: the forward call kept no alternatives")
+    if dlogprob is not None and ids is None:
+        raise ValueError("dlogprob: needs the ids of the forward call")
+    a = _logprob_args(logits, ids, k, inv_temperature)
+    lead, dev, f32 = logits.shape[:-1], logits.device, (torch.float32,)
+    _token_tensor(saved.stats, "saved.stats", f32, (a.rows, 4), dev)
+    for n, t, s in (("dlogprob", dlogprob, lead), ("dentropy", dentropy, lead), ("dtop", dtop, (*lead, k))):
+        if t is not None:
+            _token_tensor(t, n, f32, s, dev)
+    if k:
+        _token_tensor(saved.top_ids, "saved.top_ids", (torch.int64,), (*lead, k), dev)
+    with _on(dev):
+        if out is None:
+            out = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
+        else:
+            _token_tensor(out, "out", (logits.dtype,), logits.shape, dev, contiguous=False)
+        d = _logprob_args(out, None, 0, 1.0)
+        if out.data_ptr() == logits.data_ptr() and d.ld != a.ld:
+            raise ValueError("out: in place needs the logits' own row stride")
+        a.stats, a.top_ids, a.dlogprob, a.dentropy, a.dtop, a.dlogits, a.ldd = (_a(saved.stats), _a(saved.top_ids) if k else None, _a(dlogprob),
+                                                                                _a(dentropy), _a(dtop), _a(out), d.ld)
+        check(_lib.lib().dua_token_logprobs_bwd(ctypes.byref(a), _stream()), "dua_token_logprobs_bwd")
+    return out

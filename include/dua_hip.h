@@ -10,7 +10,8 @@
  *
  * Conventions
  *  - All pointers are DEVICE pointers (HBM) unless the name ends in _host.
- *  - fp32 everywhere; activations inside the denoiser are NHWC
+ *  - fp32 everywhere, except for the token operators at the end (fp32, bf16 or
+ *    fp16 by a dtype code); activations inside the denoiser are NHWC
  *    ([N][H][W][C], C fastest), NCHW at the sampler edge.
  *  - `stream` is a hipStream_t passed as void* (NULL = default stream).
  *    Calls are asynchronous; nothing allocates, frees or synchronises.
@@ -595,6 +596,96 @@ int dua_place_even(const float* g, float* out, int N, int H, int W, int C, void*
 /* grad[m] = scale * (stack[m] - mean_m stack): d/d e_m of (scale/2) * sum_m (e_m - mean)^2, i.e. of the unbiased variance over
  * M samples summed over pixels and averaged over B samples when scale = 2 / ((M-1) * B) (uncertainty_guidance.py:106-107). */
 int dua_mc_var_grad(const float* stack, float* grad, int M, size_t n, float scale, void* stream);
+
+/* ---------------- token operators: transformers over tokens, their training and their answers ----------------
+ * The pieces a denoiser / language model over TOKENS needs next to the image path above; each with its gradient.  Tensors of one of three
+ * types; sums, softmax statistics and norms in fp32.  Results of a call do not depend on the run (no unordered sums). */
+#define DUA_DTYPE_F32 0
+#define DUA_DTYPE_BF16 1
+#define DUA_DTYPE_F16 2
+
+/* The norms around a block with its gate and residual scale:  u = post(y);  r = res_scale * x + gate * u;  z = pre(r).
+ * x, y, r, z [rows][D] (dtype); post / pre: 0 none (u = y / no z), 1 RMS norm t / sqrt(mean t^2 + eps), 2 LayerNorm; weights and shifts [D]
+ * or NULL (1 / 0); gate [gate_rows][D] or NULL (1): row i takes gate row i / (rows / gate_rows) - one row: a gate per channel, one per sample,
+ * one per token.  Parameters and gate of type param_dtype: fp32 or dtype.  D <= 8192.  stats [rows][4] (mean, 1/std of y and of r; NULL: not
+ * kept) is what the backward pass takes.  r may be x, z may be y. */
+typedef struct {
+    const void *x, *y;
+    int dtype, param_dtype;
+    long rows;
+    int D, post, pre;
+    const void *post_w, *post_b, *pre_w, *pre_b, *gate;
+    long gate_rows;
+    float res_scale, eps;
+    void *r, *z;
+    float* stats;
+    /* backward: gradients of r and z (dz unused without pre) -> of x, y and of the parameters that are given (param_dtype) */
+    const void *dr, *dz;
+    void *dx, *dy, *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+    void* workspace; size_t workspace_bytes;
+} dua_sandwich_norm_args;
+int dua_sandwich_norm(const dua_sandwich_norm_args* args_host, void* stream);
+size_t dua_sandwich_norm_bwd_workspace_bytes(const dua_sandwich_norm_args* args_host);
+/* dr may be dx, dz may be dy. */
+int dua_sandwich_norm_bwd(const dua_sandwich_norm_args* args_host, void* stream);
+
+/* Attention with a learned relative position bias by buckets:
+ *   s_ij = scale q_i . k_j + table[bucket_map[clip(j - p_i, -radius, radius) + radius]][h],  p_i = qstart[b] + i  (qstart NULL: 0),
+ * over keys j < klen[b] (NULL: Tk) and, with causal, j <= p_i;  out = softmax(s) v;  lse [B][heads][Tq] = log sum e^s (NULL: not kept).  A query
+ * without keys gives zeros (lse = -inf).  Keys behind klen are not read.  q, out [B][Tq][heads * ch], k, v [B][Tk][kv_heads * ch] with strides
+ * of their own (elements); query head h reads kv head h / (heads / kv_heads); ch <= 128.  table [num_buckets][heads] (table_dtype: fp32 or
+ * dtype), bucket_map [2 radius + 1]: entries outside [0, num_buckets) add no bias; radius <= 1024.  Tq = 1 is decoding. */
+typedef struct {
+    const void *q, *k, *v;
+    int dtype, B, Tq, Tk, heads, kv_heads, ch;
+    long q_batch, q_row, k_batch, k_row, v_batch, v_row;
+    const void* table;
+    int table_dtype;
+    const int32_t* bucket_map;
+    int radius, num_buckets;
+    const int32_t *klen, *qstart;
+    int causal;
+    float scale;
+    void* out;
+    long out_batch, out_row;
+    float* lse;
+    /* backward: out, lse of the forward call and dout -> dq, dk, dv (zeros behind klen), dtable [num_buckets][heads] (table_dtype) */
+    const void* dout;
+    long dout_batch, dout_row;
+    void *dq, *dk, *dv;
+    long dq_batch, dq_row, dk_batch, dk_row, dv_batch, dv_row;
+    void* dtable;
+    void* workspace; size_t workspace_bytes;
+} dua_rel_attention_args;
+size_t dua_rel_attention_workspace_bytes(const dua_rel_attention_args* args_host, int backward);
+int dua_rel_attention(const dua_rel_attention_args* args_host, void* stream);
+int dua_rel_attention_bwd(const dua_rel_attention_args* args_host, void* stream);
+
+/* Log probabilities of given tokens with entropy and alternatives; l = inv_temperature * logits, logits [rows][V] with row stride ld:
+ *   logprob[i] = l[ids[i]] - lse[i] (an id outside [0, V), or ids NULL: 0 and no gradient), entropy[i] = -sum p log p, lse[i] = log sum e^l,
+ *   top_ids / top_logprobs [rows][k]: the k largest, ties to the lowest index, NaN above every number; k <= 64.
+ * Logits of -inf have probability 0; a row without a finite value gives logprob = lse = -inf, entropy 0 and no gradient; NaN or +inf: NaN.
+ * stats [rows][4] is what the backward pass takes. */
+typedef struct {
+    const void* logits;
+    int dtype;
+    long rows, V, ld;
+    const int64_t* ids;
+    int k;
+    float inv_temperature;
+    float *logprob, *entropy, *lse;
+    int64_t* top_ids;
+    float* top_logprobs;
+    float* stats;
+    /* backward: gradients of logprob, entropy (NULL: none) and, with k > 0, of top_logprobs at top_ids -> dlogits, row stride ldd (may be logits) */
+    const float *dlogprob, *dentropy, *dtop;
+    void* dlogits;
+    long ldd;
+    void* workspace; size_t workspace_bytes;
+} dua_token_logprobs_args;
+size_t dua_token_logprobs_workspace_bytes(const dua_token_logprobs_args* args_host);
+int dua_token_logprobs(const dua_token_logprobs_args* args_host, void* stream);
+int dua_token_logprobs_bwd(const dua_token_logprobs_args* args_host, void* stream);
 
 #ifdef __cplusplus
 }
