@@ -58,7 +58,7 @@ class RelAttentionArgs(_c.Structure):
     _fields_ = [("q", _P), ("k", _P), ("v", _P), ("dtype", _I), ("B", _I), ("Tq", _I), ("Tk", _I), ("heads", _I), ("kv_heads", _I), ("ch", _I),
                 ("q_batch", _L), ("q_row", _L), ("k_batch", _L), ("k_row", _L), ("v_batch", _L), ("v_row", _L),
                 ("table", _P), ("table_dtype", _I), ("bucket_map", _P), ("radius", _I), ("num_buckets", _I), ("klen", _P), ("qstart", _P),
-                ("causal", _I), ("scale", _F), ("out", _P), ("out_batch", _L), ("out_row", _L), ("lse", _P),
+                ("causal", _I), ("scale", _F), ("out", _P), ("out_batch", _L), ("out_row", _L), ("lse", _P), ("out_lo", _P),
                 ("dout", _P), ("dout_batch", _L), ("dout_row", _L), ("dq", _P), ("dk", _P), ("dv", _P),
                 ("dq_batch", _L), ("dq_row", _L), ("dk_batch", _L), ("dk_row", _L), ("dv_batch", _L), ("dv_row", _L),
                 ("dtable", _P), ("workspace", _P), ("workspace_bytes", _Z)]

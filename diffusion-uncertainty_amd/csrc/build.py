@@ -9,7 +9,7 @@ OUT = os.path.join(PKG, "libdua_hip.so")
 SOURCES = [("sampler.hip", ["-ffp-contract=off"]), ("denoiser.hip", []), ("mfma_gemm.hip", []), ("mfma_bf16x3.hip", []), ("conv_f16x3.hip", []), ("gemm_f16x3.hip", []), ("gemm_skip_f16x3.hip", []), ("conv_wino_f16x3.hip", []), ("conv_wino4_f16x3.hip", []), ("conv_wino_f32.hip", []), ("conv_wino4_f32.hip", []), ("attention.hip", []), ("blocks.hip", []), ("backward.hip", [])]
 # no packed fp32 instructions: some of their forms have given wrong results on this part now and then
 SCALAR_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCES += [(s, SCALAR_F32) for s in ("sandwich_norm.hip", "rel_attention.hip", "token_logprobs.hip")]
+SOURCES += [(s, SCALAR_F32) for s in ("sandwich_norm.hip", "rel_attention.hip", "rel_attention_bwd.hip", "token_logprobs.hip")]
 COMMON = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wno-unused-result"]
 
 
@@ -22,7 +22,7 @@ def _stale(target, deps):
 
 def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    hdrs = [os.path.join(HERE, "common.h"), os.path.join(HERE, "dconv.h"), os.path.join(HERE, "wconv.h"), os.path.join(HERE, "hgemm.h"), os.path.join(HERE, "elem.h"), os.path.join(os.path.dirname(PKG), "include", "dua_hip.h")]
+    hdrs = [os.path.join(HERE, "common.h"), os.path.join(HERE, "dconv.h"), os.path.join(HERE, "wconv.h"), os.path.join(HERE, "hgemm.h"), os.path.join(HERE, "elem.h"), os.path.join(HERE, "rel_attention.h"), os.path.join(os.path.dirname(PKG), "include", "dua_hip.h")]
     objs = []
     for src, extra in SOURCES:
         s = os.path.join(HERE, src)
@@ -49,7 +49,7 @@ def build_select_variant(verbose=True):
     out_dir = os.path.join(os.path.dirname(PKG), "scripts", "diag", "build")
     os.makedirs(out_dir, exist_ok=True)
     out = os.path.join(out_dir, "libdua_hip_select.so")
-    hdrs = [os.path.join(HERE, "common.h"), os.path.join(HERE, "dconv.h"), os.path.join(HERE, "wconv.h"), os.path.join(HERE, "hgemm.h"), os.path.join(HERE, "elem.h"), os.path.join(os.path.dirname(PKG), "include", "dua_hip.h")]
+    hdrs = [os.path.join(HERE, "common.h"), os.path.join(HERE, "dconv.h"), os.path.join(HERE, "wconv.h"), os.path.join(HERE, "hgemm.h"), os.path.join(HERE, "elem.h"), os.path.join(HERE, "rel_attention.h"), os.path.join(os.path.dirname(PKG), "include", "dua_hip.h")]
     alt = {}
     for name in ("conv_f16x3.hip", "conv_wino_f16x3.hip", "conv_wino4_f16x3.hip", "conv_wino_f32.hip"):   # (conv_wino4_f32.hip has the out-of-range form only)          # the kernels with row-shifted fragment reads
         src = os.path.join(HERE, name)

@@ -1,0 +1,364 @@
+// Attention with a learned relative position bias by buckets, fused, and its gradients:
+//   s_ij = scale q_i . k_j + table[map[clip(j - p_i, -R, R) + R]][h]   for j < klen_b (causal: and j <= p_i),   p_i = qstart_b + i
+//   P = softmax(s), o = P v, lse_i = log sum_j e^s_ij;   a row without keys: o = 0, lse = -inf, no gradient
+//   dS = P (dO v^T - D), D_i = sum_c dO_ic o_ic;  dq = scale dS k;  dk = scale dS^T q;  dv = P^T dO;  dtable[n][h] = sum of dS where map = n
+// The bias is never materialised: a head's 2R + 1 values lie in LDS (padded so that a tile near the diagonal indexes them without a clamp), and a
+// tile farther than R from the diagonal sees one value.  All products run on 16x16 matrix instructions (K = 32 for sixteen-bit elements; fp32
+// as eight K = 4 steps on the same fragments), softmax and sums in fp32.  Every product is arranged so that its result's columns are the axis the
+// wave owns (queries in the forward and dq passes, keys in the dk / dv pass): scores come out with a query's keys in one lane's registers, and go
+// straight back in as the next product's right operand - P and dS never pass through LDS.  Their key order inside a K = 32 step
+// (16 (j / 4) + 4 (lane / 16) + j % 4) is matched by reading the other operand transposed from its row-major tile.
+// dk / dv and dq are two passes (scores computed twice, 14 instead of 10 products' flops): no atomics, the same bits in every run.
+#pragma once
+#include "elem.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int RMAX = 1024;
+constexpr int NWAVE = 4, NTHR = 64 * NWAVE;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+
+// A fragment covers KSTEP of the summed axis: 32 sixteen-bit elements (8 a lane), 16 fp32 ones (4 a lane).
+template <typename T> struct Frag;
+template <> struct Frag<float> { typedef f32x4 type; static constexpr int N = 4; };
+template <> struct Frag<bf16_t> { typedef bf16x8 type; static constexpr int N = 8; };
+template <> struct Frag<f16_t> { typedef f16x8 type; static constexpr int N = 8; };
+
+// D[16 x 16] += A[16 x 4N] B[4N x 16]: lane l holds A[l % 16][N (l / 16) + j], B[N (l / 16) + j][l % 16], D[4 (l / 16) + r][l % 16].  fp32: four
+// K = 4 instructions, the j-th over the lanes' j-th elements - the order of the summed axis is free as long as A and B agree.
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+constexpr f32x4 ZERO4 = {0.f, 0.f, 0.f, 0.f};
+
+struct AttP {
+    const void *q, *k, *v, *table, *out, *dout, *olo_in;
+    void *o, *olo, *dq, *dk, *dv, *dtable;
+    long qb, qr, kb, kr, vb, vr, ob, orow, db, dr, dqb, dqr, dkb, dkr, dvb, dvr;      // batch and row strides, elements
+    const int32_t *map, *klen, *qstart;
+    float *lse, *dsum, *part, *part_ml;
+    int B, Tq, Tk, H, Hk, ch, R, nb, causal, table_dtype, vec, splits, nblk, swz;
+    float scale;
+};
+
+// Shapes of the tiles of a type and a padded head width (a multiple of 16).
+template <typename T, int CHP> struct Shape {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int KSTEP = 4 * Frag<T>::N, NP = KSTEP / 16;   // summed elements of one product; result tiles that feed one
+    static constexpr int KW = (CHP + KSTEP - 1) / KSTEP * KSTEP, KS = KW / KSTEP, CT = CHP / 16;
+    static constexpr int KT = F32 ? 32 : 64;              // rows of a staged tile
+    static constexpr int NQ = F32 ? 1 : 2;                // 16-query column tiles of a wave: each fragment read from LDS feeds NQ products
+    static constexpr int NK = F32 || CHP > 64 ? 1 : 2;    // 16-key column tiles of a wave in the dk / dv pass (its accumulators are twice as many)
+    static constexpr int QB = 16 * NQ * NWAVE, KB = 16 * NK * NWAVE;
+    static constexpr int PITCH = KW + 16 / (int)sizeof(T);   // elements: 16 rows' 16-byte pieces fall on distinct banks
+    static constexpr int PAD = KT + 16 * NQ;                // bias values beyond +-R that a tile near the diagonal can index
+    static constexpr size_t TILE = (size_t)KT * PITCH * sizeof(T);
+};
+
+// Workgroup -> (batch, kv head, query head, block): the blocks of one kv head stay on one of the eight XCDs (consecutive workgroups go
+// round them), so its keys and values are fetched into one L2 - where there are enough kv heads to fill all eight.
+struct Where { int b, h, hk, blk; };
+__device__ __forceinline__ Where place(const AttP& p, int heads_inner, unsigned id) {
+    const unsigned inner = (unsigned)heads_inner * p.nblk;
+    unsigned unit, in;
+    if (p.swz) {
+        const unsigned x = id & 7, i = id >> 3;
+        unit = x + 8 * (i / inner);
+        in = i % inner;
+    } else {
+        unit = id / inner;
+        in = id % inner;
+    }
+    Where w;
+    w.b = (int)(unit / p.Hk);
+    w.hk = (int)(unit % p.Hk);
+    w.h = w.hk * (p.H / p.Hk) + (int)(in / p.nblk);
+    w.blk = (int)(in % p.nblk);
+    return w;
+}
+
+__device__ __forceinline__ int keys_of(const AttP& p, int b) { return p.klen ? min(max(p.klen[b], 0), p.Tk) : p.Tk; }
+__device__ __forceinline__ int start_of(const AttP& p, int b) { return p.qstart ? min(max(p.qstart[b], -(1 << 30)), 1 << 30) : 0; }
+
+// Bias of head h at clipped distance index i in [0, 2R], in log2 units; a map entry outside [0, nb) adds nothing.
+__device__ __forceinline__ float bias_at(const AttP& p, int h, int i) {
+    const int m = p.map[i];
+    if (m < 0 || m >= p.nb) return 0.f;
+    const long at = (long)m * p.H + h;
+    return LOG2E * (p.table_dtype == DUA_DTYPE_F32 ? ((const float*)p.table)[at]
+                                                   : (p.table_dtype == DUA_DTYPE_BF16 ? (float)((const bf16_t*)p.table)[at] : (float)((const f16_t*)p.table)[at]));
+}
+// lut[rel + R + pad], rel clipped to [-R, R]
+__device__ __forceinline__ void load_lut(const AttP& p, int h, int pad, float* lut) {
+    const int n = 2 * (p.R + pad) + 1;
+    for (int i = threadIdx.x; i < n; i += NTHR) lut[i] = bias_at(p, h, min(max(i - pad, 0), 2 * p.R));
+}
+
+template <typename T> using Vec16 = typename VecOf<T, Elem<T>::VEC>::type;
+
+// 16 bytes of a row at column c, zero at and past ch
+template <typename T>
+__device__ __forceinline__ Vec16<T> load16(const T* row, int c, int ch, bool vec) {
+    constexpr int V = Elem<T>::VEC;
+    Vec16<T> r;
+    if (vec) {
+        if (c < ch) return *(const Vec16<T>*)(row + c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = (T)0.f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = c + j < ch ? row[c + j] : (T)0.f;
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ Vec16<T> zero16() {
+    Vec16<T> r;
+#pragma unroll
+    for (int j = 0; j < Elem<T>::VEC; ++j) r[j] = (T)0.f;
+    return r;
+}
+
+// A lane's part of a fragment from global memory (16 bytes); a row that is not there reads as zeros
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::type row_frag_global(const T* row, int c, int ch, bool vec, bool there) {
+    static_assert(Frag<T>::N == Elem<T>::VEC, "a lane's part of a fragment is 16 bytes");
+    return there ? load16<T>(row, c, ch, vec) : zero16<T>();
+}
+
+// A tile of ROWS rows on its way from global memory through registers to LDS: the loads of the next tile are in flight while the present one
+// is multiplied.  Rows at and past n and the columns past ch are zeros.
+template <typename T, int CHP, int ROWS, int THREADS = NTHR> struct Carrier {
+    static constexpr int V = Elem<T>::VEC, C = Shape<T, CHP>::KW / V, P = Shape<T, CHP>::PITCH, N = (ROWS * C + THREADS - 1) / THREADS;
+    static constexpr bool EVEN = ROWS * C % THREADS == 0;
+    Vec16<T> x[N];
+    __device__ __forceinline__ void fetch(const T* src, long stride, int n, int ch, bool vec, int tid) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int i = tid + u * THREADS, r = i / C, c = i % C * V;
+            x[u] = r < n && (EVEN || r < ROWS) ? load16<T>(src + r * stride, c, ch, vec) : zero16<T>();
+        }
+    }
+    __device__ __forceinline__ void put(T* tile, int tid) const {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int i = tid + u * THREADS, r = i / C, c = i % C * V;
+            if (EVEN || r < ROWS) *(Vec16<T>*)(tile + r * P + c) = x[u];
+        }
+    }
+};
+
+// Fragment of a row-major tile: lane -> row row0 + l % 16, its part of columns c .. c + KSTEP - 1
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::type row_frag(const T* tile, int pitch, int row0, int c, int lane) {
+    return *(const typename Frag<T>::type*)(tile + (row0 + (lane & 15)) * pitch + c + Frag<T>::N * (lane >> 4));
+}
+// The same tile transposed: lane -> column c0 + l % 16, element j -> row row0 + 16 (j / 4) + 4 (l / 16) + j % 4.  Sixteen-bit elements by two
+// transposing LDS reads (each 16-lane group reads a block of 4 rows x 16 columns, a lane gets its column's 4 rows).
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::type col_frag(const T* tile, int pitch, int row0, int c0, int lane) {
+    typename Frag<T>::type f;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = tile[(row0 + 4 * (lane >> 4) + j) * pitch + c0 + (lane & 15)];
+    } else {
+        typedef short s4 __attribute__((__vector_size__(8)));
+        const T* a = tile + (row0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * pitch + c0 + 4 * (lane & 3);
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)a);
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(a + 16 * pitch));
+        struct { s4 lo, hi; } pr{x, y};
+        __builtin_memcpy(&f, &pr, 16);
+    }
+    return f;
+}
+// NP result tiles as the right operand of the next product
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::type acc_frag(const f32x4* a) {
+    if constexpr (sizeof(T) == 4) {
+        return a[0];
+    } else {
+        typename Frag<T>::type f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { f[j] = (T)a[0][j]; f[4 + j] = (T)a[1][j]; }
+        return f;
+    }
+}
+
+// four consecutive channels of a row
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int c, int ch, bool vec, f32x4 v) {
+    if (vec) {
+        if (c < ch) {
+            typename VecOf<T, 4>::type x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = (T)v[j];
+            *(typename VecOf<T, 4>::type*)(row + c) = x;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < ch) row[c + j] = (T)v[j];
+    }
+}
+// what the rounding to T left of v
+template <typename T>
+__device__ __forceinline__ f32x4 rest4(f32x4 v) {
+    f32x4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = v[j] - (float)(T)v[j];
+    return r;
+}
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// max / sum over the four lanes that share a column
+__device__ __forceinline__ float col_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float col_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// Where a tile of keys [k0, k0 + n) lies for queries at positions [pmin, pmax]: -1 / 1: all of it at least R to the left / right (one bias value), 0: near.
+__device__ __forceinline__ int side_of(int k0, int n, int pmin, int pmax, int R) { return k0 + n - 1 - pmin <= -R ? -1 : (k0 - pmax >= R ? 1 : 0); }
+
+// ... the scores of N16 result tiles (rows: keys k0 + 16 n + 4 (l / 16) + r; column: a query at pos) become log2 logits: raw * sl + bias,
+// places past nk or (causal) past pos -inf.  lut points at distance 0.
+template <int N16>
+__device__ __forceinline__ void bias_mask(f32x4* s, float sl, const float* lut, int side, float b, bool masked, int k0, int nk, int pos, bool causal, int lane) {
+    const int key = k0 + 4 * (lane >> 4);
+    if (side) {
+#pragma unroll
+        for (int n = 0; n < N16; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[n][r] = s[n][r] * sl + b;
+    } else {
+        const float* l = lut + (key - pos);
+#pragma unroll
+        for (int n = 0; n < N16; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[n][r] = s[n][r] * sl + l[16 * n + r];
+    }
+    if (masked) {
+#pragma unroll
+        for (int n = 0; n < N16; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int kk = key + 16 * n + r;
+                if (kk >= nk || (causal && kk > pos)) s[n][r] = -INFINITY;
+            }
+    }
+}
+
+template <int N16>
+__device__ __forceinline__ float max_of(const f32x4* s) {
+    float m = s[0][0];
+#pragma unroll
+    for (int n = 0; n < N16; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = fmaxf(m, s[n][r]);
+    return m;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------- host
+[[maybe_unused]] static int check_common(const dua_rel_attention_args* a, const char* who) {
+    DUA_REQUIRE(a, "%s: null arguments", who);
+    DUA_REQUIRE(dua_dtype_ok(a->dtype) && dua_dtype_ok(a->table_dtype) && (a->table_dtype == DUA_DTYPE_F32 || a->table_dtype == a->dtype),
+                "%s: dtype must be fp32, bf16 or fp16 and the table's fp32 or the same", who);
+    DUA_REQUIRE(a->B >= 0 && a->Tq >= 0 && a->Tk >= 0 && a->Tq < (1 << 29) && a->Tk < (1 << 29), "%s: lengths must be in [0, 2^29)", who);
+    DUA_REQUIRE(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0, "%s: kv_heads must divide heads", who);
+    DUA_REQUIRE(a->ch >= 1 && a->ch <= 128, "%s: head width must be in [1, 128]", who);
+    DUA_REQUIRE(a->radius >= 1 && a->radius <= RMAX && a->num_buckets >= 1, "%s: radius must be in [1, %d]", who, RMAX);
+    DUA_REQUIRE(a->table && a->bucket_map, "%s: null table / bucket map", who);
+    DUA_REQUIRE((a->B == 0 || a->Tq == 0 || a->q) && (a->B == 0 || a->Tk == 0 || (a->k && a->v)), "%s: null operand", who);
+    DUA_REQUIRE((long)a->B * a->heads * ((a->Tq > a->Tk ? a->Tq : a->Tk) / 64 + 1) < (1L << 23), "%s: too many blocks for one launch", who);
+    return DUA_OK;
+}
+
+// 16-byte accesses everywhere: widths, strides and addresses in whole 16 bytes
+struct Align {
+    size_t bits = 0;
+    void ptr(const void* q) { bits |= (uintptr_t)q; }
+    void str(long s, size_t es) { bits |= (size_t)s * es; }
+    bool ok() const { return (bits & 15) == 0; }
+};
+
+[[maybe_unused]] static AttP pack(const dua_rel_attention_args* a, bool bwd) {
+    AttP p{};
+    p.q = a->q; p.k = a->k; p.v = a->v; p.table = a->table; p.o = a->out; p.out = a->out; p.olo = a->out_lo; p.olo_in = a->out_lo; p.dout = a->dout;
+    p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.dtable = a->dtable;
+    p.qb = a->q_batch; p.qr = a->q_row; p.kb = a->k_batch; p.kr = a->k_row; p.vb = a->v_batch; p.vr = a->v_row; p.ob = a->out_batch; p.orow = a->out_row;
+    p.db = a->dout_batch; p.dr = a->dout_row; p.dqb = a->dq_batch; p.dqr = a->dq_row; p.dkb = a->dk_batch; p.dkr = a->dk_row; p.dvb = a->dv_batch; p.dvr = a->dv_row;
+    p.map = a->bucket_map; p.klen = a->klen; p.qstart = a->qstart; p.lse = a->lse;
+    p.B = a->B; p.Tq = a->Tq; p.Tk = a->Tk; p.H = a->heads; p.Hk = a->kv_heads; p.ch = a->ch; p.R = a->radius; p.nb = a->num_buckets;
+    p.causal = a->causal != 0; p.table_dtype = a->table_dtype; p.scale = a->scale;
+    const size_t es = dua_dtype_size(a->dtype);
+    Align al;
+    al.bits |= (size_t)a->ch * es;
+    al.ptr(a->q); al.ptr(a->k); al.ptr(a->v); al.ptr(a->out);
+    for (long s : {p.qb, p.qr, p.kb, p.kr, p.vb, p.vr, p.ob, p.orow}) al.str(s, es);
+    if (bwd) {
+        al.ptr(a->dout); al.ptr(a->dq); al.ptr(a->dk); al.ptr(a->dv);
+        for (long s : {p.db, p.dr, p.dqb, p.dqr, p.dkb, p.dkr, p.dvb, p.dvr}) al.str(s, es);
+    }
+    p.vec = al.ok();
+    return p;
+}
+
+[[maybe_unused]] static unsigned grid_of(AttP& p, int heads_inner, int nblk) {
+    p.nblk = nblk;
+    const long units = (long)p.B * p.Hk, inner = (long)heads_inner * nblk;
+    // eight XCDs: only where a last, partly filled round of kv heads does not leave them unevenly loaded
+    p.swz = units % 8 == 0 || units >= 64;
+    return (unsigned)((p.swz ? (units + 7) / 8 * 8 : units) * inner);
+}
+
+[[maybe_unused]] static int chp_of(int ch) { return ch <= 32 ? 32 : ch <= 64 ? 64 : ch <= 80 ? 80 : ch <= 96 ? 96 : 128; }
+[[maybe_unused]] static int query_block(int dtype) { return (dtype == DUA_DTYPE_F32 ? 16 : 32) * NWAVE; }        // Shape::QB
+[[maybe_unused]] static int key_block(int dtype, int ch) { return (dtype == DUA_DTYPE_F32 || chp_of(ch) > 64 ? 16 : 32) * NWAVE; }   // Shape::KB
+
+// Workspace of the backward pass: D of every row, the diagonal sums of every block of keys and head.
+[[maybe_unused]] static size_t rel_attention_bwd_bytes(const dua_rel_attention_args* a) {
+    const size_t rows = (size_t)a->B * a->heads * a->Tq, nkb = (a->Tk + key_block(a->dtype, a->ch) - 1) / key_block(a->dtype, a->ch);
+    return (rows + a->B * nkb * a->heads * (2 * a->radius + 1)) * sizeof(float);
+}
+
+// Launch with `lds` bytes of dynamic LDS (more than 64 KB, wide radii with wide fp32 heads, have to be asked for)
+template <typename... A>
+int launch(void (*kernel)(A...), const char* what, dim3 grid, unsigned block, size_t lds, hipStream_t st, A... args) {
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) {
+            dua_set_error("%s: %s", what, hipGetErrorString(e));
+            return DUA_EHIP;
+        }
+    }
+    hipLaunchKernelGGL(kernel, grid, block, lds, st, args...);
+    return dua_check_launch(what);
+}
+
+template <template <typename, int> class L>
+int dispatch(int dtype, const AttP& p, bool few, hipStream_t st) {
+#define GO(T)                                             \
+    switch (chp_of(p.ch)) {                               \
+        case 32: return L<T, 32>::run(p, few, st);        \
+        case 64: return L<T, 64>::run(p, few, st);        \
+        case 80: return L<T, 80>::run(p, few, st);        \
+        case 96: return L<T, 96>::run(p, few, st);        \
+        default: return L<T, 128>::run(p, few, st);       \
+    }
+    if (dtype == DUA_DTYPE_F32) { GO(float) } else if (dtype == DUA_DTYPE_BF16) { GO(bf16_t) } else { GO(f16_t) }
+#undef GO
+}
+
+}  // namespace

@@ -1,0 +1,400 @@
+// Gradients of attention with a bucketed relative bias (rel_attention.h): dq with the table's diagonal sums, dk and dv, the table.
+#include "rel_attention.h"
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------------------------ diagonals
+// Sums along the diagonals of a 16 x 16 block x (row 4 g + r, column c of lane 16 g + c): lane (g, c) of `a` collects diagonal row - column =
+// 4 g - c, of `b` (c >= 13) diagonal 4 g + 16 - c.  A lane's four rows are shifted along its 16 columns, zeros coming in.
+template <int CTRL> __device__ __forceinline__ float dpp_in(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ void diagonals(f32x4 x, float& a, float& b) {
+    a = x[0] + dpp_in<0x101>(x[1]) + dpp_in<0x102>(x[2]) + dpp_in<0x103>(x[3]);      // row_shl: from the column 1, 2, 3 to the right
+    b = dpp_in<0x11F>(x[1]) + dpp_in<0x11E>(x[2]) + dpp_in<0x11D>(x[3]);              // row_shr by 15, 14, 13: what left the row there
+}
+
+// The four waves' sums along the diagonals (diag [wave][nl], distance 0 at R + pad) clipped to 2R + 1 distances, into this workgroup's row of the
+// partial sums; then zeros again.
+__device__ __forceinline__ void flush_diagonals(float* diag, int nl, int R, int pad, float far_lo, float far_hi, float* out) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    far_lo = wave_sum(far_lo);
+    far_hi = wave_sum(far_hi);
+    if (lane == 0) {
+        diag[wave * nl] += far_lo;
+        diag[wave * nl + nl - 1] += far_hi;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i <= 2 * R; i += NTHR) {
+        const int lo = i == 0 ? 0 : i + pad, hi = i == 2 * R ? nl - 1 : i + pad;
+        float t = 0.f;
+        for (int j = lo; j <= hi; ++j)
+#pragma unroll
+            for (int x = 0; x < NWAVE; ++x) t += diag[x * nl + j];
+        out[i] = t;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < NWAVE * nl; i += NTHR) diag[i] = 0.f;
+}
+
+// ------------------------------------------------------------------------------------------------------------------------ dq
+template <typename T, int CHP>
+__global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
+    typedef Shape<T, CHP> S;
+    typedef typename Frag<T>::type frag;
+    constexpr int KT = S::KT, NQ = S::NQ, KS = S::KS, CT = S::CT, P = S::PITCH, NP = S::NP;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    T* const tiles = (T*)smem;                                             // [2][K, V]
+    float* const lut = (float*)(smem + 4 * S::TILE);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const Where w = place(p, p.H / p.Hk, blockIdx.x);
+    if (w.b >= p.B) return;
+    const int blk = p.causal ? p.nblk - 1 - w.blk : w.blk;
+    const int q0 = blk * S::QB, nk = keys_of(p, w.b), qs = start_of(p, w.b);
+    const bool vec = p.vec;
+    const int kend = p.causal ? max(0, min(nk, qs + min(q0 + S::QB, p.Tq))) : nk;
+    const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
+    const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
+    Carrier<T, CHP, KT> ck, cv;
+    if (kend > 0) {
+        ck.fetch(kp, p.kr, nk, p.ch, vec, tid);
+        cv.fetch(vp, p.vr, nk, p.ch, vec, tid);
+    }
+    load_lut(p, w.h, S::PAD, lut);
+    const int qw = q0 + wave * 16 * NQ, pmin = qs + qw, pmax = pmin + 16 * NQ - 1;
+    const T* qp = (const T*)p.q + w.b * p.qb + (long)w.h * p.ch;
+    const T* op = (const T*)p.out + w.b * p.ob + (long)w.h * p.ch;
+    const T* dp = (const T*)p.dout + w.b * p.db + (long)w.h * p.ch;
+    const long row0 = ((long)w.b * p.H + w.h) * p.Tq;
+    frag qf[NQ][KS], df[NQ][KS];
+    float ls[NQ], D[NQ], rest[NQ];
+    f32x4 a[NQ][CT];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const int q = qw + 16 * i + (lane & 15);
+        const bool there = q < p.Tq;
+        float d = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int c = S::KSTEP * s + Frag<T>::N * g;
+            qf[i][s] = row_frag_global<T>(qp + q * p.qr, c, p.ch, vec, there);
+            df[i][s] = row_frag_global<T>(dp + q * p.dr, c, p.ch, vec, there);
+            const frag of = row_frag_global<T>(op + q * p.orow, c, p.ch, vec, there);
+            frag lo = zero16<T>();                                          // the output's rounding: D's error would be the gradients' largest
+            if (sizeof(T) == 2 && p.olo_in) lo = row_frag_global<T>((const T*)p.olo_in + (row0 + q) * p.ch, c, p.ch, (p.ch & 7) == 0, there);
+#pragma unroll
+            for (int j = 0; j < Frag<T>::N; ++j) d += (float)df[i][s][j] * ((float)of[j] + (float)lo[j]);
+        }
+        D[i] = col_sum(d);
+        ls[i] = there ? p.lse[row0 + q] * LOG2E : INFINITY;
+        if (ls[i] == -INFINITY) ls[i] = INFINITY;                          // a row without keys: P = 0
+        rest[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) a[i][c] = ZERO4;
+    }
+    const float sl = p.scale * LOG2E;
+    __syncthreads();
+    const float flo = lut[0], fhi = lut[2 * (p.R + S::PAD)], *lut0 = lut + p.R + S::PAD;
+    for (int k0 = 0, t = 0; k0 < kend; k0 += KT, ++t) {
+        T* const Kt = tiles + (t & 1) * 2 * KT * P;
+        T* const Vt = Kt + KT * P;
+        ck.put(Kt, tid);
+        cv.put(Vt, tid);
+        __syncthreads();
+        if (k0 + KT < kend) {
+            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, nk - k0 - KT, p.ch, vec, tid);
+            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, nk - k0 - KT, p.ch, vec, tid);
+        }
+        if (qw >= p.Tq) continue;
+        // steps of 16 NP keys: scores, dP, dS, and dS straight into dq - few registers live
+        for (int n0 = 0; n0 < KT / 16; n0 += NP) {
+            const int ks0 = k0 + 16 * n0;
+            if (ks0 >= kend || (p.causal && ks0 > pmax)) break;
+            f32x4 s[NQ][NP], d[NQ][NP];
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) { s[i][n] = ZERO4; d[i][n] = ZERO4; }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const frag x = row_frag<T>(Kt, P, 16 * (n0 + n), S::KSTEP * ks, lane), y = row_frag<T>(Vt, P, 16 * (n0 + n), S::KSTEP * ks, lane);
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        s[i][n] = mma(x, qf[i][ks], s[i][n]);
+                        d[i][n] = mma(y, df[i][ks], d[i][n]);
+                    }
+                }
+            }
+            const int side = side_of(ks0, 16 * NP, pmin, pmax, p.R);
+            const bool masked = ks0 + 16 * NP > nk || (p.causal && ks0 + 16 * NP - 1 > pmin);
+            frag pf[NQ];
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                bias_mask<NP>(s[i], sl, lut0, side, side < 0 ? flo : fhi, masked, ks0, nk, pmin + 16 * i + (lane & 15), p.causal, lane);
+                f32x4 e[NP];
+#pragma unroll
+                for (int n = 0; n < NP; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float x = exp2_raw(s[i][n][r] - ls[i]);
+                        s[i][n][r] = masked && x == 0.f ? 0.f : x * (d[i][n][r] - D[i]);   // (masked places may hold anything)
+                        rest[i] += s[i][n][r];
+                        e[n][r] = s[i][n][r] * p.scale;
+                    }
+                pf[i] = acc_frag<T>(e);
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                const frag x = col_frag<T>(Kt, P, 16 * n0, 16 * c, lane);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) a[i][c] = mma(x, pf[i], a[i][c]);
+            }
+        }
+    }
+    T* gp = (T*)p.dq + w.b * p.dqb + (long)w.h * p.ch;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const int q = qw + 16 * i + (lane & 15);
+        // sum_j dS_ij is 0 for the exact D: what is left is D's error (the output came from P rounded for its product, and was rounded itself).
+        // dk and the table take the corrected value - the table's sums cancel to little, it would be their largest error.
+        const float dt = D[i] + col_sum(rest[i]);
+        if (q >= p.Tq) continue;
+        if (g == 0) p.dsum[row0 + q] = dt;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) store4<T>(gp + q * p.dqr, 16 * c + 4 * g, p.ch, vec, a[i][c]);
+    }
+}
+
+// dtable[n][h]: the workgroups' diagonal sums of head h in their order, then the diagonals of each bucket.
+template <typename TT>
+__global__ __launch_bounds__(1024) void k_rel_attention_dtable(AttP p, int nparts) {
+    __shared__ float sum[2 * RMAX + 1];
+    const int h = blockIdx.x, nd = 2 * p.R + 1;
+    for (int i = threadIdx.x; i < nd; i += 1024) {
+        float t = 0.f;
+        for (int j = 0; j < nparts; ++j) t += p.part[((long)j * p.H + h) * nd + i];
+        sum[i] = t;
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < p.nb; n += 1024) {
+        float t = 0.f;
+        for (int i = 0; i < nd; ++i) t += p.map[i] == n ? sum[i] : 0.f;
+        ((TT*)p.dtable)[(long)n * p.H + h] = (TT)t;
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------------------- dk, dv
+template <typename T, int CHP>
+__global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
+    typedef Shape<T, CHP> S;
+    typedef typename Frag<T>::type frag;
+    constexpr int QT = S::KT, NK = S::NK, KS = S::KS, CT = S::CT, P = S::PITCH, NP = S::NP;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    T* const tiles = (T*)smem;                                             // [2][Q, dO]
+    float* const rows = (float*)(smem + 4 * S::TILE);                       // [2][lse, D][QT]
+    float* const lut = rows + 4 * QT;
+    const int nl = 2 * (p.R + S::PAD) + 1;
+    float* const diag = lut + nl;                                          // [wave][nl]: a head's sums of dS along the diagonals
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    const Where w = place(p, 1, blockIdx.x);
+    if (w.b >= p.B) return;
+    const int k0 = w.blk * S::KB, nk = keys_of(p, w.b), qs = start_of(p, w.b);
+    const bool vec = p.vec;
+    const int kw = k0 + wave * 16 * NK;
+    const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
+    const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
+    frag kf[NK][KS], vf[NK][KS];
+    f32x4 ak[NK][CT], av[NK][CT];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+        const int kk = kw + 16 * i + (lane & 15);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int c = S::KSTEP * s + Frag<T>::N * g;
+            kf[i][s] = row_frag_global<T>(kp + kk * p.kr, c, p.ch, vec, kk < nk);
+            vf[i][s] = row_frag_global<T>(vp + kk * p.vr, c, p.ch, vec, kk < nk);
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) { ak[i][c] = ZERO4; av[i][c] = ZERO4; }
+    }
+    const float sl = p.scale * LOG2E;
+    const int rep = p.H / p.Hk;
+    // tiles of queries that see this block's first key (position >= k0), head after head of the group
+    const int qbeg = p.causal ? max(0, k0 - qs) / QT : 0, per = max(0, (p.Tq + QT - 1) / QT - qbeg), total = k0 < nk ? per * rep : 0;
+    Carrier<T, CHP, QT> cq, cd;
+    float row_next = 0.f;
+    auto fetch = [&](int t) {
+        const int h = w.hk * rep + t / per, q0 = (qbeg + t % per) * QT;
+        cq.fetch((const T*)p.q + w.b * p.qb + (long)h * p.ch + (long)q0 * p.qr, p.qr, p.Tq - q0, p.ch, vec, tid);
+        cd.fetch((const T*)p.dout + w.b * p.db + (long)h * p.ch + (long)q0 * p.dr, p.dr, p.Tq - q0, p.ch, vec, tid);
+        if (tid < 2 * QT) {
+            const int q = q0 + tid % QT;
+            const float* src = tid < QT ? p.lse : p.dsum;
+            row_next = q < p.Tq ? src[((long)w.b * p.H + h) * p.Tq + q] : (tid < QT ? -INFINITY : 0.f);
+        }
+    };
+    for (int i = tid; i < NWAVE * nl; i += NTHR) diag[i] = 0.f;
+    float far_lo = 0.f, far_hi = 0.f;
+    float* const part = p.part + (((long)w.b * p.nblk + w.blk) * p.H + w.hk * rep) * (2 * p.R + 1);
+    if (total > 0) fetch(0);
+    for (int t = 0; t < total; ++t) {
+        if (t % per == 0) {
+            __syncthreads();                                                // (the last head's bias is read until here)
+            if (t > 0) flush_diagonals(diag, nl, p.R, S::PAD, far_lo, far_hi, part + (t / per - 1) * (2 * p.R + 1));
+            far_lo = far_hi = 0.f;
+            load_lut(p, w.hk * rep + t / per, S::PAD, lut);
+        }
+        T* const Qt = tiles + (t & 1) * 2 * QT * P;
+        T* const Dt = Qt + QT * P;
+        float* const row_ls = rows + (t & 1) * 2 * QT, *const row_d = row_ls + QT;
+        cq.put(Qt, tid);
+        cd.put(Dt, tid);
+        if (tid < QT) row_ls[tid] = row_next == -INFINITY ? INFINITY : row_next * LOG2E;   // no keys, no query: P = 0
+        else if (tid < 2 * QT) row_ls[tid] = row_next;
+        __syncthreads();
+        if (t + 1 < total) fetch(t + 1);
+        const int q0 = (qbeg + t % per) * QT;
+        if (kw >= nk) continue;
+        const float flo = lut[0], fhi = lut[2 * (p.R + S::PAD)], *lut0 = lut + p.R + S::PAD;
+        for (int n0 = 0; n0 < QT / 16; n0 += NP) {
+            const int qq = q0 + 16 * n0, pmin = qs + qq, pmax = pmin + 16 * NP - 1;
+            if (qq >= p.Tq) break;
+            if (p.causal && kw > pmax) continue;
+            f32x4 s[NK][NP], d[NK][NP];
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+#pragma unroll
+                for (int i = 0; i < NK; ++i) { s[i][n] = ZERO4; d[i][n] = ZERO4; }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const frag x = row_frag<T>(Qt, P, 16 * (n0 + n), S::KSTEP * ks, lane), y = row_frag<T>(Dt, P, 16 * (n0 + n), S::KSTEP * ks, lane);
+#pragma unroll
+                    for (int i = 0; i < NK; ++i) {
+                        s[i][n] = mma(x, kf[i][ks], s[i][n]);
+                        d[i][n] = mma(y, vf[i][ks], d[i][n]);
+                    }
+                }
+            }
+            const int side = side_of(kw, 16 * NK, pmin, pmax, p.R);
+            const bool masked = kw + 16 * NK > nk || (p.causal && kw + 16 * NK - 1 > pmin);
+            const float b = side < 0 ? flo : fhi;
+            frag pf[NK], sf[NK];
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                const int key = kw + 16 * i + (lane & 15);
+                const float* lp = side ? lut0 : lut0 + (key - pmin - 4 * g);
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    const f32x4 L = *(const f32x4*)(row_ls + 16 * (n0 + n) + 4 * g), Dr = *(const f32x4*)(row_d + 16 * (n0 + n) + 4 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int qi = 16 * n + 4 * g + r;
+                        float e = exp2_raw(s[i][n][r] * sl + ((side ? b : lp[-16 * n - r]) - L[r]));
+                        if (masked && (key >= nk || (p.causal && key > pmin + qi))) e = 0.f;
+                        s[i][n][r] = e;
+                        d[i][n][r] = masked && e == 0.f ? 0.f : e * (d[i][n][r] - Dr[r]);
+                    }
+                }
+                pf[i] = acc_frag<T>(s[i]);
+            }
+            if (side) {
+                float tot = 0.f;
+#pragma unroll
+                for (int i = 0; i < NK; ++i)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) tot += (d[i][n][0] + d[i][n][1]) + (d[i][n][2] + d[i][n][3]);
+                if (side < 0) far_lo += tot;
+                else far_hi += tot;
+            } else {
+                // blocks with the same i - n share their diagonals; block dd's `b` diagonals are block dd - 1's `a` diagonals
+                float keep = 0.f;
+                float* dg = diag + wave * nl + (kw + (lane & 15) - pmin - 4 * g + p.R + S::PAD);
+#pragma unroll
+                for (int dd = NK - 1; dd >= -NP; --dd) {
+                    float x = keep;
+                    if (dd > -NP) {
+                        f32x4 z = ZERO4;
+#pragma unroll
+                        for (int n = 0; n < NP; ++n)
+                            if (dd + n >= 0 && dd + n < NK) z += d[dd + n][n];
+                        float a, bb;
+                        diagonals(z, a, bb);
+                        x += a;
+                        keep = bb;
+                    }
+                    // a group's 16 lanes hit 16 places, the groups go one after the other: the order of a wave's sums is fixed
+#pragma unroll
+                    for (int gg = 0; gg < 4; ++gg)
+                        if (g == gg) atomicAdd(dg + 16 * dd, x);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+#pragma unroll
+                for (int n = 0; n < NP; ++n) d[i][n] *= p.scale;
+                sf[i] = acc_frag<T>(d[i]);
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                const frag x = col_frag<T>(Dt, P, 16 * n0, 16 * c, lane), y = col_frag<T>(Qt, P, 16 * n0, 16 * c, lane);
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    av[i][c] = mma(x, pf[i], av[i][c]);
+                    ak[i][c] = mma(y, sf[i], ak[i][c]);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (total > 0) {
+        flush_diagonals(diag, nl, p.R, S::PAD, far_lo, far_hi, part + (rep - 1) * (2 * p.R + 1));
+    } else {
+        for (int i = tid; i < rep * (2 * p.R + 1); i += NTHR) part[i] = 0.f;
+    }
+    T* gk = (T*)p.dk + w.b * p.dkb + (long)w.hk * p.ch;
+    T* gv = (T*)p.dv + w.b * p.dvb + (long)w.hk * p.ch;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+        const int kk = kw + 16 * i + (lane & 15);
+        if (kk >= p.Tk) continue;                                          // keys behind klen: zeros
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            store4<T>(gk + kk * p.dkr, 16 * c + 4 * g, p.ch, vec, ak[i][c]);
+            store4<T>(gv + kk * p.dvr, 16 * c + 4 * g, p.ch, vec, av[i][c]);
+        }
+    }
+}
+
+template <typename T, int CHP> struct Bwd {
+    static int run(AttP p, bool, hipStream_t st) {
+        typedef Shape<T, CHP> S;
+        const int nqb = (p.Tq + S::QB - 1) / S::QB, nl = 2 * (p.R + S::PAD) + 1;
+        if (p.B > 0 && nqb > 0) {
+            const unsigned grid = grid_of(p, p.H / p.Hk, nqb);
+            if (int rc = launch(k_rel_attention_dq<T, CHP>, "dua_rel_attention_bwd", dim3(grid), NTHR, 4 * S::TILE + nl * sizeof(float), st, p)) return rc;
+        }
+        if (p.B > 0 && p.Tk > 0) {
+            const unsigned grid = grid_of(p, 1, (p.Tk + S::KB - 1) / S::KB);
+            if (int rc = launch(k_rel_attention_dkv<T, CHP>, "dua_rel_attention_bwd", dim3(grid), NTHR, 4 * S::TILE + (4 * S::KT + (1 + NWAVE) * nl) * sizeof(float), st, p)) return rc;
+        }
+        const int nparts = p.B * ((p.Tk + S::KB - 1) / S::KB);
+        if (p.table_dtype == DUA_DTYPE_F32) return launch(k_rel_attention_dtable<float>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p, nparts);
+        if (p.table_dtype == DUA_DTYPE_BF16) return launch(k_rel_attention_dtable<bf16_t>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p, nparts);
+        return launch(k_rel_attention_dtable<f16_t>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p, nparts);
+    }
+};
+
+}  // namespace
+
+extern "C" int dua_rel_attention_bwd(const dua_rel_attention_args* a, void* stream) {
+    if (int rc = check_common(a, "dua_rel_attention_bwd")) return rc;
+    DUA_REQUIRE(a->dtable, "dua_rel_attention_bwd: null dtable");
+    DUA_REQUIRE(a->B == 0 || a->Tq == 0 || (a->out && a->lse && a->dout && a->dq), "dua_rel_attention_bwd: null operand");
+    DUA_REQUIRE(a->B == 0 || a->Tk == 0 || (a->dk && a->dv), "dua_rel_attention_bwd: null output");
+    const size_t need = rel_attention_bwd_bytes(a);
+    DUA_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), "dua_rel_attention_bwd: workspace smaller than dua_rel_attention_workspace_bytes");
+    AttP p = pack(a, true);
+    p.dsum = (float*)a->workspace;
+    p.part = p.dsum + (size_t)a->B * a->heads * a->Tq;
+    return dispatch<Bwd>(a->dtype, p, false, as_stream(stream));
+}

@@ -1375,37 +1375,45 @@ def _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qst
     return a
 
 
+RelAttentionSaved = collections.namedtuple("RelAttentionSaved", "lse out_lo")
+
+
 def rel_attention(q, k, v, table, buckets, heads, kv_heads=None, causal=False, scale=None, klen=None, qstart=None, want_lse=False):
     """Multi-head attention with a learned relative position bias, fused (neither scores nor bias in HBM):
     softmax(scale q k^T + table[bucket(j - p_i), h]) v, p_i = qstart[b] + i, over keys j < klen[b] and, if causal, j <= p_i -> [B, Tq, heads * ch].
     q [B, Tq, heads * ch], k / v [B, Tk, kv_heads * ch] (views with unit stride along the last dimension: thirds of a qkv projection, slots
     of a cache), head widths up to 128; query head h attends to kv head h // (heads // kv_heads); table [num_buckets, heads] in fp32 or q's
     type; klen / qstart int32 [B].  A query without keys gives zeros; keys behind klen are not read.  Tq = 1 with qstart = klen - 1
-    is decoding.  want_lse=True: also lse [B, heads, Tq], for the backward pass."""
+    is decoding.  want_lse=True: also RelAttentionSaved(lse [B, heads, Tq] = log sum e^s, out_lo: what out's rounding left), for the backward pass."""
     a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
     with _on(q.device):
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         lse = torch.empty((a.B, heads, a.Tq), device=q.device, dtype=torch.float32) if want_lse else None
-        a.out, a.out_batch, a.out_row, a.lse = _a(out), out.stride(0), out.stride(1), _a(lse)
+        lo = torch.empty((a.B, heads, a.Tq, a.ch), device=q.device, dtype=q.dtype) if want_lse and q.dtype != torch.float32 else None
+        a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1), _a(lse), _a(lo)
         L = _lib.lib()
         a.workspace_bytes = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 0)
         ws = _workspace(a.workspace_bytes, q.device)
         a.workspace = _a(ws)
         check(L.dua_rel_attention(ctypes.byref(a), _stream()), "dua_rel_attention")
-    return (out, lse) if want_lse else out
+    return (out, RelAttentionSaved(lse, lo)) if want_lse else out
 
 
-def rel_attention_bwd(q, k, v, table, buckets, out, lse, dout, heads, kv_heads=None, causal=False, scale=None, klen=None, qstart=None):
-    """Gradients of rel_attention (same arguments, `out` and `lse` of the forward call) given that of out -> dq, dk, dv, dtable (in their
+def rel_attention_bwd(q, k, v, table, buckets, out, saved, dout, heads, kv_heads=None, causal=False, scale=None, klen=None, qstart=None):
+    """Gradients of rel_attention (same arguments, `out` and `saved` of the forward call with want_lse) given that of out -> dq, dk, dv, dtable (in their
     operands' types; shared kv heads and the table summed over all that read them; zeros for keys behind klen)."""
     a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
     _token_tensor(out, "out", (q.dtype,), q.shape, q.device, contiguous=False)
     _token_tensor(dout, "dout", (q.dtype,), q.shape, q.device, contiguous=False)
-    _token_tensor(lse, "lse", (torch.float32,), (a.B, heads, a.Tq), q.device)
+    if not isinstance(saved, RelAttentionSaved):
+        raise TypeError("saved: expected the RelAttentionSaved of the forward call")
+    _token_tensor(saved.lse, "saved.lse", (torch.float32,), (a.B, heads, a.Tq), q.device)
+    if saved.out_lo is not None:
+        _token_tensor(saved.out_lo, "saved.out_lo", (q.dtype,), (a.B, heads, a.Tq, a.ch), q.device)
     with _on(q.device):
         new = lambda t: torch.empty(t.shape, device=q.device, dtype=t.dtype)
         dq, dk, dv, dtable = new(q), new(k), new(v), new(table)
-        a.out, a.out_batch, a.out_row, a.lse = _a(out), out.stride(0), out.stride(1), _a(lse)
+        a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1), _a(saved.lse), _a(saved.out_lo)
         a.dout, a.dout_batch, a.dout_row = _a(dout), dout.stride(0), dout.stride(1)
         a.dq, a.dk, a.dv, a.dtable = _a(dq), _a(dk), _a(dv), _a(dtable)
         a.dq_batch, a.dq_row, a.dk_batch, a.dk_row, a.dv_batch, a.dv_row = (s for t in (dq, dk, dv) for s in t.stride()[:2])

@@ -631,7 +631,9 @@ int dua_sandwich_norm_bwd(const dua_sandwich_norm_args* args_host, void* stream)
 
 /* Attention with a learned relative position bias by buckets:
  *   s_ij = scale q_i . k_j + table[bucket_map[clip(j - p_i, -radius, radius) + radius]][h],  p_i = qstart[b] + i  (qstart NULL: 0),
- * over keys j < klen[b] (NULL: Tk) and, with causal, j <= p_i;  out = softmax(s) v;  lse [B][heads][Tq] = log sum e^s (NULL: not kept).  A query
+ * over keys j < klen[b] (NULL: Tk) and, with causal, j <= p_i;  out = softmax(s) v;  lse [B][heads][Tq] = log sum e^s (NULL: not kept);
+ * out_lo [B][heads][Tq][ch] = what out's rounding to bf16 / fp16 left, 16-byte aligned (NULL: not kept; the backward pass then takes out as it
+ * is, and its gradients carry that rounding).  A query
  * without keys gives zeros (lse = -inf).  Keys behind klen are not read.  q, out [B][Tq][heads * ch], k, v [B][Tk][kv_heads * ch] with strides
  * of their own (elements); query head h reads kv head h / (heads / kv_heads); ch <= 128.  table [num_buckets][heads] (table_dtype: fp32 or
  * dtype), bucket_map [2 radius + 1]: entries outside [0, num_buckets) add no bias; radius <= 1024.  Tq = 1 is decoding. */
@@ -649,7 +651,8 @@ typedef struct {
     void* out;
     long out_batch, out_row;
     float* lse;
-    /* backward: out, lse of the forward call and dout -> dq, dk, dv (zeros behind klen), dtable [num_buckets][heads] (table_dtype) */
+    void* out_lo;
+    /* backward: out, lse, out_lo of the forward call and dout -> dq, dk, dv (zeros behind klen), dtable [num_buckets][heads] (table_dtype) */
     const void* dout;
     long dout_batch, dout_row;
     void *dq, *dk, *dv;

@@ -52,8 +52,8 @@ def attention_bounds(r, dt, ch, Tk, Tq, rep):
                lse=dp + 4 * U * r["lse"].abs().nan_to_num(posinf=0.0) + 1e-30)
     if "dq" in r:
         w = dp.max()
-        # dS: P's factor, dP's chain over ch, D from the rounded output (e) and its chain
-        ds = w + (ch + 4) * U + e + ep
+        # dS: P's factor, dP's chain over ch, D's chain (from the output and what its rounding left: e^2), its own rounding
+        ds = w + (ch + 4) * U + e * e + ep
         tol.update(dq=r["adq"] * (ds + (Tk + 8) * U) + e * r["dq"].abs() + sub, dk=r["adk"] * (ds + (rep * Tq + 8) * U) + e * r["dk"].abs() + sub,
                    dv=r["adv"] * (w + ep + (rep * Tq + 8) * U) + e * r["dv"].abs() + sub,
                    dtable=r["adtable"] * (ds + (600 + Tq + Tk) * U) + e * r["dtable"].abs())
@@ -81,7 +81,7 @@ def attention_case(dt, B, Tq, Tk, H, Hk, ch, causal=False, klen=None, qstart=Non
     args = (D(q), kg, vg, D(table), bk)
     out, lse = ops.rel_attention(*args, want_lse=True, **kw)
     close(out, r["out"], tol["out"], "out")
-    close(lse, r["lse"], tol["lse"], "lse")
+    close(lse.lse, r["lse"], tol["lse"], "lse")
     if grads:
         got = ops.rel_attention_bwd(*args, out, lse, D(do), **kw)
         for n, t in zip(("dq", "dk", "dv", "dtable"), got):
@@ -147,14 +147,14 @@ def test_rel_attention_custom_map_and_minus_infinite_bias():
     r["logit"] = r["logit"].nan_to_num(posinf=50.0).clamp(max=50.0)
     tol = attention_bounds(r, torch.float32, ch, T, T, 1)
     close(out, r["out"], tol["out"], "out")
-    close(lse, r["lse"], tol["lse"], "lse")
+    close(lse.lse, r["lse"], tol["lse"], "lse")
     for n, t in zip(("dq", "dk", "dv", "dtable"), got):
         close(t, r[n], tol[n] + 1e-30, n)
     # the only distance left is masked: every query is empty
     table[2] = -math.inf
     m2 = torch.zeros(3, dtype=torch.int32)
     out, lse = ops.rel_attention(*a[:3], table.to(dev), ops.RelativeBuckets.from_map(m2.to(dev), 3), heads=H, want_lse=True)
-    assert (out == 0).all() and (lse == -math.inf).all()
+    assert (out == 0).all() and (lse.lse == -math.inf).all()
 
 
 @pytest.mark.parametrize("dt", DTYPES)
@@ -172,7 +172,7 @@ def test_rel_attention_strided_views(dt):
         do = rnd(g, T, B, C, dtype=dt).to(dev).transpose(0, 1)
         want, lse = ops.rel_attention(q.contiguous(), k.contiguous(), v.contiguous(), table, bk, heads=H, want_lse=True)
         got, lse2 = ops.rel_attention(q, k, v, table, bk, heads=H, want_lse=True)
-        assert torch.equal(got, want) and torch.equal(lse, lse2)
+        assert torch.equal(got, want) and torch.equal(lse.lse, lse2.lse)
         a = ops.rel_attention_bwd(q, k, v, table, bk, got, lse, do, heads=H)
         b = ops.rel_attention_bwd(q.contiguous(), k.contiguous(), v.contiguous(), table, bk, want, lse, do.contiguous(), heads=H)
         for x, y in zip(a, b):
@@ -189,7 +189,7 @@ def test_rel_attention_empty_tensors():
     table = torch.ones(8, 2, device=dev)
     z = lambda *s: torch.zeros(*s, device=dev)
     out, lse = ops.rel_attention(z(2, 5, 64) + 1, z(2, 0, 64), z(2, 0, 64), table, bk, heads=2, want_lse=True)
-    assert (out == 0).all() and (lse == -math.inf).all()
+    assert (out == 0).all() and (lse.lse == -math.inf).all()
     dq, dk, dv, dt = ops.rel_attention_bwd(z(2, 5, 64) + 1, z(2, 0, 64), z(2, 0, 64), table, bk, out, lse, z(2, 5, 64) + 1, heads=2)
     assert (dq == 0).all() and dk.shape == (2, 0, 64) and (dt == 0).all()
     out, lse = ops.rel_attention(z(2, 0, 64), z(2, 5, 64), z(2, 5, 64), table, bk, heads=2, want_lse=True)
@@ -520,7 +520,8 @@ def test_token_operator_refusals():
            (ValueError, lambda: ops.rel_attention(q, q, q, table, bk, heads=2, klen=torch.zeros(2, device=dev, dtype=torch.int32))),
            (RuntimeError, lambda: ops.rel_attention(z(1, 4, 258), z(1, 4, 258), z(1, 4, 258), table, bk, heads=2)),
            (RuntimeError, lambda: ops.rel_attention(torch.zeros(1, 4, 64), q, q, table, bk, heads=2)),
-           (ValueError, lambda: ops.rel_attention_bwd(q, q, q, table, bk, q, z(1, 2, 5), q, heads=2)),
+           (TypeError, lambda: ops.rel_attention_bwd(q, q, q, table, bk, q, z(1, 2, 4), q, heads=2)),
+           (ValueError, lambda: ops.rel_attention_bwd(q, q, q, table, bk, q, ops.RelAttentionSaved(z(1, 2, 5), None), q, heads=2)),
            (ValueError, lambda: ops.sandwich_norm(z(4, 8), z(4, 9))),
            (ValueError, lambda: ops.sandwich_norm(z(4, 8), z(4, 8), post=None, post_w=z(8))),
            (ValueError, lambda: ops.sandwich_norm(z(4, 8), z(4, 8), post="batch")),
