@@ -44,8 +44,8 @@ struct AttP {
     void *o, *olo, *dq, *dk, *dv, *dtable;
     long qb, qr, kb, kr, vb, vr, ob, orow, db, dr, dqb, dqr, dkb, dkr, dvb, dvr;      // batch and row strides, elements
     const int32_t *map, *klen, *qstart;
-    float *lse, *dsum, *part, *part_ml;
-    int B, Tq, Tk, H, Hk, ch, R, nb, causal, table_dtype, vec, splits, nblk, swz;
+    float *lse, *dsum, *diag, *part, *part_ml;
+    int B, Tq, Tk, H, Hk, ch, R, nb, causal, table_dtype, splits, nblk, swz;
     float scale;
 };
 
@@ -106,14 +106,13 @@ template <typename T> using Vec16 = typename VecOf<T, Elem<T>::VEC>::type;
 
 // 16 bytes of a row at column c, zero at and past ch
 template <typename T>
-__device__ __forceinline__ Vec16<T> load16(const T* row, int c, int ch, bool vec) {
+__device__ __forceinline__ Vec16<T> load16(const T* row, int c, int ch) {
     constexpr int V = Elem<T>::VEC;
+    if (c + V <= ch) return *(const typename MemVec<T, V>::type*)(row + c);
     Vec16<T> r;
-    if (vec) {
-        if (c < ch) return *(const Vec16<T>*)(row + c);
 #pragma unroll
-        for (int j = 0; j < V; ++j) r[j] = (T)0.f;
-    } else {
+    for (int j = 0; j < V; ++j) r[j] = (T)0.f;
+    if (c < ch) {
 #pragma unroll
         for (int j = 0; j < V; ++j) r[j] = c + j < ch ? row[c + j] : (T)0.f;
     }
@@ -129,9 +128,9 @@ __device__ __forceinline__ Vec16<T> zero16() {
 
 // A lane's part of a fragment from global memory (16 bytes); a row that is not there reads as zeros
 template <typename T>
-__device__ __forceinline__ typename Frag<T>::type row_frag_global(const T* row, int c, int ch, bool vec, bool there) {
+__device__ __forceinline__ typename Frag<T>::type row_frag_global(const T* row, int c, int ch, bool there) {
     static_assert(Frag<T>::N == Elem<T>::VEC, "a lane's part of a fragment is 16 bytes");
-    return there ? load16<T>(row, c, ch, vec) : zero16<T>();
+    return there ? load16<T>(row, c, ch) : zero16<T>();
 }
 
 // A tile of ROWS rows on its way from global memory through registers to LDS: the loads of the next tile are in flight while the present one
@@ -140,11 +139,11 @@ template <typename T, int CHP, int ROWS, int THREADS = NTHR> struct Carrier {
     static constexpr int V = Elem<T>::VEC, C = Shape<T, CHP>::KW / V, P = Shape<T, CHP>::PITCH, N = (ROWS * C + THREADS - 1) / THREADS;
     static constexpr bool EVEN = ROWS * C % THREADS == 0;
     Vec16<T> x[N];
-    __device__ __forceinline__ void fetch(const T* src, long stride, int n, int ch, bool vec, int tid) {
+    __device__ __forceinline__ void fetch(const T* src, long stride, int n, int ch, int tid) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int i = tid + u * THREADS, r = i / C, c = i % C * V;
-            x[u] = r < n && (EVEN || r < ROWS) ? load16<T>(src + r * stride, c, ch, vec) : zero16<T>();
+            x[u] = r < n && (EVEN || r < ROWS) ? load16<T>(src + r * stride, c, ch) : zero16<T>();
         }
     }
     __device__ __forceinline__ void put(T* tile, int tid) const {
@@ -194,14 +193,12 @@ __device__ __forceinline__ typename Frag<T>::type acc_frag(const f32x4* a) {
 
 // four consecutive channels of a row
 template <typename T>
-__device__ __forceinline__ void store4(T* row, int c, int ch, bool vec, f32x4 v) {
-    if (vec) {
-        if (c < ch) {
-            typename VecOf<T, 4>::type x;
+__device__ __forceinline__ void store4(T* row, int c, int ch, f32x4 v) {
+    if (c + 4 <= ch) {
+        typename VecOf<T, 4>::type x;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = (T)v[j];
-            *(typename VecOf<T, 4>::type*)(row + c) = x;
-        }
+        for (int j = 0; j < 4; ++j) x[j] = (T)v[j];
+        *(typename MemVec<T, 4>::type*)(row + c) = x;
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -276,7 +273,7 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
     DUA_REQUIRE(dua_dtype_ok(a->dtype) && dua_dtype_ok(a->table_dtype) && (a->table_dtype == DUA_DTYPE_F32 || a->table_dtype == a->dtype),
                 "%s: dtype must be fp32, bf16 or fp16 and the table's fp32 or the same", who);
     DUA_REQUIRE(a->B >= 0 && a->Tq >= 0 && a->Tk >= 0 && a->Tq < (1 << 29) && a->Tk < (1 << 29), "%s: lengths must be in [0, 2^29)", who);
-    DUA_REQUIRE(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0, "%s: kv_heads must divide heads", who);
+    DUA_REQUIRE(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0 && a->heads <= 65535, "%s: kv_heads must divide heads (at most 65535)", who);
     DUA_REQUIRE(a->ch >= 1 && a->ch <= 128, "%s: head width must be in [1, 128]", who);
     DUA_REQUIRE(a->radius >= 1 && a->radius <= RMAX && a->num_buckets >= 1, "%s: radius must be in [1, %d]", who, RMAX);
     DUA_REQUIRE(a->table && a->bucket_map, "%s: null table / bucket map", who);
@@ -285,15 +282,7 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
     return DUA_OK;
 }
 
-// 16-byte accesses everywhere: widths, strides and addresses in whole 16 bytes
-struct Align {
-    size_t bits = 0;
-    void ptr(const void* q) { bits |= (uintptr_t)q; }
-    void str(long s, size_t es) { bits |= (size_t)s * es; }
-    bool ok() const { return (bits & 15) == 0; }
-};
-
-[[maybe_unused]] static AttP pack(const dua_rel_attention_args* a, bool bwd) {
+[[maybe_unused]] static AttP pack(const dua_rel_attention_args* a) {
     AttP p{};
     p.q = a->q; p.k = a->k; p.v = a->v; p.table = a->table; p.o = a->out; p.out = a->out; p.olo = a->out_lo; p.olo_in = a->out_lo; p.dout = a->dout;
     p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.dtable = a->dtable;
@@ -302,16 +291,6 @@ struct Align {
     p.map = a->bucket_map; p.klen = a->klen; p.qstart = a->qstart; p.lse = a->lse;
     p.B = a->B; p.Tq = a->Tq; p.Tk = a->Tk; p.H = a->heads; p.Hk = a->kv_heads; p.ch = a->ch; p.R = a->radius; p.nb = a->num_buckets;
     p.causal = a->causal != 0; p.table_dtype = a->table_dtype; p.scale = a->scale;
-    const size_t es = dua_dtype_size(a->dtype);
-    Align al;
-    al.bits |= (size_t)a->ch * es;
-    al.ptr(a->q); al.ptr(a->k); al.ptr(a->v); al.ptr(a->out);
-    for (long s : {p.qb, p.qr, p.kb, p.kr, p.vb, p.vr, p.ob, p.orow}) al.str(s, es);
-    if (bwd) {
-        al.ptr(a->dout); al.ptr(a->dq); al.ptr(a->dk); al.ptr(a->dv);
-        for (long s : {p.db, p.dr, p.dqb, p.dqr, p.dkb, p.dkr, p.dvb, p.dvr}) al.str(s, es);
-    }
-    p.vec = al.ok();
     return p;
 }
 
@@ -327,10 +306,10 @@ struct Align {
 [[maybe_unused]] static int query_block(int dtype) { return (dtype == DUA_DTYPE_F32 ? 16 : 32) * NWAVE; }        // Shape::QB
 [[maybe_unused]] static int key_block(int dtype, int ch) { return (dtype == DUA_DTYPE_F32 || chp_of(ch) > 64 ? 16 : 32) * NWAVE; }   // Shape::KB
 
-// Workspace of the backward pass: D of every row, the diagonal sums of every block of keys and head.
+// Workspace of the backward pass: D of every row, the diagonal sums of every head, and of every block of keys and head.
 [[maybe_unused]] static size_t rel_attention_bwd_bytes(const dua_rel_attention_args* a) {
     const size_t rows = (size_t)a->B * a->heads * a->Tq, nkb = (a->Tk + key_block(a->dtype, a->ch) - 1) / key_block(a->dtype, a->ch);
-    return (rows + a->B * nkb * a->heads * (2 * a->radius + 1)) * sizeof(float);
+    return (rows + (1 + a->B * nkb) * a->heads * (2 * a->radius + 1)) * sizeof(float);
 }
 
 // Launch with `lds` bytes of dynamic LDS (more than 64 KB, wide radii with wide fp32 heads, have to be asked for)

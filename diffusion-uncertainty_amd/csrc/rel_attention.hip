@@ -4,6 +4,9 @@
 namespace {
 
 // -------------------------------------------------------------------------------------------------------------------- forward
+// Row stride of the partial sums: whole 16 bytes
+__device__ __forceinline__ int ch4(const AttP& p) { return (p.ch + 3) & ~3; }
+
 // A row of the result: written, or (keys split over workgroups) left as unnormalised sums with its maximum and sum for the join.
 // o: columns' channels 16 c + 4 (l / 16) + r of one query; m in log2 units, l its whole sum.
 template <typename T, int CT>
@@ -11,9 +14,10 @@ __device__ __forceinline__ void finish_query(const AttP& p, int b, int h, int q,
     const long row = ((long)b * p.H + h) * p.Tq + q;
     if (p.splits > 1) {
         const long at = (long)split * p.B * p.H * p.Tq + row;
-        float* po = p.part + at * p.ch;
+        float* po = p.part + at * ch4(p);
 #pragma unroll
-        for (int c = 0; c < CT; ++c) store4<float>(po, 16 * c + 4 * g, p.ch, (p.ch & 3) == 0, o[c]);
+        for (int c = 0; c < CT; ++c)
+            if (16 * c + 4 * g < p.ch) *(f32x4*)(po + 16 * c + 4 * g) = o[c];
         if (g == 0) *(float2*)(p.part_ml + 2 * at) = make_float2(m, l);
         return;
     }
@@ -22,8 +26,8 @@ __device__ __forceinline__ void finish_query(const AttP& p, int b, int h, int q,
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const f32x4 v = o[c] * inv;
-        store4<T>((T*)p.o + at, 16 * c + 4 * g, p.ch, p.vec, v);
-        if (sizeof(T) == 2 && p.olo) store4<T>((T*)p.olo + row * p.ch, 16 * c + 4 * g, p.ch, (p.ch & 7) == 0, rest4<T>(v));
+        store4<T>((T*)p.o + at, 16 * c + 4 * g, p.ch, v);
+        if (sizeof(T) == 2 && p.olo) store4<T>((T*)p.olo + row * p.ch, 16 * c + 4 * g, p.ch, rest4<T>(v));
     }
     if (p.lse && g == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
@@ -44,15 +48,14 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
     if (w.b >= p.B) return;
     const int blk = p.causal ? p.nblk - 1 - w.blk : w.blk;                 // long rows first
     const int q0 = blk * S::QB, nk = keys_of(p, w.b), qs = start_of(p, w.b);
-    const bool vec = p.vec;
     const int kend = p.causal ? max(0, min(nk, qs + min(q0 + S::QB, p.Tq))) : nk;
     const int nt = (kend + KT - 1) / KT, t0 = (int)((long)nt * split / p.splits), t1 = (int)((long)nt * (split + 1) / p.splits);
     const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
     Carrier<T, CHP, KT> ck, cv;
     if (t0 < t1) {
-        ck.fetch(kp + (long)t0 * KT * p.kr, p.kr, nk - t0 * KT, p.ch, vec, tid);
-        cv.fetch(vp + (long)t0 * KT * p.vr, p.vr, nk - t0 * KT, p.ch, vec, tid);
+        ck.fetch(kp + (long)t0 * KT * p.kr, p.kr, nk - t0 * KT, p.ch, tid);
+        cv.fetch(vp + (long)t0 * KT * p.vr, p.vr, nk - t0 * KT, p.ch, tid);
     }
     const int qw = q0 + wave * 16 * NQ, pmin = qs + qw, pmax = pmin + 16 * NQ - 1;
     const T* qp = (const T*)p.q + w.b * p.qb + (long)w.h * p.ch;
@@ -63,7 +66,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
     for (int i = 0; i < NQ; ++i) {
         const int q = qw + 16 * i + (lane & 15);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[i][s] = row_frag_global<T>(qp + q * p.qr, S::KSTEP * s + Frag<T>::N * g, p.ch, vec, q < p.Tq);
+        for (int s = 0; s < KS; ++s) qf[i][s] = row_frag_global<T>(qp + q * p.qr, S::KSTEP * s + Frag<T>::N * g, p.ch, q < p.Tq);
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
@@ -81,8 +84,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
         __syncthreads();                                                    // (the other pair of tiles is read until here)
         const int k0 = t * KT;
         if (t + 1 < t1) {
-            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, nk - k0 - KT, p.ch, vec, tid);
-            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, nk - k0 - KT, p.ch, vec, tid);
+            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, nk - k0 - KT, p.ch, tid);
+            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, nk - k0 - KT, p.ch, tid);
         }
         if (qw >= p.Tq || (p.causal && k0 > pmax)) continue;               // (a wave without queries, or past its last key)
         f32x4 s[NQ][N16];
@@ -167,25 +170,31 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
     const T* vp = (const T*)p.v + b * p.vb + (long)hk * p.ch;
     const T* qp = (const T*)p.q + b * p.qb + q * p.qr + (long)h * p.ch;
     T* const Vt = (T*)(smem + wave * TILE);
+    Carrier<T, CHP, KT, 64> cv;
+    frag kf[N16][KS];
+    auto fetch_k = [&](int t) {
+#pragma unroll
+        for (int n = 0; n < N16; ++n) {
+            const int key = t * KT + 16 * n + col;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) kf[n][s] = row_frag_global<T>(kp + key * p.kr, S::KSTEP * s + Frag<T>::N * g, p.ch, key < nk);
+        }
+    };
+    if (t0 + wave < t1) {
+        fetch_k(t0 + wave);
+        cv.fetch(vp + (long)(t0 + wave) * KT * p.vr, p.vr, nk - (t0 + wave) * KT, p.ch, lane);
+    }
     frag qf[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = row_frag_global<T>(qp, S::KSTEP * s + Frag<T>::N * g, p.ch, p.vec, there);
+    for (int s = 0; s < KS; ++s) qf[s] = row_frag_global<T>(qp, S::KSTEP * s + Frag<T>::N * g, p.ch, there);
     const float flo = bias_at(p, h, 0), fhi = bias_at(p, h, 2 * p.R), sl = p.scale * LOG2E;
     f32x4 o[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) o[c] = ZERO4;
     float m = -INFINITY, l = 0.f;
+    // the next tile's keys are requested as soon as the products have taken the present ones, its values once those lie in LDS
     for (int t = t0 + wave; t < t1; t += NWAVE) {
         const int k0 = t * KT;
-        Carrier<T, CHP, KT, 64> cv;
-        frag kf[N16][KS];
-#pragma unroll
-        for (int n = 0; n < N16; ++n) {
-            const int key = k0 + 16 * n + col;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) kf[n][s] = row_frag_global<T>(kp + key * p.kr, S::KSTEP * s + Frag<T>::N * g, p.ch, p.vec, key < nk);
-        }
-        cv.fetch(vp + (long)k0 * p.vr, p.vr, nk - k0, p.ch, p.vec, lane);
         f32x4 s[N16];
 #pragma unroll
         for (int n = 0; n < N16; ++n) {
@@ -193,6 +202,12 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) s[n] = mma(kf[n][ks], qf[ks], s[n]);
         }
+        if (t + NWAVE < t1) fetch_k(t + NWAVE);
+        __builtin_amdgcn_wave_barrier();                                    // (the tile is this wave's own; LDS keeps a wave's order)
+        cv.put(Vt, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (t + NWAVE < t1) cv.fetch(vp + (long)(k0 + NWAVE * KT) * p.vr, p.vr, nk - k0 - NWAVE * KT, p.ch, lane);
         const int side = side_of(k0, KT, qs, qs + p.Tq - 1, p.R);
         if (side) {
             const float bias = side < 0 ? flo : fhi;
@@ -227,10 +242,6 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
                 s[n][r] = exp2_raw(s[n][r] + c0);
                 l += s[n][r];
             }
-        __builtin_amdgcn_wave_barrier();                                    // (the tile is this wave's own; LDS keeps a wave's order)
-        cv.put(Vt, lane);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int kb = 0; kb < N16; kb += S::NP) {
             const frag pf = acc_frag<T>(&s[kb]);
@@ -264,28 +275,47 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
     finish_query<T, CT>(p, b, h, q, split, o, M, L, g);
 }
 
-// One workgroup a row (b, h, q): the splits' sums moved to their common maximum and added in order, two halves of the splits side by side.
+// One workgroup a row (b, h, q): the splits' weights (a thread each), then their sums times the weights, 32 threads across the channels and 8
+// runs of splits side by side, added in order.
+constexpr int SMAX = 128;
 template <typename T>
 __global__ __launch_bounds__(NTHR) void k_rel_attention_join(AttP p) {
-    __shared__ float half[128];
+    __shared__ float wt[SMAX], red[2 * NWAVE];
+    __shared__ f32x4 sum[8][32];
     const long rows = (long)p.B * p.H * p.Tq, row = blockIdx.x;
-    const int c = threadIdx.x & 127, part = threadIdx.x >> 7;
-    float M = -INFINITY, L = 0.f, a = 0.f;
-    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[2 * (s * rows + row)]);
-    const float ms = M == -INFINITY ? 0.f : M;
-    for (int s = 0; s < p.splits; ++s) L += exp2_raw(p.part_ml[2 * (s * rows + row)] - ms) * p.part_ml[2 * (s * rows + row) + 1];
-    if (c < p.ch)
-        for (int s = part; s < p.splits; s += 2) a += exp2_raw(p.part_ml[2 * (s * rows + row)] - ms) * p.part[(s * rows + row) * p.ch + c];
-    if (part) half[c] = a;
-    __syncthreads();
-    if (part) return;
-    a = (a + half[c]) * (L > 0.f || L != L ? 1.0f / L : 0.f);
-    const int q = (int)(row % p.Tq), h = (int)(row / p.Tq % p.H), b = (int)(row / p.Tq / p.H);
-    if (c < p.ch) {
-        const T r = (T)a;
-        ((T*)p.o)[b * p.ob + q * p.orow + (long)h * p.ch + c] = r;
-        if (sizeof(T) == 2 && p.olo) ((T*)p.olo)[row * p.ch + c] = (T)(a - (float)r);
+    const int tid = threadIdx.x, c = 4 * (tid & 31), run = tid >> 5, per = (p.splits + 7) / 8, s0 = run * per, s1 = min(s0 + per, p.splits);
+    float m = -INFINITY, l = 0.f;
+    if (tid < p.splits) {
+        const float2 x = *(const float2*)(p.part_ml + 2 * (tid * rows + row));
+        m = x.x;
+        l = x.y;
     }
+    float M = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float w = exp2_raw(m - (M == -INFINITY ? 0.f : M)), part = wave_sum(w * l);
+    if (tid < p.splits) wt[tid] = w;
+    if ((tid & 63) == 0) red[NWAVE + (tid >> 6)] = part;
+    __syncthreads();
+    const float L = (red[NWAVE] + red[NWAVE + 1]) + (red[NWAVE + 2] + red[NWAVE + 3]);
+    f32x4 a = ZERO4;
+    if (c < p.ch) {
+        const float* src = p.part + row * ch4(p) + c;
+#pragma unroll 4
+        for (int s = s0; s < s1; ++s) a += wt[s] * *(const f32x4*)(src + s * rows * ch4(p));
+    }
+    sum[run][tid & 31] = a;
+    __syncthreads();
+    if (run || c >= p.ch) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a += sum[i][tid];
+    a *= L > 0.f || L != L ? 1.0f / L : 0.f;
+    const int q = (int)(row % p.Tq), h = (int)(row / p.Tq % p.H), b = (int)(row / p.Tq / p.H);
+    store4<T>((T*)p.o + b * p.ob + q * p.orow + (long)h * p.ch, c, p.ch, a);
+    if (sizeof(T) == 2 && p.olo) store4<T>((T*)p.olo + row * p.ch, c, p.ch, rest4<T>(a));
     if (p.lse && c == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * LN2;
 }
 
@@ -298,13 +328,13 @@ Plan plan(const dua_rel_attention_args* a) {
     const long wgs = pl.few ? units : units * rep * ((a->Tq + query_block(a->dtype) - 1) / query_block(a->dtype));
     const long want = pl.few ? (1024 + wgs - 1) / wgs : (wgs < 256 ? (512 + wgs - 1) / wgs : 1), most = a->Tk / (pl.few ? 128 : 256);
     long s = want < most ? want : most;
-    s = s < 1 ? 1 : (s > 128 ? 128 : s);
+    s = s < 1 ? 1 : (s > SMAX ? SMAX : s);
     pl.splits = (int)s;
     return pl;
 }
 
-// Unnormalised sums of the splits, whole 16 bytes
-size_t split_floats(const dua_rel_attention_args* a, int splits) { return ((size_t)splits * a->B * a->heads * a->Tq * a->ch + 3) / 4 * 4; }
+// Unnormalised sums of the splits
+size_t split_floats(const dua_rel_attention_args* a, int splits) { return (size_t)splits * a->B * a->heads * a->Tq * ((a->ch + 3) / 4 * 4); }
 
 template <typename T, int CHP> struct Fwd {
     static int run(AttP p, bool few, hipStream_t st) {
@@ -338,7 +368,7 @@ extern "C" int dua_rel_attention(const dua_rel_attention_args* a, void* stream) 
     const Plan pl = plan(a);
     DUA_REQUIRE(pl.splits == 1 || (a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= dua_rel_attention_workspace_bytes(a, 0)),
                 "dua_rel_attention: workspace smaller than dua_rel_attention_workspace_bytes, or not 16-byte aligned");
-    AttP p = pack(a, false);
+    AttP p = pack(a);
     p.splits = pl.splits;
     p.part = (float*)a->workspace;
     p.part_ml = p.part + split_floats(a, pl.splits);

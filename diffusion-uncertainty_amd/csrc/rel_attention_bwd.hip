@@ -51,14 +51,13 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
     if (w.b >= p.B) return;
     const int blk = p.causal ? p.nblk - 1 - w.blk : w.blk;
     const int q0 = blk * S::QB, nk = keys_of(p, w.b), qs = start_of(p, w.b);
-    const bool vec = p.vec;
     const int kend = p.causal ? max(0, min(nk, qs + min(q0 + S::QB, p.Tq))) : nk;
     const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
     Carrier<T, CHP, KT> ck, cv;
     if (kend > 0) {
-        ck.fetch(kp, p.kr, nk, p.ch, vec, tid);
-        cv.fetch(vp, p.vr, nk, p.ch, vec, tid);
+        ck.fetch(kp, p.kr, nk, p.ch, tid);
+        cv.fetch(vp, p.vr, nk, p.ch, tid);
     }
     load_lut(p, w.h, S::PAD, lut);
     const int qw = q0 + wave * 16 * NQ, pmin = qs + qw, pmax = pmin + 16 * NQ - 1;
@@ -77,11 +76,11 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int c = S::KSTEP * s + Frag<T>::N * g;
-            qf[i][s] = row_frag_global<T>(qp + q * p.qr, c, p.ch, vec, there);
-            df[i][s] = row_frag_global<T>(dp + q * p.dr, c, p.ch, vec, there);
-            const frag of = row_frag_global<T>(op + q * p.orow, c, p.ch, vec, there);
+            qf[i][s] = row_frag_global<T>(qp + q * p.qr, c, p.ch, there);
+            df[i][s] = row_frag_global<T>(dp + q * p.dr, c, p.ch, there);
+            const frag of = row_frag_global<T>(op + q * p.orow, c, p.ch, there);
             frag lo = zero16<T>();                                          // the output's rounding: D's error would be the gradients' largest
-            if (sizeof(T) == 2 && p.olo_in) lo = row_frag_global<T>((const T*)p.olo_in + (row0 + q) * p.ch, c, p.ch, (p.ch & 7) == 0, there);
+            if (sizeof(T) == 2 && p.olo_in) lo = row_frag_global<T>((const T*)p.olo_in + (row0 + q) * p.ch, c, p.ch, there);
 #pragma unroll
             for (int j = 0; j < Frag<T>::N; ++j) d += (float)df[i][s][j] * ((float)of[j] + (float)lo[j]);
         }
@@ -102,8 +101,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
         cv.put(Vt, tid);
         __syncthreads();
         if (k0 + KT < kend) {
-            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, nk - k0 - KT, p.ch, vec, tid);
-            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, nk - k0 - KT, p.ch, vec, tid);
+            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, nk - k0 - KT, p.ch, tid);
+            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, nk - k0 - KT, p.ch, tid);
         }
         if (qw >= p.Tq) continue;
         // steps of 16 NP keys: scores, dP, dS, and dS straight into dq - few registers live
@@ -161,25 +160,35 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
         if (q >= p.Tq) continue;
         if (g == 0) p.dsum[row0 + q] = dt;
 #pragma unroll
-        for (int c = 0; c < CT; ++c) store4<T>(gp + q * p.dqr, 16 * c + 4 * g, p.ch, vec, a[i][c]);
+        for (int c = 0; c < CT; ++c) store4<T>(gp + q * p.dqr, 16 * c + 4 * g, p.ch, a[i][c]);
     }
 }
 
-// dtable[n][h]: the workgroups' diagonal sums of head h in their order, then the diagonals of each bucket.
-template <typename TT>
-__global__ __launch_bounds__(1024) void k_rel_attention_dtable(AttP p, int nparts) {
-    __shared__ float sum[2 * RMAX + 1];
-    const int h = blockIdx.x, nd = 2 * p.R + 1;
-    for (int i = threadIdx.x; i < nd; i += 1024) {
-        float t = 0.f;
-        for (int j = 0; j < nparts; ++j) t += p.part[((long)j * p.H + h) * nd + i];
-        sum[i] = t;
+// The workgroups' diagonal sums of head h added in their order, 64 distances a workgroup and a run of parts for each of its 16 waves ...
+__global__ __launch_bounds__(1024) void k_rel_attention_diag(AttP p, int nparts) {
+    __shared__ float sm[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.y, nd = 2 * p.R + 1, i = blockIdx.x * 64 + lane;
+    const int per = (nparts + 15) / 16, j0 = wave * per, j1 = min(j0 + per, nparts);
+    float t = 0.f;
+    if (i < nd) {
+#pragma unroll 8
+        for (int j = j0; j < j1; ++j) t += p.part[((long)j * p.H + h) * nd + i];
     }
+    sm[wave][lane] = t;
     __syncthreads();
-    for (int n = threadIdx.x; n < p.nb; n += 1024) {
+    if (wave || i >= nd) return;
+    for (int x = 1; x < 16; ++x) t += sm[x][lane];
+    p.diag[h * nd + i] = t;
+}
+// ... and dtable[n][h]: the distances of bucket n, a wave a bucket.
+template <typename TT>
+__global__ __launch_bounds__(1024) void k_rel_attention_dtable(AttP p) {
+    const int lane = threadIdx.x & 63, h = blockIdx.x, nd = 2 * p.R + 1;
+    for (int n = threadIdx.x >> 6; n < p.nb; n += 16) {
         float t = 0.f;
-        for (int i = 0; i < nd; ++i) t += p.map[i] == n ? sum[i] : 0.f;
-        ((TT*)p.dtable)[(long)n * p.H + h] = (TT)t;
+        for (int i = lane; i < nd; i += 64) t += p.map[i] == n ? p.diag[h * nd + i] : 0.f;
+        t = wave_sum(t);
+        if (lane == 0) ((TT*)p.dtable)[(long)n * p.H + h] = (TT)t;
     }
 }
 
@@ -199,7 +208,6 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
     const Where w = place(p, 1, blockIdx.x);
     if (w.b >= p.B) return;
     const int k0 = w.blk * S::KB, nk = keys_of(p, w.b), qs = start_of(p, w.b);
-    const bool vec = p.vec;
     const int kw = k0 + wave * 16 * NK;
     const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
@@ -211,8 +219,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int c = S::KSTEP * s + Frag<T>::N * g;
-            kf[i][s] = row_frag_global<T>(kp + kk * p.kr, c, p.ch, vec, kk < nk);
-            vf[i][s] = row_frag_global<T>(vp + kk * p.vr, c, p.ch, vec, kk < nk);
+            kf[i][s] = row_frag_global<T>(kp + kk * p.kr, c, p.ch, kk < nk);
+            vf[i][s] = row_frag_global<T>(vp + kk * p.vr, c, p.ch, kk < nk);
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c) { ak[i][c] = ZERO4; av[i][c] = ZERO4; }
@@ -225,8 +233,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
     float row_next = 0.f;
     auto fetch = [&](int t) {
         const int h = w.hk * rep + t / per, q0 = (qbeg + t % per) * QT;
-        cq.fetch((const T*)p.q + w.b * p.qb + (long)h * p.ch + (long)q0 * p.qr, p.qr, p.Tq - q0, p.ch, vec, tid);
-        cd.fetch((const T*)p.dout + w.b * p.db + (long)h * p.ch + (long)q0 * p.dr, p.dr, p.Tq - q0, p.ch, vec, tid);
+        cq.fetch((const T*)p.q + w.b * p.qb + (long)h * p.ch + (long)q0 * p.qr, p.qr, p.Tq - q0, p.ch, tid);
+        cd.fetch((const T*)p.dout + w.b * p.db + (long)h * p.ch + (long)q0 * p.dr, p.dr, p.Tq - q0, p.ch, tid);
         if (tid < 2 * QT) {
             const int q = q0 + tid % QT;
             const float* src = tid < QT ? p.lse : p.dsum;
@@ -359,8 +367,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
         if (kk >= p.Tk) continue;                                          // keys behind klen: zeros
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            store4<T>(gk + kk * p.dkr, 16 * c + 4 * g, p.ch, vec, ak[i][c]);
-            store4<T>(gv + kk * p.dvr, 16 * c + 4 * g, p.ch, vec, av[i][c]);
+            store4<T>(gk + kk * p.dkr, 16 * c + 4 * g, p.ch, ak[i][c]);
+            store4<T>(gv + kk * p.dvr, 16 * c + 4 * g, p.ch, av[i][c]);
         }
     }
 }
@@ -378,9 +386,10 @@ template <typename T, int CHP> struct Bwd {
             if (int rc = launch(k_rel_attention_dkv<T, CHP>, "dua_rel_attention_bwd", dim3(grid), NTHR, 4 * S::TILE + (4 * S::KT + (1 + NWAVE) * nl) * sizeof(float), st, p)) return rc;
         }
         const int nparts = p.B * ((p.Tk + S::KB - 1) / S::KB);
-        if (p.table_dtype == DUA_DTYPE_F32) return launch(k_rel_attention_dtable<float>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p, nparts);
-        if (p.table_dtype == DUA_DTYPE_BF16) return launch(k_rel_attention_dtable<bf16_t>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p, nparts);
-        return launch(k_rel_attention_dtable<f16_t>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p, nparts);
+        if (int rc = launch(k_rel_attention_diag, "dua_rel_attention_bwd", dim3((2 * p.R + 64) / 64, p.H), 1024, 0, st, p, nparts)) return rc;
+        if (p.table_dtype == DUA_DTYPE_F32) return launch(k_rel_attention_dtable<float>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
+        if (p.table_dtype == DUA_DTYPE_BF16) return launch(k_rel_attention_dtable<bf16_t>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
+        return launch(k_rel_attention_dtable<f16_t>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
     }
 };
 
@@ -393,8 +402,9 @@ extern "C" int dua_rel_attention_bwd(const dua_rel_attention_args* a, void* stre
     DUA_REQUIRE(a->B == 0 || a->Tk == 0 || (a->dk && a->dv), "dua_rel_attention_bwd: null output");
     const size_t need = rel_attention_bwd_bytes(a);
     DUA_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), "dua_rel_attention_bwd: workspace smaller than dua_rel_attention_workspace_bytes");
-    AttP p = pack(a, true);
+    AttP p = pack(a);
     p.dsum = (float*)a->workspace;
-    p.part = p.dsum + (size_t)a->B * a->heads * a->Tq;
+    p.diag = p.dsum + (size_t)a->B * a->heads * a->Tq;
+    p.part = p.diag + (size_t)a->heads * (2 * a->radius + 1);
     return dispatch<Bwd>(a->dtype, p, false, as_stream(stream));
 }

@@ -21,20 +21,24 @@ constexpr int RESCAN = 64;               // threads re-read whole before the ord
 constexpr int SMAX = 32;                 // parts of a row
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-struct Soft { float m, s, w; };          // w in log2 units
-// moves a partial sum to a larger maximum; c = t log2 e.  The difference is clamped so that 0 * inf cannot arise (2^-1e4 = 0)
-__device__ __forceinline__ void soft_to(Soft& a, float m, float c) {
-    const float d = fmaxf((a.m - m) * c, -1e4f), f = __builtin_amdgcn_exp2f(d);
+// Sums of a set of logits in log2 units, L = x c with c = t log2 e: s = sum 2^(L - ref), w = sum 2^(L - ref) (L - ref).  The reference is any float
+// near the largest L - d = fma(x, c, -ref) is exact but for its own rounding - so it moves only when a value passes it by 2^16.  Logits beyond
+// +-2^28 (masks of the type's lowest value everywhere, offsets of 1e30) have no such reference: s comes out 0, infinite or NaN, and the
+// row is summed again relative to its own largest logit (scan_huge), where L - ref = (x - m) c.
+struct Soft { float ref, s, w; };
+__device__ __forceinline__ void soft_shift(Soft& a, float d) {              // to a reference higher by -d; clamped: 2^-1e4 = 0 and no 0 * inf
+    d = fmaxf(d, -1e4f);
+    const float f = __builtin_amdgcn_exp2f(d);
     a.w = f * (a.w + a.s * d);
     a.s *= f;
-    a.m = m;
 }
-__device__ __forceinline__ Soft soft_join(Soft a, Soft b, float c) {
-    const float m = fmaxf(a.m, b.m);
-    soft_to(a, m, c);
-    soft_to(b, m, c);
-    return Soft{m, a.s + b.s, a.w + b.w};
+__device__ __forceinline__ Soft soft_join(Soft a, Soft b, float c) {          // c: log2 units of a reference's unit
+    const float ref = fmaxf(a.ref, b.ref);
+    soft_shift(a, (a.ref - ref) * c);
+    soft_shift(b, (b.ref - ref) * c);
+    return Soft{ref, a.s + b.s, a.w + b.w};
 }
+constexpr float REF_MAX = 268435456.f;                                       // 2^28
 
 // total order of floats as whole numbers: -0 = +0, every NaN above +inf
 __device__ __forceinline__ uint32_t okey(float x) {
@@ -46,13 +50,13 @@ __device__ __forceinline__ uint32_t okey(float x) {
 struct LogpP {
     const void* x;
     const int64_t* ids;
-    float *logprob, *entropy, *lse, *stats;          // stats [rows][4]: m, log s, H, -
+    float *logprob, *entropy, *lse, *stats;          // stats [rows][4]: reference, log2 s, H, 1 if the reference is a logit (else log2 units)
     int64_t* top_ids;
     float* top_lp;
     long rows, ld, V;
     int k, splits;
     float t;
-    float* part;                                      // [rows][splits][4 + 2 k]: m, s, w, - ; values ; indices (as int32 bits, within V < 2^31)
+    float* part;                                      // [rows][splits][4 + 2 k]: ref, s, w, huge ; values ; indices (as int32 bits, within V < 2^31)
     // backward
     const float *dlp, *dent, *dtop;
     const int64_t* tids;
@@ -88,7 +92,7 @@ struct Shared {
     uint32_t ck[CAP];                     // candidates: key, index
     int ci[CAP];
     int rescan[RESCAN];
-    uint32_t tau;
+    uint32_t tau;                         // (candidates of the fast selection reach it)
     int ncand, nrescan, any;
     uint32_t bk[2][KMAX];                 // running best of the ordered scan
     int bi[2][KMAX];
@@ -159,67 +163,117 @@ __device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
     return cur;
 }
 
-// Soft sums and the k best (sorted, with their values) of elements [v0, v1) of one row by one workgroup; k <= v1 - v0.
-template <typename T>
-__device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared& sh, int& best_set) {
-    constexpr int VEC = Elem<T>::VEC;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Groups<T> gr(row, v0, v1);
-    Soft a{-FLT_MAX, 0.f, 0.f};
-    float b1 = -INFINITY, b2 = -INFINITY;                 // best value, best value outside the best group
-    long bg = -1;
-    auto eat = [&](const float* f, long g) {
-        float vm = f[0];
+// The workgroup's sum of its threads' sums; c as in soft_join
+__device__ __forceinline__ Soft block_join(Soft t, float c, Soft* soft) {
 #pragma unroll
-        for (int j = 1; j < VEC; ++j) vm = fmaxf(vm, f[j]);
-        b2 = fmaxf(b2, fminf(b1, vm));
-        if (vm > b1 || bg < 0) bg = g;
-        b1 = fmaxf(b1, vm);
-        const float m = fmaxf(a.m, vm);
-        if (m > a.m) soft_to(a, m, c);
+    for (int o = 32; o > 0; o >>= 1) {
+        const Soft u{__shfl_xor(t.ref, o, 64), __shfl_xor(t.s, o, 64), __shfl_xor(t.w, o, 64)};
+        t = soft_join(t, u, c);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) soft[threadIdx.x >> 6] = t;
+    __syncthreads();
+    t = soft[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) t = soft_join(t, soft[i], c);
+    return t;
+}
+
+// Rows without a reference in log2 units: relative to the largest logit itself
+template <typename T>
+__device__ Soft scan_huge(const Groups<T>& gr, float c, Soft* soft) {
+    constexpr int VEC = Elem<T>::VEC;
+    Soft a{-FLT_MAX, 0.f, 0.f};
+    for (long g = threadIdx.x; g < gr.n; g += NT) {
+        float f[VEC], m = a.ref;
+        gr.load(g, f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = fmaxf(m, f[j]);
+        soft_shift(a, (a.ref - m) * c);
+        a.ref = m;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             const float d = (f[j] - m) * c, e = __builtin_amdgcn_exp2f(d);
             a.s += e;
+            a.w += e * fmaxf(d, -150.f);
+        }
+    }
+    return block_join(a, c, soft);
+}
+
+// Sums and the k best (sorted) of elements [v0, v1) of one row by one workgroup; k <= v1 - v0.
+template <typename T>
+__device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared& sh, int& best_set, bool& huge) {
+    constexpr int VEC = Elem<T>::VEC;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Groups<T> gr(row, v0, v1);
+    Soft a{-REF_MAX, 0.f, 0.f};
+    float b1 = -INFINITY, b2 = -INFINITY;                 // best value, best value outside the best group
+    int bg = -1;
+    auto eat = [&](const float* f, int g) {
+        float vm = f[0];
+#pragma unroll
+        for (int j = 1; j < VEC; ++j) vm = fmaxf(vm, f[j]);
+        b2 = fmaxf(b2, fminf(b1, vm));
+        bg = vm > b1 || bg < 0 ? g : bg;
+        b1 = fmaxf(b1, vm);
+        const float top = fminf(vm * c, REF_MAX);
+        if (__any(top > a.ref + 16.f)) {
+            const float ref = fmaxf(top, a.ref);
+            soft_shift(a, a.ref - ref);
+            a.ref = ref;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float d = fmaf(f[j], c, -a.ref), e = __builtin_amdgcn_exp2f(d);
+            a.s += e;
             a.w += e * fmaxf(d, -150.f);                  // 2^-150 = 0: e is 0 wherever the clamp acts, and 0 * -inf does not arise
         }
     };
-    long g = tid;
-    for (; g + NT < gr.n; g += 2 * NT) {
+    const int n = (int)gr.n;
+    int g = tid;
+    for (; g + NT < n; g += 2 * NT) {
         float f0[VEC], f1[VEC];
         gr.load(g, f0);
         gr.load(g + NT, f1);
         eat(f0, g);
         eat(f1, g + NT);
     }
-    if (g < gr.n) {
+    if (g < n) {
         float f0[VEC];
         gr.load(g, f0);
         eat(f0, g);
     }
-    Soft t = a;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const Soft u{__shfl_xor(t.m, o, 64), __shfl_xor(t.s, o, 64), __shfl_xor(t.w, o, 64)};
-        t = soft_join(t, u, c);
+    const uint32_t mine = bg < 0 ? 0u : okey(b1);
+    // a bound of the k-th value from the maxima of 64, 128 or 256 sets of threads: the smallest of the k largest maxima
+    const int sets = k <= 16 ? 64 : (k <= 32 ? 128 : 256);
+    if (k) {
+        uint32_t best = mine;
+        if (sets <= 128) best = max(best, (uint32_t)__shfl_xor((int)best, 1, 64));
+        if (sets == 64) best = max(best, (uint32_t)__shfl_xor((int)best, 2, 64));
+        if (tid % (NT / sets) == 0) sh.key[tid / (NT / sets)] = best;
+        if (tid == 0) { sh.ncand = 0; sh.nrescan = 0; sh.any = 0; sh.tau = 0xFFFFFFFFu; }
     }
-    __syncthreads();
-    if (lane == 0) sh.soft[wave] = t;
-    sh.key[tid] = bg < 0 ? 0u : okey(b1);
-    if (tid == 0) { sh.ncand = 0; sh.nrescan = 0; sh.any = 0; }
-    __syncthreads();
-    t = sh.soft[0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) t = soft_join(t, sh.soft[i], c);
+    Soft t = block_join(a, 1.f, sh.soft);
+    huge = !(t.s > 0.f && t.s < INFINITY);
+    if (huge) t = scan_huge(gr, c, sh.soft);
     best_set = 0;
     if (k == 0) return t;
 
-    const bool odd = !(t.s < INFINITY);                    // NaN, or infinite: NaN / +inf among the logits
-    if (!odd) {
-        const uint32_t mine = sh.key[tid];
-        if (rank_of_thread(sh.key, mine, tid) == k - 1) sh.tau = mine;
+    if (!huge) {                                           // (no NaN, no +inf)
+        if (tid < sets) {
+            const uint4* keys = (const uint4*)sh.key;
+            const uint32_t x = sh.key[tid];
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < sets / 4; ++j) {
+                const uint4 q = keys[j];
+                above += (q.x > x) + (q.y > x) + (q.z > x) + (q.w > x);
+            }
+            if (above < k) atomicMin(&sh.tau, x);
+        }
         __syncthreads();
-        const uint32_t tau = sh.tau;                       // 0: fewer than k threads hold elements - every element is a candidate
+        const uint32_t tau = sh.tau;                       // 0: fewer than k sets hold elements - every element is a candidate
         auto push = [&](long e, float x) {
             if (e >= gr.v0 && e < gr.v1 && okey(x) >= tau) {
                 const int at = atomicAdd(&sh.ncand, 1);
@@ -227,33 +281,34 @@ __device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared&
             }
         };
         if (bg >= 0 && mine >= tau) {
-            if (tau && okey(b2) >= tau && b2 > -INFINITY) {
+            const bool more = n > NT && okey(b2) >= tau;    // (with one group a thread there is no value outside it)
+            if (more && b2 == -INFINITY) {
+                sh.any = 1;                                 // the bound itself is -inf: too few finite values
+            } else if (more) {
                 const int at = atomicAdd(&sh.nrescan, 1);
                 if (at < RESCAN) sh.rescan[at] = tid;
-            } else if (tau && okey(b2) >= tau) {
-                sh.any = 1;                                 // the bound itself is -inf: too few finite values
             } else {
                 float f[VEC];
                 gr.load(bg, f);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) push(gr.first + bg * VEC + j, f[j]);
+                for (int j = 0; j < VEC; ++j) push(gr.first + (long)bg * VEC + j, f[j]);
             }
         }
         __syncthreads();
         const int nr = sh.nrescan;
         if (nr <= RESCAN && !sh.any) {
             for (int i = wave; i < nr; i += NW)
-                for (long gg = sh.rescan[i] + (long)lane * NT; gg < gr.n; gg += 64L * NT) {
+                for (int gg = sh.rescan[i] + lane * NT; gg < n; gg += 64 * NT) {
                     float f[VEC];
                     gr.load(gg, f);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) push(gr.first + gg * VEC + j, f[j]);
+                    for (int j = 0; j < VEC; ++j) push(gr.first + (long)gg * VEC + j, f[j]);
                 }
             __syncthreads();
-            const int n = sh.ncand;
-            if (n <= CAP) {
-                for (int i = tid; i < n; i += NT) {
-                    const int r = rank_of(sh.ck, sh.ci, n, sh.ck[i], sh.ci[i]);
+            const int nc = sh.ncand;
+            if (nc <= CAP) {
+                for (int i = tid; i < nc; i += NT) {
+                    const int r = rank_of(sh.ck, sh.ci, nc, sh.ck[i], sh.ci[i]);
                     if (r < k) { sh.bk[0][r] = sh.ck[i]; sh.bi[0][r] = sh.ci[i]; }
                 }
                 __syncthreads();
@@ -269,26 +324,27 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return k == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((k >> 31) ? k & 0x7FFFFFFFu : ~k);
 }
 
-// log probability of a value; a row without any finite value has no distribution: -inf everywhere, entropy 0
-__device__ __forceinline__ float value_lp(float x, float m, float logs, float t) {
-    return logs == -INFINITY ? -INFINITY : (x - m) * t - logs;
-}
+// log2 of p of a value from the row's reference and log2 s
+__device__ __forceinline__ float log2_p(float x, float ref, float logs, bool huge, float c) { return (huge ? (x - ref) * c : fmaf(x, c, -ref)) - logs; }
 
+// A row without any finite value has no distribution: log probabilities -inf, entropy 0.
 template <typename T>
-__device__ void finish_row(const LogpP& p, long r, Soft a, const uint32_t* bk, const int* bi) {
-    const float logs = a.s > 0.f || a.s != a.s ? logf(a.s) : -INFINITY;
+__device__ void finish_row(const LogpP& p, long r, Soft a, bool huge, const uint32_t* bk, const int* bi) {
+    const float c = p.t * LOG2E, logs = a.s > 0.f || a.s != a.s ? log2f(a.s) : -INFINITY;
+    const bool none = logs == -INFINITY;
     if (threadIdx.x == 0) {
-        const float H = logs == -INFINITY ? 0.f : logs - LN2 * a.w / a.s;
+        const float H = none ? 0.f : LN2 * (logs - a.w / a.s);
         const int64_t id = p.ids ? p.ids[r] : -1;
-        const float xid = id >= 0 && id < p.V ? (float)((const T*)p.x)[r * p.ld + id] : 0.f;
-        p.logprob[r] = id >= 0 && id < p.V ? value_lp(xid, a.m, logs, p.t) : 0.f;
+        float lp = 0.f;
+        if (id >= 0 && id < p.V) lp = none ? -INFINITY : LN2 * log2_p((float)((const T*)p.x)[r * p.ld + id], a.ref, logs, huge, c);
+        p.logprob[r] = lp;
         p.entropy[r] = H;
-        p.lse[r] = logs == -INFINITY ? -INFINITY : a.m * p.t + logs;
-        *(float4*)(p.stats + 4 * r) = make_float4(a.m, logs, H, 0.f);
+        p.lse[r] = none ? -INFINITY : (huge ? a.ref * p.t + LN2 * logs : LN2 * (a.ref + logs));
+        *(float4*)(p.stats + 4 * r) = make_float4(a.ref, logs, H, huge ? 1.f : 0.f);
     }
     for (int j = threadIdx.x; j < p.k; j += NT) {
         p.top_ids[r * p.k + j] = bi[j];
-        p.top_lp[r * p.k + j] = value_lp(key_value(bk[j]), a.m, logs, p.t);
+        p.top_lp[r * p.k + j] = none ? -INFINITY : LN2 * log2_p(key_value(bk[j]), a.ref, logs, huge, c);
     }
 }
 
@@ -297,8 +353,9 @@ __global__ __launch_bounds__(NT) void k_token_logprobs(LogpP p) {
     __shared__ Shared sh;
     const long r = blockIdx.x;
     int set;
-    const Soft a = scan_row((const T*)p.x + r * p.ld, 0, p.V, p.t * LOG2E, p.k, sh, set);
-    finish_row<T>(p, r, a, sh.bk[set], sh.bi[set]);
+    bool huge;
+    const Soft a = scan_row((const T*)p.x + r * p.ld, 0, p.V, p.t * LOG2E, p.k, sh, set, huge);
+    finish_row<T>(p, r, a, huge, sh.bk[set], sh.bi[set]);
 }
 
 // Few rows: `splits` workgroups a row, each with its part's sums and its k best; k_token_logprobs_join puts them together.
@@ -308,9 +365,10 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_part(LogpP p) {
     const long r = blockIdx.x / p.splits, i = blockIdx.x % p.splits;
     const long v0 = p.V * i / p.splits, v1 = p.V * (i + 1) / p.splits;
     int set;
-    const Soft a = scan_row((const T*)p.x + r * p.ld, v0, v1, p.t * LOG2E, p.k, sh, set);
+    bool huge;
+    const Soft a = scan_row((const T*)p.x + r * p.ld, v0, v1, p.t * LOG2E, p.k, sh, set, huge);
     float* o = p.part + (long)blockIdx.x * (4 + 2 * p.k);
-    if (threadIdx.x == 0) { o[0] = a.m; o[1] = a.s; o[2] = a.w; }
+    if (threadIdx.x == 0) { o[0] = a.ref; o[1] = a.s; o[2] = a.w; o[3] = huge ? 1.f : 0.f; }
     for (int j = threadIdx.x; j < p.k; j += NT) {
         o[4 + j] = __uint_as_float(sh.bk[set][j]);
         o[4 + p.k + j] = __int_as_float(sh.bi[set][j]);
@@ -324,15 +382,22 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_join(LogpP p) {
     __shared__ uint32_t bk[KMAX];
     __shared__ int bi[KMAX];
     __shared__ int n;
+    __shared__ Soft soft[NW];
     const long r = blockIdx.x;
-    const float* q = p.part + r * p.splits * (4 + 2 * p.k);
-    Soft a{q[0], q[1], q[2]};
+    const float *q = p.part + r * p.splits * (4 + 2 * p.k), c = p.t * LOG2E;
+    // Parts summed relative to a logit (sum 0: nothing finite in them) do not mix with the others; far below them (a part that is masked with
+    // the type's lowest value) they add nothing, else the row is summed again here.
+    Soft a{-REF_MAX, 0.f, 0.f};
+    bool huge = false, low = false;
     uint32_t tau = 0;                                       // the best of the parts' k-th values bounds the row's k-th from below
     for (int i = 0; i < p.splits; ++i) {
         const float* o = q + i * (4 + 2 * p.k);
-        if (i) a = soft_join(a, Soft{o[0], o[1], o[2]}, p.t * LOG2E);
+        if (o[3] == 0.f) a = soft_join(a, Soft{o[0], o[1], o[2]}, 1.f);
+        else if (o[1] != 0.f) (o[1] < INFINITY && o[0] < 0.f ? low : huge) = true;
         if (p.k) tau = max(tau, __float_as_uint(o[4 + p.k - 1]));
     }
+    huge = huge || (low && a.ref < -0.5f * REF_MAX);
+    if (huge) a = scan_huge(Groups<T>((const T*)p.x + r * p.ld, 0, p.V), c, soft);
     if (threadIdx.x == 0) n = 0;
     __syncthreads();
     for (int j = threadIdx.x; j < p.splits * p.k; j += NT) {
@@ -350,7 +415,7 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_join(LogpP p) {
         if (rk < p.k) { bk[rk] = ck[j]; bi[rk] = ci[j]; }
     }
     __syncthreads();
-    finish_row<T>(p, r, a, bk, bi);
+    finish_row<T>(p, r, a, huge, bk, bi);
 }
 
 // One pass: reads a part of a row, writes its gradient.  The tokens that carry gradients of their own (the given one, the alternatives) are read
@@ -367,7 +432,7 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_bwd(LogpP p) {
     const T* row = (const T*)p.x + r * p.ld;
     T* out = (T*)p.dx + r * p.ldd;
     const float4 st = *(const float4*)(p.stats + 4 * r);
-    const float m = st.x, logs = st.y, H = st.z, gH = p.dent ? p.dent[r] : 0.f;
+    const float c = p.t * LOG2E, off = st.w != 0.f ? st.x : 0.f, ref = st.w != 0.f ? 0.f : st.x, logs = st.y, H = st.z, gH = p.dent ? p.dent[r] : 0.f;
     if (tid <= p.k) {
         const long id = tid == 0 ? (p.ids ? (long)p.ids[r] : -1) : (long)p.tids[r * p.k + tid - 1];
         const bool in = id >= 0 && id < p.V;
@@ -398,8 +463,8 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_bwd(LogpP p) {
     const float A = gsum;
     const bool none = logs == -INFINITY;
     auto grad = [&](float x, float g) {
-        const float lp = (x - m) * p.t - logs, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
-        return none ? 0.f : p.t * (g - pr * (A + gH * (fmaxf(lp, -200.f) + H)));     // e^-200 = 0 in fp32: no 0 * inf
+        const float l2 = fmaf(x - off, c, -ref) - logs, pr = __builtin_amdgcn_exp2f(l2);
+        return none ? 0.f : p.t * (g - pr * (A + gH * (LN2 * fmaxf(l2, -300.f) + H)));      // 2^-300 = 0 in fp32: no 0 * inf
     };
     const Groups<T> gr(row, v0, v1);
     const bool same = (((uintptr_t)(out + v0) ^ (uintptr_t)(row + v0)) & 15) == 0;
