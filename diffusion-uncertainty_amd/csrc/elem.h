@@ -40,6 +40,7 @@ static inline bool dua_dtype_ok(int dt) { return dt == DUA_DTYPE_F32 || dt == DU
 template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_add(float v) {
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xF, false));
 }
+template <int CTRL> __device__ __forceinline__ float dpp_move(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true)); }
 __device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
 __device__ __forceinline__ float row_scan(float v) {          // lane 15 of every 16: the sum of its row
     v = dpp_add<0x111, 0xF>(v);

@@ -104,20 +104,6 @@ __device__ __forceinline__ void load_lut(const AttP& p, int h, int pad, float* l
 
 template <typename T> using Vec16 = typename VecOf<T, Elem<T>::VEC>::type;
 
-// 16 bytes of a row at column c, zero at and past ch
-template <typename T>
-__device__ __forceinline__ Vec16<T> load16(const T* row, int c, int ch) {
-    constexpr int V = Elem<T>::VEC;
-    if (c + V <= ch) return *(const typename MemVec<T, V>::type*)(row + c);
-    Vec16<T> r;
-#pragma unroll
-    for (int j = 0; j < V; ++j) r[j] = (T)0.f;
-    if (c < ch) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) r[j] = c + j < ch ? row[c + j] : (T)0.f;
-    }
-    return r;
-}
 template <typename T>
 __device__ __forceinline__ Vec16<T> zero16() {
     Vec16<T> r;
@@ -125,32 +111,62 @@ __device__ __forceinline__ Vec16<T> zero16() {
     for (int j = 0; j < Elem<T>::VEC; ++j) r[j] = (T)0.f;
     return r;
 }
+// 16 bytes of a row from column c on, zeros at and past ch: the load is whole and unconditional (from the row's own elements where it would stick
+// out), what does not count is zeroed when it is used.  Loads behind lanes' conditions would be waited for at once: the zeros go to their registers.
+template <typename T>
+__device__ __forceinline__ Vec16<T> load16(const T* row, int c, int ch) {
+    constexpr int V = Elem<T>::VEC;
+    if (ch >= V) return *(const typename MemVec<T, V>::type*)(row + min(c, ch - V));
+    Vec16<T> r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) r[j] = row[min(j, ch - 1)];
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ Vec16<T> keep16(Vec16<T> x, int c, int ch, bool there) {
+    constexpr int V = Elem<T>::VEC;
+    if (ch % V == 0) return there && c < ch ? x : zero16<T>();
+    // a row that ends inside the 16 bytes: they were read up to its end, the elements from c on are their last ones
+    const int shift = max(c - max(ch - V, 0), 0);
+    Vec16<T> r = zero16<T>();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        T e = (T)0.f;
+#pragma unroll
+        for (int i = j; i < V; ++i) e = i == j + shift ? x[i] : e;
+        r[j] = there && c + j < ch ? e : (T)0.f;
+    }
+    return r;
+}
 
-// A lane's part of a fragment from global memory (16 bytes); a row that is not there reads as zeros
+// A lane's part of a fragment from global memory (16 bytes); a row that is not there (`row` may be any that is) reads as zeros
 template <typename T>
 __device__ __forceinline__ typename Frag<T>::type row_frag_global(const T* row, int c, int ch, bool there) {
     static_assert(Frag<T>::N == Elem<T>::VEC, "a lane's part of a fragment is 16 bytes");
-    return there ? load16<T>(row, c, ch) : zero16<T>();
+    return keep16<T>(load16<T>(row, c, ch), c, ch, there);
 }
 
 // A tile of ROWS rows on its way from global memory through registers to LDS: the loads of the next tile are in flight while the present one
-// is multiplied.  Rows at and past n and the columns past ch are zeros.
+// is multiplied.  Rows at and past n (n > 0) and the columns past ch are zeros.
 template <typename T, int CHP, int ROWS, int THREADS = NTHR> struct Carrier {
     static constexpr int V = Elem<T>::VEC, C = Shape<T, CHP>::KW / V, P = Shape<T, CHP>::PITCH, N = (ROWS * C + THREADS - 1) / THREADS;
     static constexpr bool EVEN = ROWS * C % THREADS == 0;
     Vec16<T> x[N];
+    int rows;
     __device__ __forceinline__ void fetch(const T* src, long stride, int n, int ch, int tid) {
+        rows = n;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int i = tid + u * THREADS, r = i / C, c = i % C * V;
-            x[u] = r < n && (EVEN || r < ROWS) ? load16<T>(src + r * stride, c, ch) : zero16<T>();
+            x[u] = load16<T>(src + min(r, min(n, ROWS) - 1) * stride, c, ch);
         }
     }
-    __device__ __forceinline__ void put(T* tile, int tid) const {
+    __device__ __forceinline__ void put(T* tile, int ch, int tid) const {
+        const bool whole = rows >= ROWS && ch == Shape<T, CHP>::KW;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int i = tid + u * THREADS, r = i / C, c = i % C * V;
-            if (EVEN || r < ROWS) *(Vec16<T>*)(tile + r * P + c) = x[u];
+            if (EVEN || r < ROWS) *(Vec16<T>*)(tile + r * P + c) = whole ? x[u] : keep16<T>(x[u], c, ch, r < rows);
         }
     }
 };

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
     for (int i = 0; i < NQ; ++i) {
         const int q = qw + 16 * i + (lane & 15);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[i][s] = row_frag_global<T>(qp + q * p.qr, S::KSTEP * s + Frag<T>::N * g, p.ch, q < p.Tq);
+        for (int s = 0; s < KS; ++s) qf[i][s] = row_frag_global<T>(qp + min(q, p.Tq - 1) * p.qr, S::KSTEP * s + Frag<T>::N * g, p.ch, q < p.Tq);
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
@@ -79,8 +79,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
     for (int t = t0; t < t1; ++t) {
         T* const Kt = tiles + (t & 1) * 2 * KT * P;
         T* const Vt = Kt + KT * P;
-        ck.put(Kt, tid);
-        cv.put(Vt, tid);
+        ck.put(Kt, p.ch, tid);
+        cv.put(Vt, p.ch, tid);
         __syncthreads();                                                    // (the other pair of tiles is read until here)
         const int k0 = t * KT;
         if (t + 1 < t1) {
@@ -175,9 +175,9 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
     auto fetch_k = [&](int t) {
 #pragma unroll
         for (int n = 0; n < N16; ++n) {
-            const int key = t * KT + 16 * n + col;
+            const int key = min(t * KT + 16 * n + col, nk - 1);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) kf[n][s] = row_frag_global<T>(kp + key * p.kr, S::KSTEP * s + Frag<T>::N * g, p.ch, key < nk);
+            for (int s = 0; s < KS; ++s) kf[n][s] = load16<T>(kp + key * p.kr, S::KSTEP * s + Frag<T>::N * g, p.ch);
         }
     };
     if (t0 + wave < t1) {
@@ -196,15 +196,20 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
     for (int t = t0 + wave; t < t1; t += NWAVE) {
         const int k0 = t * KT;
         f32x4 s[N16];
+        const bool whole = k0 + KT <= nk && p.ch == S::KW;
 #pragma unroll
         for (int n = 0; n < N16; ++n) {
             s[n] = ZERO4;
+            if (!whole) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) kf[n][ks] = keep16<T>(kf[n][ks], S::KSTEP * ks + Frag<T>::N * g, p.ch, k0 + 16 * n + col < nk);
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) s[n] = mma(kf[n][ks], qf[ks], s[n]);
         }
         if (t + NWAVE < t1) fetch_k(t + NWAVE);
         __builtin_amdgcn_wave_barrier();                                    // (the tile is this wave's own; LDS keeps a wave's order)
-        cv.put(Vt, lane);
+        cv.put(Vt, p.ch, lane);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (t + NWAVE < t1) cv.fetch(vp + (long)(k0 + NWAVE * KT) * p.vr, p.vr, nk - k0 - NWAVE * KT, p.ch, lane);

@@ -6,12 +6,9 @@ namespace {
 // ------------------------------------------------------------------------------------------------------------------ diagonals
 // Sums along the diagonals of a 16 x 16 block x (row 4 g + r, column c of lane 16 g + c): lane (g, c) of `a` collects diagonal row - column =
 // 4 g - c, of `b` (c >= 13) diagonal 4 g + 16 - c.  A lane's four rows are shifted along its 16 columns, zeros coming in.
-template <int CTRL> __device__ __forceinline__ float dpp_in(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
-}
 __device__ __forceinline__ void diagonals(f32x4 x, float& a, float& b) {
-    a = x[0] + dpp_in<0x101>(x[1]) + dpp_in<0x102>(x[2]) + dpp_in<0x103>(x[3]);      // row_shl: from the column 1, 2, 3 to the right
-    b = dpp_in<0x11F>(x[1]) + dpp_in<0x11E>(x[2]) + dpp_in<0x11D>(x[3]);              // row_shr by 15, 14, 13: what left the row there
+    a = x[0] + dpp_move<0x101>(x[1]) + dpp_move<0x102>(x[2]) + dpp_move<0x103>(x[3]);      // row_shl: from the column 1, 2, 3 to the right
+    b = dpp_move<0x11F>(x[1]) + dpp_move<0x11E>(x[2]) + dpp_move<0x11D>(x[3]);              // row_shr by 15, 14, 13: what left the row there
 }
 
 // The four waves' sums along the diagonals (diag [wave][nl], distance 0 at R + pad) clipped to 2R + 1 distances, into this workgroup's row of the
@@ -72,15 +69,16 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
     for (int i = 0; i < NQ; ++i) {
         const int q = qw + 16 * i + (lane & 15);
         const bool there = q < p.Tq;
+        const int qr = min(q, p.Tq - 1);
         float d = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int c = S::KSTEP * s + Frag<T>::N * g;
-            qf[i][s] = row_frag_global<T>(qp + q * p.qr, c, p.ch, there);
-            df[i][s] = row_frag_global<T>(dp + q * p.dr, c, p.ch, there);
-            const frag of = row_frag_global<T>(op + q * p.orow, c, p.ch, there);
+            qf[i][s] = row_frag_global<T>(qp + qr * p.qr, c, p.ch, there);
+            df[i][s] = row_frag_global<T>(dp + qr * p.dr, c, p.ch, there);
+            const frag of = row_frag_global<T>(op + qr * p.orow, c, p.ch, there);
             frag lo = zero16<T>();                                          // the output's rounding: D's error would be the gradients' largest
-            if (sizeof(T) == 2 && p.olo_in) lo = row_frag_global<T>((const T*)p.olo_in + (row0 + q) * p.ch, c, p.ch, there);
+            if (sizeof(T) == 2 && p.olo_in) lo = row_frag_global<T>((const T*)p.olo_in + (row0 + qr) * p.ch, c, p.ch, there);
 #pragma unroll
             for (int j = 0; j < Frag<T>::N; ++j) d += (float)df[i][s][j] * ((float)of[j] + (float)lo[j]);
         }
@@ -97,8 +95,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
     for (int k0 = 0, t = 0; k0 < kend; k0 += KT, ++t) {
         T* const Kt = tiles + (t & 1) * 2 * KT * P;
         T* const Vt = Kt + KT * P;
-        ck.put(Kt, tid);
-        cv.put(Vt, tid);
+        ck.put(Kt, p.ch, tid);
+        cv.put(Vt, p.ch, tid);
         __syncthreads();
         if (k0 + KT < kend) {
             ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, nk - k0 - KT, p.ch, tid);
@@ -219,8 +217,9 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int c = S::KSTEP * s + Frag<T>::N * g;
-            kf[i][s] = row_frag_global<T>(kp + kk * p.kr, c, p.ch, kk < nk);
-            vf[i][s] = row_frag_global<T>(vp + kk * p.vr, c, p.ch, kk < nk);
+            const int kr = min(kk, max(nk - 1, 0));
+            kf[i][s] = row_frag_global<T>(kp + kr * p.kr, c, p.ch, kk < nk);
+            vf[i][s] = row_frag_global<T>(vp + kr * p.vr, c, p.ch, kk < nk);
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c) { ak[i][c] = ZERO4; av[i][c] = ZERO4; }
@@ -255,8 +254,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
         T* const Qt = tiles + (t & 1) * 2 * QT * P;
         T* const Dt = Qt + QT * P;
         float* const row_ls = rows + (t & 1) * 2 * QT, *const row_d = row_ls + QT;
-        cq.put(Qt, tid);
-        cd.put(Dt, tid);
+        cq.put(Qt, p.ch, tid);
+        cd.put(Dt, p.ch, tid);
         if (tid < QT) row_ls[tid] = row_next == -INFINITY ? INFINITY : row_next * LOG2E;   // no keys, no query: P = 0
         else if (tid < 2 * QT) row_ls[tid] = row_next;
         __syncthreads();

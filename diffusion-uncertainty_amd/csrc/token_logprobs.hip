@@ -56,7 +56,7 @@ struct LogpP {
     long rows, ld, V;
     int k, splits;
     float t;
-    float* part;                                      // [rows][splits][4 + 2 k]: ref, s, w, huge ; values ; indices (as int32 bits, within V < 2^31)
+    float* part;                                      // [rows][splits][4 + 2 k]: ref, s, w, huge ; values ; indices (as int32 bits, within V < 2^30)
     // backward
     const float *dlp, *dent, *dtop;
     const int64_t* tids;
@@ -64,24 +64,28 @@ struct LogpP {
     long ldd;
 };
 
-// The 16-byte groups of elements [v0, v1) of a row: group g holds elements first + g * VEC ... ; the first and last may stick out.
+// The 16-byte groups of elements [v0, v1) of a row: group g holds elements first + g * VEC ... ; only the first and the last may stick out.
 template <typename T> struct Groups {
     static constexpr int VEC = Elem<T>::VEC;
-    const T* row;
-    long first, v0, v1, n;
-    __device__ Groups(const T* r, long a, long b) : row(r), v0(a), v1(b) {
-        const long mis = (long)(((uintptr_t)(r + a) & 15) / sizeof(T));
-        first = a - mis;
-        n = (b - first + VEC - 1) / VEC;
+    const T* base;                                           // of group 0 (16-byte aligned; may lie before the row)
+    long first;
+    int lead, n, last;                                       // elements before v0 in group 0; groups; elements of the last group
+    __device__ Groups(const T* row, long v0, long v1) {
+        lead = (int)(((uintptr_t)(row + v0) & 15) / sizeof(T));
+        first = v0 - lead;
+        base = row + first;
+        n = (int)((v1 - first + VEC - 1) / VEC);
+        last = (int)(v1 - first - (long)(n - 1) * VEC);
     }
-    __device__ __forceinline__ bool whole(long g) const { return first + g * VEC >= v0 && first + (g + 1) * VEC <= v1; }
-    __device__ __forceinline__ void load(long g, float* f) const {                       // elements outside [v0, v1): -inf
-        const long e = first + g * VEC;
+    __device__ __forceinline__ bool whole(int g) const { return (g > 0 || lead == 0) && (g < n - 1 || last == VEC); }
+    __device__ __forceinline__ bool holds(int g, int j) const { return (g > 0 || j >= lead) && (g < n - 1 || j < last); }
+    __device__ __forceinline__ void load(int g, float* f) const {                        // elements outside [v0, v1): -inf
+        const T* p = (const T*)((const char*)base + 16u * (unsigned)g);                  // (rows of less than 4 GB)
         if (whole(g)) {
-            ld_elems<T, VEC>(row + e, f);
+            ld_elems<T, VEC>(p, f);
         } else {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f[j] = e + j >= v0 && e + j < v1 ? (float)row[e + j] : -INFINITY;
+            for (int j = 0; j < VEC; ++j) f[j] = holds(g, j) ? (float)p[j] : -INFINITY;
         }
     }
 };
@@ -119,15 +123,16 @@ __device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
     const int tid = threadIdx.x;
     int cur = 0;
     long have = 0;
-    for (long g0 = 0; g0 < gr.n; g0 += NT) {
-        const long g = g0 + tid, e0 = gr.first + g * VEC;
+    for (int g0 = 0; g0 < gr.n; g0 += NT) {
+        const int g = g0 + tid;
+        const long e0 = gr.first + (long)g * VEC;
         float f[VEC];
         uint32_t best = 0;                                     // 0: below every float's key
         if (g < gr.n) {
             gr.load(g, f);
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if (e0 + j >= gr.v0 && e0 + j < gr.v1) best = max(best, okey(f[j]));
+                if (gr.holds(g, j)) best = max(best, okey(f[j]));
         }
         __syncthreads();
         if (tid == 0) { sh.any = 0; sh.ncand = 0; }
@@ -140,7 +145,7 @@ __device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
         if (best > bar && rank_of_thread(sh.key, best, tid) < k) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if (e0 + j >= gr.v0 && e0 + j < gr.v1 && okey(f[j]) > bar) {
+                if (gr.holds(g, j) && okey(f[j]) > bar) {
                     const int at = atomicAdd(&sh.ncand, 1);     // at most k * VEC <= 512: fits
                     sh.ck[at] = okey(f[j]);
                     sh.ci[at] = (int)(e0 + j);
@@ -184,7 +189,7 @@ template <typename T>
 __device__ Soft scan_huge(const Groups<T>& gr, float c, Soft* soft) {
     constexpr int VEC = Elem<T>::VEC;
     Soft a{-FLT_MAX, 0.f, 0.f};
-    for (long g = threadIdx.x; g < gr.n; g += NT) {
+    for (int g = threadIdx.x; g < gr.n; g += NT) {
         float f[VEC], m = a.ref;
         gr.load(g, f);
 #pragma unroll
@@ -208,12 +213,21 @@ __device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared&
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Groups<T> gr(row, v0, v1);
     Soft a{-REF_MAX, 0.f, 0.f};
-    float b1 = -INFINITY, b2 = -INFINITY;                 // best value, best value outside the best group
+    float b1 = -INFINITY, b2 = -INFINITY;                 // best value, best value outside the best pair of groups (g, g + NT)
     int bg = -1;
-    auto eat = [&](const float* f, int g) {
+    const int n = gr.n;
+    for (int g = tid; g < n; g += 2 * NT) {
+        float f[2 * VEC];
+        gr.load(g, f);
+        if (g + NT < n) {
+            gr.load(g + NT, f + VEC);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[VEC + j] = -INFINITY;
+        }
         float vm = f[0];
 #pragma unroll
-        for (int j = 1; j < VEC; ++j) vm = fmaxf(vm, f[j]);
+        for (int j = 1; j < 2 * VEC; ++j) vm = fmaxf(vm, f[j]);
         b2 = fmaxf(b2, fminf(b1, vm));
         bg = vm > b1 || bg < 0 ? g : bg;
         b1 = fmaxf(b1, vm);
@@ -224,25 +238,11 @@ __device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared&
             a.ref = ref;
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
+        for (int j = 0; j < 2 * VEC; ++j) {
             const float d = fmaf(f[j], c, -a.ref), e = __builtin_amdgcn_exp2f(d);
             a.s += e;
             a.w += e * fmaxf(d, -150.f);                  // 2^-150 = 0: e is 0 wherever the clamp acts, and 0 * -inf does not arise
         }
-    };
-    const int n = (int)gr.n;
-    int g = tid;
-    for (; g + NT < n; g += 2 * NT) {
-        float f0[VEC], f1[VEC];
-        gr.load(g, f0);
-        gr.load(g + NT, f1);
-        eat(f0, g);
-        eat(f1, g + NT);
-    }
-    if (g < n) {
-        float f0[VEC];
-        gr.load(g, f0);
-        eat(f0, g);
     }
     const uint32_t mine = bg < 0 ? 0u : okey(b1);
     // a bound of the k-th value from the maxima of 64, 128 or 256 sets of threads: the smallest of the k largest maxima
@@ -274,36 +274,34 @@ __device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared&
         }
         __syncthreads();
         const uint32_t tau = sh.tau;                       // 0: fewer than k sets hold elements - every element is a candidate
-        auto push = [&](long e, float x) {
-            if (e >= gr.v0 && e < gr.v1 && okey(x) >= tau) {
-                const int at = atomicAdd(&sh.ncand, 1);
-                if (at < CAP) { sh.ck[at] = okey(x); sh.ci[at] = (int)e; }
-            }
+        auto push = [&](int g) {                            // a group's elements that reach the bound
+            if (g >= n) return;
+            float f[VEC];
+            gr.load(g, f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (gr.holds(g, j) && okey(f[j]) >= tau) {
+                    const int at = atomicAdd(&sh.ncand, 1);
+                    if (at < CAP) { sh.ck[at] = okey(f[j]); sh.ci[at] = (int)(gr.first + (long)g * VEC + j); }
+                }
         };
         if (bg >= 0 && mine >= tau) {
-            const bool more = n > NT && okey(b2) >= tau;    // (with one group a thread there is no value outside it)
+            const bool more = n > 2 * NT && okey(b2) >= tau;   // (with one pair a thread there is no value outside it)
             if (more && b2 == -INFINITY) {
                 sh.any = 1;                                 // the bound itself is -inf: too few finite values
             } else if (more) {
                 const int at = atomicAdd(&sh.nrescan, 1);
                 if (at < RESCAN) sh.rescan[at] = tid;
             } else {
-                float f[VEC];
-                gr.load(bg, f);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) push(gr.first + (long)bg * VEC + j, f[j]);
+                push(bg);
+                push(bg + NT);
             }
         }
         __syncthreads();
         const int nr = sh.nrescan;
         if (nr <= RESCAN && !sh.any) {
             for (int i = wave; i < nr; i += NW)
-                for (int gg = sh.rescan[i] + lane * NT; gg < n; gg += 64 * NT) {
-                    float f[VEC];
-                    gr.load(gg, f);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) push(gr.first + (long)gg * VEC + j, f[j]);
-                }
+                for (int gg = sh.rescan[i] + lane * NT; gg < n; gg += 64 * NT) push(gg);
             __syncthreads();
             const int nc = sh.ncand;
             if (nc <= CAP) {
@@ -386,17 +384,19 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_join(LogpP p) {
     const long r = blockIdx.x;
     const float *q = p.part + r * p.splits * (4 + 2 * p.k), c = p.t * LOG2E;
     // Parts summed relative to a logit (sum 0: nothing finite in them) do not mix with the others; far below them (a part that is masked with
-    // the type's lowest value) they add nothing, else the row is summed again here.
-    Soft a{-REF_MAX, 0.f, 0.f};
-    bool huge = false, low = false;
-    uint32_t tau = 0;                                       // the best of the parts' k-th values bounds the row's k-th from below
-    for (int i = 0; i < p.splits; ++i) {
-        const float* o = q + i * (4 + 2 * p.k);
-        if (o[3] == 0.f) a = soft_join(a, Soft{o[0], o[1], o[2]}, 1.f);
-        else if (o[1] != 0.f) (o[1] < INFINITY && o[0] < 0.f ? low : huge) = true;
-        if (p.k) tau = max(tau, __float_as_uint(o[4 + p.k - 1]));
+    // the type's lowest value) they add nothing, else the row is summed again here.  A lane a part, every wave the same.
+    const int i = threadIdx.x & 63;
+    const float* o = q + (i < p.splits ? i : 0) * (4 + 2 * p.k);
+    const float o0 = o[0], o1 = o[1], o2 = o[2], o3 = o[3];
+    uint32_t tau = p.k ? __float_as_uint(o[4 + p.k - 1]) : 0;  // the best of the parts' k-th values bounds the row's k-th from below
+    const bool in = i < p.splits, odd = in && o3 != 0.f && o1 != 0.f, low = odd && o1 < INFINITY && o0 < 0.f;
+    Soft a = in && o3 == 0.f ? Soft{o0, o1, o2} : Soft{-REF_MAX, 0.f, 0.f};
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) {
+        a = soft_join(a, Soft{__shfl_xor(a.ref, x, 64), __shfl_xor(a.s, x, 64), __shfl_xor(a.w, x, 64)}, 1.f);
+        tau = max(tau, (uint32_t)__shfl_xor((int)tau, x, 64));
     }
-    huge = huge || (low && a.ref < -0.5f * REF_MAX);
+    const bool huge = __any(odd && !low) || (__any(low) && a.ref < -0.5f * REF_MAX);
     if (huge) a = scan_huge(Groups<T>((const T*)p.x + r * p.ld, 0, p.V), c, soft);
     if (threadIdx.x == 0) n = 0;
     __syncthreads();
@@ -467,19 +467,19 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_bwd(LogpP p) {
         return none ? 0.f : p.t * (g - pr * (A + gH * (LN2 * fmaxf(l2, -300.f) + H)));      // 2^-300 = 0 in fp32: no 0 * inf
     };
     const Groups<T> gr(row, v0, v1);
-    const bool same = (((uintptr_t)(out + v0) ^ (uintptr_t)(row + v0)) & 15) == 0;
-    for (long g = tid; g < gr.n; g += NT) {
+    T* const obase = out + gr.first;
+    for (int g = tid; g < gr.n; g += NT) {
         float f[VEC];
         gr.load(g, f);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) f[j] = grad(f[j], 0.f);
-        const long e = gr.first + g * VEC;
-        if (same && gr.whole(g)) {
-            st_elems<T, VEC>(out + e, f);
+        T* const o = (T*)((char*)obase + 16u * (unsigned)g);
+        if (gr.whole(g)) {
+            st_elems<T, VEC>(o, f);                         // (rows of dx may lie at another alignment)
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if (e + j >= v0 && e + j < v1) out[e + j] = (T)f[j];
+                if (gr.holds(g, j)) o[j] = (T)f[j];
         }
     }
     __syncthreads();                                        // (orders this workgroup's stores: the special tokens are written last)
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_bwd(LogpP p) {
 int check_common(const dua_token_logprobs_args* a, const char* who) {
     DUA_REQUIRE(a, "%s: null arguments", who);
     DUA_REQUIRE(dua_dtype_ok(a->dtype), "%s: dtype must be fp32, bf16 or fp16", who);
-    DUA_REQUIRE(a->rows >= 0 && a->rows < (1L << 24) && a->V >= 1 && a->V < (1L << 31) - 64 && a->ld >= a->V, "%s: rows in [0, 2^24), V in [1, 2^31 - 64), ld >= V", who);
+    DUA_REQUIRE(a->rows >= 0 && a->rows < (1L << 24) && a->V >= 1 && a->V < (1L << 30) && a->ld >= a->V, "%s: rows in [0, 2^24), V in [1, 2^30), ld >= V", who);
     DUA_REQUIRE(a->k >= 0 && a->k <= KMAX && a->k <= a->V, "%s: k must be in [0, %d] and at most V", who, KMAX);
     DUA_REQUIRE(a->inv_temperature > 0.f && a->inv_temperature < INFINITY, "%s: inv_temperature must be positive and finite", who);
     DUA_REQUIRE(a->rows == 0 || (a->logits && a->stats && ((uintptr_t)a->stats & 15) == 0), "%s: null logits / stats, or stats not 16-byte aligned", who);

@@ -321,6 +321,13 @@ def test_sandwich_norm_gradient_chunks(shape, gate_rows):
     norm_case(torch.float32, shape, "rms", "layer", gate_rows)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D,gate_rows", [(3, 211), (64, 0), (65, 422), (127, 1), (128, 2), (130, 0), (250, 422), (257, 0), (511, 2), (513, 211), (2049, 0), (4096, 2)])
+def test_sandwich_norm_units_of_every_width(dt, D, gate_rows):
+    """Rows held by 16 or 32 lanes, a wavefront, up to 16 wavefronts, and the widths around each border; 422 rows."""
+    norm_case(dt, (422, D), "layer", "rms", gate_rows, seed=D)
+
+
 def test_sandwich_norm_large_offset_and_constant_rows():
     """LayerNorm of rows whose mean is far from zero (two-pass variance) and of constant rows (variance 0: 1 / std = eps^-1/2)."""
     from diffusion_uncertainty_amd import ops
