@@ -111,33 +111,13 @@ __device__ __forceinline__ Vec16<T> zero16() {
     for (int j = 0; j < Elem<T>::VEC; ++j) r[j] = (T)0.f;
     return r;
 }
-// 16 bytes of a row from column c on, zeros at and past ch: the load is whole and unconditional (from the row's own elements where it would stick
-// out), what does not count is zeroed when it is used.  Loads behind lanes' conditions would be waited for at once: the zeros go to their registers.
+// 16 bytes of a row from column c on, zeros at and past ch (a multiple of 16 bytes): the load is unconditional, from the row's own elements where
+// there are none, and what does not count is zeroed when it is used.  (Loads behind lanes' conditions are waited for at once: the zeros
+// go to their registers.)
 template <typename T>
-__device__ __forceinline__ Vec16<T> load16(const T* row, int c, int ch) {
-    constexpr int V = Elem<T>::VEC;
-    if (ch >= V) return *(const typename MemVec<T, V>::type*)(row + min(c, ch - V));
-    Vec16<T> r;
-#pragma unroll
-    for (int j = 0; j < V; ++j) r[j] = row[min(j, ch - 1)];
-    return r;
-}
+__device__ __forceinline__ Vec16<T> load16(const T* row, int c, int ch) { return *(const typename MemVec<T, Elem<T>::VEC>::type*)(row + min(c, ch - Elem<T>::VEC)); }
 template <typename T>
-__device__ __forceinline__ Vec16<T> keep16(Vec16<T> x, int c, int ch, bool there) {
-    constexpr int V = Elem<T>::VEC;
-    if (ch % V == 0) return there && c < ch ? x : zero16<T>();
-    // a row that ends inside the 16 bytes: they were read up to its end, the elements from c on are their last ones
-    const int shift = max(c - max(ch - V, 0), 0);
-    Vec16<T> r = zero16<T>();
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        T e = (T)0.f;
-#pragma unroll
-        for (int i = j; i < V; ++i) e = i == j + shift ? x[i] : e;
-        r[j] = there && c + j < ch ? e : (T)0.f;
-    }
-    return r;
-}
+__device__ __forceinline__ Vec16<T> keep16(Vec16<T> x, int c, int ch, bool there) { return there && c < ch ? x : zero16<T>(); }
 
 // A lane's part of a fragment from global memory (16 bytes); a row that is not there (`row` may be any that is) reads as zeros
 template <typename T>
@@ -152,21 +132,40 @@ template <typename T, int CHP, int ROWS, int THREADS = NTHR> struct Carrier {
     static constexpr int V = Elem<T>::VEC, C = Shape<T, CHP>::KW / V, P = Shape<T, CHP>::PITCH, N = (ROWS * C + THREADS - 1) / THREADS;
     static constexpr bool EVEN = ROWS * C % THREADS == 0;
     Vec16<T> x[N];
+    unsigned off[N];                                         // bytes from a tile's first row (row strides are below 2^24 elements)
     int rows;
+    __device__ __forceinline__ Carrier(long stride, int ch, int tid) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) off[u] = at(u, ROWS, stride, ch, tid);
+    }
+    __device__ static __forceinline__ unsigned at(int u, int n, long stride, int ch, int tid) {
+        const int i = tid + u * THREADS, r = i / C, c = i % C * V;
+        return ((unsigned)min(r, n - 1) * (unsigned)stride + (unsigned)min(c, ch - V)) * (unsigned)sizeof(T);
+    }
     __device__ __forceinline__ void fetch(const T* src, long stride, int n, int ch, int tid) {
         rows = n;
+        const char* s = (const char*)src;
+        if (n >= ROWS) {
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int i = tid + u * THREADS, r = i / C, c = i % C * V;
-            x[u] = load16<T>(src + min(r, min(n, ROWS) - 1) * stride, c, ch);
+            for (int u = 0; u < N; ++u) x[u] = *(const typename MemVec<T, V>::type*)(s + off[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u) x[u] = *(const typename MemVec<T, V>::type*)(s + at(u, n, stride, ch, tid));
         }
     }
     __device__ __forceinline__ void put(T* tile, int ch, int tid) const {
-        const bool whole = rows >= ROWS && ch == Shape<T, CHP>::KW;
+        if (rows >= ROWS && ch == Shape<T, CHP>::KW) {
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int i = tid + u * THREADS, r = i / C, c = i % C * V;
-            if (EVEN || r < ROWS) *(Vec16<T>*)(tile + r * P + c) = whole ? x[u] : keep16<T>(x[u], c, ch, r < rows);
+            for (int u = 0; u < N; ++u) {
+                const int i = tid + u * THREADS, r = i / C, c = i % C * V;
+                if (EVEN || r < ROWS) *(Vec16<T>*)(tile + r * P + c) = x[u];
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int i = tid + u * THREADS, r = i / C, c = i % C * V;
+                if (EVEN || r < ROWS) *(Vec16<T>*)(tile + r * P + c) = keep16<T>(x[u], c, ch, r < rows);
+            }
         }
     }
 };
@@ -210,16 +209,11 @@ __device__ __forceinline__ typename Frag<T>::type acc_frag(const f32x4* a) {
 // four consecutive channels of a row
 template <typename T>
 __device__ __forceinline__ void store4(T* row, int c, int ch, f32x4 v) {
-    if (c + 4 <= ch) {
-        typename VecOf<T, 4>::type x;
+    if (c >= ch) return;
+    typename VecOf<T, 4>::type x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = (T)v[j];
-        *(typename MemVec<T, 4>::type*)(row + c) = x;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c + j < ch) row[c + j] = (T)v[j];
-    }
+    for (int j = 0; j < 4; ++j) x[j] = (T)v[j];
+    *(typename MemVec<T, 4>::type*)(row + c) = x;
 }
 // what the rounding to T left of v
 template <typename T>
@@ -290,8 +284,11 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
                 "%s: dtype must be fp32, bf16 or fp16 and the table's fp32 or the same", who);
     DUA_REQUIRE(a->B >= 0 && a->Tq >= 0 && a->Tk >= 0 && a->Tq < (1 << 29) && a->Tk < (1 << 29), "%s: lengths must be in [0, 2^29)", who);
     DUA_REQUIRE(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0 && a->heads <= 65535, "%s: kv_heads must divide heads (at most 65535)", who);
-    DUA_REQUIRE(a->ch >= 1 && a->ch <= 128, "%s: head width must be in [1, 128]", who);
+    DUA_REQUIRE(a->ch >= 1 && a->ch <= 128 && a->ch * dua_dtype_size(a->dtype) % 16 == 0,
+                "%s: head width must be a multiple of 8 (fp32: 4) up to 128", who);
     DUA_REQUIRE(a->radius >= 1 && a->radius <= RMAX && a->num_buckets >= 1, "%s: radius must be in [1, %d]", who, RMAX);
+    for (long r : {a->q_row, a->k_row, a->v_row, a->out_row, a->dout_row, a->dq_row, a->dk_row, a->dv_row})
+        DUA_REQUIRE(r >= 0 && r < (1L << 24), "%s: row strides must be in [0, 2^24) elements", who);
     DUA_REQUIRE(a->table && a->bucket_map, "%s: null table / bucket map", who);
     DUA_REQUIRE((a->B == 0 || a->Tq == 0 || a->q) && (a->B == 0 || a->Tk == 0 || (a->k && a->v)), "%s: null operand", who);
     DUA_REQUIRE((long)a->B * a->heads * ((a->Tq > a->Tk ? a->Tq : a->Tk) / 64 + 1) < (1L << 23), "%s: too many blocks for one launch", who);

@@ -4,9 +4,6 @@
 namespace {
 
 // -------------------------------------------------------------------------------------------------------------------- forward
-// Row stride of the partial sums: whole 16 bytes
-__device__ __forceinline__ int ch4(const AttP& p) { return (p.ch + 3) & ~3; }
-
 // A row of the result: written, or (keys split over workgroups) left as unnormalised sums with its maximum and sum for the join.
 // o: columns' channels 16 c + 4 (l / 16) + r of one query; m in log2 units, l its whole sum.
 template <typename T, int CT>
@@ -14,7 +11,7 @@ __device__ __forceinline__ void finish_query(const AttP& p, int b, int h, int q,
     const long row = ((long)b * p.H + h) * p.Tq + q;
     if (p.splits > 1) {
         const long at = (long)split * p.B * p.H * p.Tq + row;
-        float* po = p.part + at * ch4(p);
+        float* po = p.part + at * p.ch;
 #pragma unroll
         for (int c = 0; c < CT; ++c)
             if (16 * c + 4 * g < p.ch) *(f32x4*)(po + 16 * c + 4 * g) = o[c];
@@ -52,7 +49,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
     const int nt = (kend + KT - 1) / KT, t0 = (int)((long)nt * split / p.splits), t1 = (int)((long)nt * (split + 1) / p.splits);
     const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
-    Carrier<T, CHP, KT> ck, cv;
+    Carrier<T, CHP, KT> ck(p.kr, p.ch, tid), cv(p.vr, p.ch, tid);
     if (t0 < t1) {
         ck.fetch(kp + (long)t0 * KT * p.kr, p.kr, nk - t0 * KT, p.ch, tid);
         cv.fetch(vp + (long)t0 * KT * p.vr, p.vr, nk - t0 * KT, p.ch, tid);
@@ -170,7 +167,7 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
     const T* vp = (const T*)p.v + b * p.vb + (long)hk * p.ch;
     const T* qp = (const T*)p.q + b * p.qb + q * p.qr + (long)h * p.ch;
     T* const Vt = (T*)(smem + wave * TILE);
-    Carrier<T, CHP, KT, 64> cv;
+    Carrier<T, CHP, KT, 64> cv(p.vr, p.ch, lane);
     frag kf[N16][KS];
     auto fetch_k = [&](int t) {
 #pragma unroll
@@ -308,9 +305,9 @@ __global__ __launch_bounds__(NTHR) void k_rel_attention_join(AttP p) {
     const float L = (red[NWAVE] + red[NWAVE + 1]) + (red[NWAVE + 2] + red[NWAVE + 3]);
     f32x4 a = ZERO4;
     if (c < p.ch) {
-        const float* src = p.part + row * ch4(p) + c;
+        const float* src = p.part + row * p.ch + c;
 #pragma unroll 4
-        for (int s = s0; s < s1; ++s) a += wt[s] * *(const f32x4*)(src + s * rows * ch4(p));
+        for (int s = s0; s < s1; ++s) a += wt[s] * *(const f32x4*)(src + s * rows * p.ch);
     }
     sum[run][tid & 31] = a;
     __syncthreads();
@@ -339,7 +336,7 @@ Plan plan(const dua_rel_attention_args* a) {
 }
 
 // Unnormalised sums of the splits
-size_t split_floats(const dua_rel_attention_args* a, int splits) { return (size_t)splits * a->B * a->heads * a->Tq * ((a->ch + 3) / 4 * 4); }
+size_t split_floats(const dua_rel_attention_args* a, int splits) { return (size_t)splits * a->B * a->heads * a->Tq * a->ch; }
 
 template <typename T, int CHP> struct Fwd {
     static int run(AttP p, bool few, hipStream_t st) {

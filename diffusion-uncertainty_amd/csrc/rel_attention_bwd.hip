@@ -51,7 +51,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
     const int kend = p.causal ? max(0, min(nk, qs + min(q0 + S::QB, p.Tq))) : nk;
     const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
-    Carrier<T, CHP, KT> ck, cv;
+    Carrier<T, CHP, KT> ck(p.kr, p.ch, tid), cv(p.vr, p.ch, tid);
     if (kend > 0) {
         ck.fetch(kp, p.kr, nk, p.ch, tid);
         cv.fetch(vp, p.vr, nk, p.ch, tid);
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
     const int rep = p.H / p.Hk;
     // tiles of queries that see this block's first key (position >= k0), head after head of the group
     const int qbeg = p.causal ? max(0, k0 - qs) / QT : 0, per = max(0, (p.Tq + QT - 1) / QT - qbeg), total = k0 < nk ? per * rep : 0;
-    Carrier<T, CHP, QT> cq, cd;
+    Carrier<T, CHP, QT> cq(p.qr, p.ch, tid), cd(p.dr, p.ch, tid);
     float row_next = 0.f;
     auto fetch = [&](int t) {
         const int h = w.hk * rep + t / per, q0 = (qbeg + t % per) * QT;

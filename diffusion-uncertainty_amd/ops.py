@@ -5,7 +5,6 @@ libdua_hip.so.  All tensors must be contiguous fp32 (or the stated integer type)
 also take bf16 and fp16, and strided views where they say so.
 """
 import collections
-import contextlib
 import ctypes
 import math
 
@@ -1211,25 +1210,19 @@ _NORMS = {None: 0, "rms": 1, "layer": 2}
 
 def _token_tensor(t, name, dtypes, shape=None, device=None, contiguous=True):
     """Checks of an operand of the token operators; contiguous=False asks only for unit stride along the last dimension."""
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and (shape is None or t.shape == shape) and
+            (device is None or t.device == device) and (t.is_contiguous() or (not contiguous and (t.shape[-1] <= 1 or t.stride(-1) == 1)))):
+        return t                                              # (a few microseconds of checks count beside a decoding step)
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name}: the HIP path needs a GPU tensor (got {getattr(t, 'device', type(t))}); "
                            "there is no CPU fallback in this package")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if device is not None and t.device != device:
         raise ValueError(f"{name}: on {t.device}, the other operands on {device}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name}: must be contiguous")
-    if not contiguous and t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}: the last dimension must have unit stride")
-    return t
-
-
-def _on(device):
-    """The call's device as the current one (kernels launch on ITS current stream), whatever the caller's is."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    raise ValueError(f"{name}: must be contiguous" if contiguous else f"{name}: the last dimension must have unit stride")
 
 
 def _a(t):
@@ -1240,37 +1233,48 @@ def _workspace(nbytes, device):
     return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
 
 
+def _launch(device, fn, args, what):
+    """Call a C entry on the current stream of the operands' device, whatever the caller's current device is."""
+    i = device.index
+    if torch.cuda.current_device() == i:
+        rc = fn(ctypes.byref(args), torch.cuda.current_stream(i).cuda_stream)
+    else:
+        with torch.cuda.device(i):
+            rc = fn(ctypes.byref(args), torch.cuda.current_stream(i).cuda_stream)
+    check(rc, what)
+
+
 SandwichNormGrads = collections.namedtuple("SandwichNormGrads", "dx dy dgate dpost_w dpost_b dpre_w dpre_b")
 
 
 def _sandwich_args(x, y, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps):
     if post not in _NORMS or pre not in _NORMS:
         raise ValueError("post / pre: None, 'rms' or 'layer'")
-    _token_tensor(x, "x", tuple(_DTYPES))
+    _token_tensor(x, "x", _DTYPES)
+    dt, dev = x.dtype, x.device
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x: expected [..., D], got {tuple(x.shape)}")
     D = x.shape[-1]
     rows = x.numel() // D
-    _token_tensor(y, "y", (x.dtype,), x.shape, x.device)
-    given = [(n, t) for n, t in (("post_w", post_w), ("post_b", post_b), ("pre_w", pre_w), ("pre_b", pre_b)) if t is not None]
-    pt = given[0][1].dtype if given else (gate.dtype if gate is not None else torch.float32)
-    if pt not in (torch.float32, x.dtype):
-        raise TypeError(f"parameters: expected torch.float32 or {x.dtype}, got {pt}")
-    for n, t in given:
-        if (post if n.startswith("post") else pre) is None:
-            raise ValueError(f"{n}: given for a norm that is off")
-        _token_tensor(t, n, (pt,), (D,), x.device)
+    _token_tensor(y, "y", (dt,), x.shape, dev)
+    pt = next((t.dtype for t in (post_w, pre_w, post_b, pre_b, gate) if t is not None), torch.float32)
+    if pt != dt and pt != torch.float32:
+        raise TypeError(f"parameters: expected torch.float32 or {dt}, got {pt}")
+    for n, t, on in (("post_w", post_w, post), ("post_b", post_b, post), ("pre_w", pre_w, pre), ("pre_b", pre_b, pre)):
+        if t is not None:
+            if on is None:
+                raise ValueError(f"{n}: given for a norm that is off")
+            _token_tensor(t, n, (pt,), (D,), dev)
     gate_rows = 0
     if gate is not None:
-        _token_tensor(gate, "gate", (pt,), None, x.device)
+        _token_tensor(gate, "gate", (pt,), None, dev)
         if gate.shape[-1:] != (D,):
             raise ValueError(f"gate: expected [D] or [rows, D] with D = {D}, got {tuple(gate.shape)}")
         gate_rows = gate.numel() // D
         if gate_rows < 1 or rows % gate_rows:
             raise ValueError(f"gate: its {gate_rows} rows must divide the {rows} rows of x")
-    return SandwichNormArgs(x=_a(x), y=_a(y), dtype=_DTYPES[x.dtype], param_dtype=_DTYPES[pt], rows=rows, D=D, post=_NORMS[post], pre=_NORMS[pre],
-                            post_w=_a(post_w), post_b=_a(post_b), pre_w=_a(pre_w), pre_b=_a(pre_b), gate=_a(gate), gate_rows=gate_rows,
-                            res_scale=float(res_scale), eps=float(eps))
+    return SandwichNormArgs(x.data_ptr(), y.data_ptr(), _DTYPES[dt], _DTYPES[pt], rows, D, _NORMS[post], _NORMS[pre], _a(post_w), _a(post_b),
+                            _a(pre_w), _a(pre_b), _a(gate), gate_rows, res_scale, eps)
 
 
 def sandwich_norm(x, y, post="rms", post_w=None, post_b=None, gate=None, res_scale=1.0, pre="rms", pre_w=None, pre_b=None, eps=1e-6,
@@ -1281,12 +1285,11 @@ def sandwich_norm(x, y, post="rms", post_w=None, post_b=None, gate=None, res_sca
     equal runs of rows of x (a gate per sample, or per token).  Parameters in fp32 or x's type.  want_stats=True: also what the backward
     pass needs."""
     a = _sandwich_args(x, y, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_b, eps)
-    with _on(x.device):
-        r = torch.empty_like(x)
-        z = torch.empty_like(x) if pre is not None else None
-        stats = torch.empty((a.rows, 4), device=x.device, dtype=torch.float32) if want_stats else None
-        a.r, a.z, a.stats = _a(r), _a(z), _a(stats)
-        check(_lib.lib().dua_sandwich_norm(ctypes.byref(a), _stream()), "dua_sandwich_norm")
+    r = torch.empty_like(x)
+    z = torch.empty_like(x) if pre is not None else None
+    stats = torch.empty((a.rows, 4), device=x.device, dtype=torch.float32) if want_stats else None
+    a.r, a.z, a.stats = _a(r), _a(z), _a(stats)
+    _launch(x.device, _lib.lib().dua_sandwich_norm, a, "dua_sandwich_norm")
     return (r, z, stats) if want_stats else (r, z)
 
 
@@ -1301,16 +1304,15 @@ def sandwich_norm_bwd(x, y, stats, dr, dz, post="rms", post_w=None, post_b=None,
         _token_tensor(dz, "dz", (x.dtype,), x.shape, x.device)
     elif dz is not None:
         raise ValueError("dz: given without a pre norm")
-    with _on(x.device):
-        like = lambda t: torch.empty_like(t) if t is not None else None
-        g = SandwichNormGrads(like(x), like(y), like(gate), like(post_w), like(post_b), like(pre_w), like(pre_b))
-        a.stats, a.dr, a.dz, a.dx, a.dy, a.dgate = _a(stats), _a(dr), _a(dz), _a(g.dx), _a(g.dy), _a(g.dgate)
-        a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = _a(g.dpost_w), _a(g.dpost_b), _a(g.dpre_w), _a(g.dpre_b)
-        L = _lib.lib()
-        a.workspace_bytes = L.dua_sandwich_norm_bwd_workspace_bytes(ctypes.byref(a))
-        ws = _workspace(a.workspace_bytes, x.device)
-        a.workspace = _a(ws)
-        check(L.dua_sandwich_norm_bwd(ctypes.byref(a), _stream()), "dua_sandwich_norm_bwd")
+    like = lambda t: torch.empty_like(t) if t is not None else None
+    g = SandwichNormGrads(like(x), like(y), like(gate), like(post_w), like(post_b), like(pre_w), like(pre_b))
+    a.stats, a.dr, a.dz, a.dx, a.dy, a.dgate = _a(stats), _a(dr), _a(dz), _a(g.dx), _a(g.dy), _a(g.dgate)
+    a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = _a(g.dpost_w), _a(g.dpost_b), _a(g.dpre_w), _a(g.dpre_b)
+    L = _lib.lib()
+    a.workspace_bytes = L.dua_sandwich_norm_bwd_workspace_bytes(ctypes.byref(a))
+    ws = _workspace(a.workspace_bytes, x.device)
+    a.workspace = _a(ws)
+    _launch(x.device, L.dua_sandwich_norm_bwd, a, "dua_sandwich_norm_bwd")
     return g
 
 
@@ -1350,29 +1352,29 @@ class RelativeBuckets:
 
 
 def _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart):
-    _token_tensor(q, "q", tuple(_DTYPES), contiguous=False)
+    _token_tensor(q, "q", _DTYPES, contiguous=False)
+    dt, dev = q.dtype, q.device
     kv_heads = heads if kv_heads is None else kv_heads
     if q.dim() != 3 or heads < 1 or kv_heads < 1 or heads % kv_heads or q.shape[2] % heads:
         raise ValueError(f"q: expected [B, Tq, heads * ch] and kv_heads dividing heads, got {tuple(q.shape)}, {heads}, {kv_heads}")
     B, Tq, C = q.shape
     ch = C // heads
-    _token_tensor(k, "k", (q.dtype,), None, q.device, contiguous=False)
+    _token_tensor(k, "k", (dt,), None, dev, contiguous=False)
     if k.dim() != 3 or k.shape[0] != B or k.shape[2] != kv_heads * ch:
         raise ValueError(f"k: expected [{B}, Tk, {kv_heads * ch}], got {tuple(k.shape)}")
-    _token_tensor(v, "v", (q.dtype,), k.shape, q.device, contiguous=False)
-    Tk = k.shape[1]
-    if not isinstance(buckets, RelativeBuckets) or buckets.map.device != q.device:
-        raise ValueError(f"buckets: expected RelativeBuckets on {q.device}")
-    _token_tensor(table, "table", (torch.float32, q.dtype), (buckets.num_buckets, heads), q.device)
+    _token_tensor(v, "v", (dt,), k.shape, dev, contiguous=False)
+    if not isinstance(buckets, RelativeBuckets) or buckets.map.device != dev:
+        raise ValueError(f"buckets: expected RelativeBuckets on {dev}")
+    _token_tensor(table, "table", (torch.float32, dt), (buckets.num_buckets, heads), dev)
     for n, t in (("klen", klen), ("qstart", qstart)):
         if t is not None:
-            _token_tensor(t, n, (torch.int32,), (B,), q.device)
-    a = RelAttentionArgs(q=_a(q), k=_a(k), v=_a(v), dtype=_DTYPES[q.dtype], B=B, Tq=Tq, Tk=Tk, heads=heads, kv_heads=kv_heads, ch=ch,
-                         q_batch=q.stride(0), q_row=q.stride(1), k_batch=k.stride(0), k_row=k.stride(1), v_batch=v.stride(0), v_row=v.stride(1),
-                         table=_a(table), table_dtype=_DTYPES[table.dtype], bucket_map=_a(buckets.map), radius=buckets.radius,
-                         num_buckets=buckets.num_buckets, klen=_a(klen), qstart=_a(qstart), causal=int(bool(causal)),
-                         scale=1.0 / math.sqrt(ch) if scale is None else float(scale))
-    return a
+            _token_tensor(t, n, (torch.int32,), (B,), dev)
+    qb, qr, _ = q.stride()
+    kb, kr, _ = k.stride()
+    vb, vr, _ = v.stride()
+    return RelAttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dt], B, Tq, k.shape[1], heads, kv_heads, ch, qb, qr, kb, kr, vb, vr,
+                            table.data_ptr(), _DTYPES[table.dtype], buckets.map.data_ptr(), buckets.radius, buckets.num_buckets, _a(klen), _a(qstart),
+                            int(bool(causal)), 1.0 / math.sqrt(ch) if scale is None else scale)
 
 
 RelAttentionSaved = collections.namedtuple("RelAttentionSaved", "lse out_lo")
@@ -1382,20 +1384,21 @@ def rel_attention(q, k, v, table, buckets, heads, kv_heads=None, causal=False, s
     """Multi-head attention with a learned relative position bias, fused (neither scores nor bias in HBM):
     softmax(scale q k^T + table[bucket(j - p_i), h]) v, p_i = qstart[b] + i, over keys j < klen[b] and, if causal, j <= p_i -> [B, Tq, heads * ch].
     q [B, Tq, heads * ch], k / v [B, Tk, kv_heads * ch] (views with unit stride along the last dimension: thirds of a qkv projection, slots
-    of a cache), head widths up to 128; query head h attends to kv head h // (heads // kv_heads); table [num_buckets, heads] in fp32 or q's
+    of a cache), head widths up to 128 in multiples of 8 (fp32: 4); query head h attends to kv head h // (heads // kv_heads); table [num_buckets, heads] in fp32 or q's
     type; klen / qstart int32 [B].  A query without keys gives zeros; keys behind klen are not read.  Tq = 1 with qstart = klen - 1
     is decoding.  want_lse=True: also RelAttentionSaved(lse [B, heads, Tq] = log sum e^s, out_lo: what out's rounding left), for the backward pass."""
     a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
-    with _on(q.device):
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        lse = torch.empty((a.B, heads, a.Tq), device=q.device, dtype=torch.float32) if want_lse else None
-        lo = torch.empty((a.B, heads, a.Tq, a.ch), device=q.device, dtype=q.dtype) if want_lse and q.dtype != torch.float32 else None
-        a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1), _a(lse), _a(lo)
-        L = _lib.lib()
-        a.workspace_bytes = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 0)
-        ws = _workspace(a.workspace_bytes, q.device)
-        a.workspace = _a(ws)
-        check(L.dua_rel_attention(ctypes.byref(a), _stream()), "dua_rel_attention")
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = lo = None
+    if want_lse:
+        lse = torch.empty((a.B, heads, a.Tq), device=q.device, dtype=torch.float32)
+        lo = torch.empty((a.B, heads, a.Tq, a.ch), device=q.device, dtype=q.dtype) if q.dtype != torch.float32 else None
+    a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1), _a(lse), _a(lo)
+    L = _lib.lib()
+    a.workspace_bytes = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 0)
+    ws = _workspace(a.workspace_bytes, q.device)
+    a.workspace = _a(ws)
+    _launch(q.device, L.dua_rel_attention, a, "dua_rel_attention")
     return (out, RelAttentionSaved(lse, lo)) if want_lse else out
 
 
@@ -1410,44 +1413,51 @@ def rel_attention_bwd(q, k, v, table, buckets, out, saved, dout, heads, kv_heads
     _token_tensor(saved.lse, "saved.lse", (torch.float32,), (a.B, heads, a.Tq), q.device)
     if saved.out_lo is not None:
         _token_tensor(saved.out_lo, "saved.out_lo", (q.dtype,), (a.B, heads, a.Tq, a.ch), q.device)
-    with _on(q.device):
-        new = lambda t: torch.empty(t.shape, device=q.device, dtype=t.dtype)
-        dq, dk, dv, dtable = new(q), new(k), new(v), new(table)
-        a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1), _a(saved.lse), _a(saved.out_lo)
-        a.dout, a.dout_batch, a.dout_row = _a(dout), dout.stride(0), dout.stride(1)
-        a.dq, a.dk, a.dv, a.dtable = _a(dq), _a(dk), _a(dv), _a(dtable)
-        a.dq_batch, a.dq_row, a.dk_batch, a.dk_row, a.dv_batch, a.dv_row = (s for t in (dq, dk, dv) for s in t.stride()[:2])
-        L = _lib.lib()
-        a.workspace_bytes = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 1)
-        ws = _workspace(a.workspace_bytes, q.device)
-        a.workspace = _a(ws)
-        check(L.dua_rel_attention_bwd(ctypes.byref(a), _stream()), "dua_rel_attention_bwd")
+    new = lambda t: torch.empty(t.shape, device=q.device, dtype=t.dtype)
+    dq, dk, dv, dtable = new(q), new(k), new(v), new(table)
+    a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1), _a(saved.lse), _a(saved.out_lo)
+    a.dout, a.dout_batch, a.dout_row = _a(dout), dout.stride(0), dout.stride(1)
+    a.dq, a.dk, a.dv, a.dtable = _a(dq), _a(dk), _a(dv), _a(dtable)
+    a.dq_batch, a.dq_row, a.dk_batch, a.dk_row, a.dv_batch, a.dv_row = (s for t in (dq, dk, dv) for s in t.stride()[:2])
+    L = _lib.lib()
+    a.workspace_bytes = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 1)
+    ws = _workspace(a.workspace_bytes, q.device)
+    a.workspace = _a(ws)
+    _launch(q.device, L.dua_rel_attention_bwd, a, "dua_rel_attention_bwd")
     return dq, dk, dv, dtable
 
 
 TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprob entropy lse top_ids top_logprobs stats")
 
 
+def _even_rows(t, name):
+    """[..., V] as evenly spaced rows: their number and distance."""
+    V = t.shape[-1]
+    n = t.numel() // V
+    if t.is_contiguous() or n <= 1:
+        return n, V
+    try:
+        ld = t.view(-1, V).stride(0)
+    except RuntimeError:
+        raise ValueError(f"{name}: the rows must be evenly spaced") from None
+    if ld < V:
+        raise ValueError(f"{name}: the rows must not overlap")
+    return n, ld
+
+
 def _logprob_args(logits, ids, k, inv_temperature):
-    _token_tensor(logits, "logits", tuple(_DTYPES), contiguous=False)
+    _token_tensor(logits, "logits", _DTYPES, contiguous=False)
     if logits.dim() < 2 or logits.shape[-1] < 1:
         raise ValueError(f"logits: expected [..., V], got {tuple(logits.shape)}")
     V = logits.shape[-1]
-    try:
-        rows = logits.view(-1, V) if logits.numel() else logits.reshape(0, V)
-    except RuntimeError:
-        raise ValueError("logits: the rows must be evenly spaced") from None
-    ld = rows.stride(0) if rows.shape[0] > 1 else V
-    if rows.shape[0] > 1 and ld < V:
-        raise ValueError("logits: the rows must not overlap")
+    rows, ld = _even_rows(logits, "logits")
     if ids is not None:
         _token_tensor(ids, "ids", (torch.int64,), logits.shape[:-1], logits.device)
     if not 0 <= k <= min(64, V):
         raise ValueError(f"k: expected 0 to min(64, V), got {k}")
     if not 0.0 < inv_temperature < math.inf:
         raise ValueError(f"inv_temperature: must be positive and finite, got {inv_temperature}")
-    return TokenLogprobsArgs(logits=_a(logits), dtype=_DTYPES[logits.dtype], rows=rows.shape[0], V=V, ld=ld, ids=_a(ids), k=k,
-                             inv_temperature=float(inv_temperature))
+    return TokenLogprobsArgs(logits.data_ptr(), _DTYPES[logits.dtype], rows, V, ld, _a(ids), k, inv_temperature)
 
 
 def token_logprobs(logits, ids=None, k=0, inv_temperature=1.0):
@@ -1460,16 +1470,16 @@ def token_logprobs(logits, ids=None, k=0, inv_temperature=1.0):
     All but the ids fp32.  A row without a finite logit: logprob = lse = -inf, entropy 0."""
     a = _logprob_args(logits, ids, k, inv_temperature)
     lead, dev = logits.shape[:-1], logits.device
-    with _on(dev):
-        new = lambda *s, dtype=torch.float32: torch.empty(s, device=dev, dtype=dtype)
-        o = TokenLogprobs(new(*lead), new(*lead), new(*lead), new(*lead, k, dtype=torch.int64) if k else None, new(*lead, k) if k else None,
-                          new(a.rows, 4))
-        a.logprob, a.entropy, a.lse, a.top_ids, a.top_logprobs, a.stats = (_a(t) for t in o)
-        L = _lib.lib()
-        a.workspace_bytes = L.dua_token_logprobs_workspace_bytes(ctypes.byref(a))
-        ws = _workspace(a.workspace_bytes, dev)
-        a.workspace = _a(ws)
-        check(L.dua_token_logprobs(ctypes.byref(a), _stream()), "dua_token_logprobs")
+    three = torch.empty((3, *lead), device=dev, dtype=torch.float32).unbind(0)
+    top = torch.empty((*lead, k), device=dev, dtype=torch.int64) if k else None
+    tlp = torch.empty((*lead, k), device=dev, dtype=torch.float32) if k else None
+    o = TokenLogprobs(*three, top, tlp, torch.empty((a.rows, 4), device=dev, dtype=torch.float32))
+    a.logprob, a.entropy, a.lse, a.top_ids, a.top_logprobs, a.stats = (_a(t) for t in o)
+    L = _lib.lib()
+    a.workspace_bytes = L.dua_token_logprobs_workspace_bytes(ctypes.byref(a))
+    ws = _workspace(a.workspace_bytes, dev)
+    a.workspace = _a(ws)
+    _launch(dev, L.dua_token_logprobs, a, "dua_token_logprobs")
     return o
 
 
@@ -1489,15 +1499,14 @@ def token_logprobs_bwd(logits, ids, saved, dlogprob=None, dentropy=None, dtop=No
             _token_tensor(t, n, f32, s, dev)
     if k:
         _token_tensor(saved.top_ids, "saved.top_ids", (torch.int64,), (*lead, k), dev)
-    with _on(dev):
-        if out is None:
-            out = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
-        else:
-            _token_tensor(out, "out", (logits.dtype,), logits.shape, dev, contiguous=False)
-        d = _logprob_args(out, None, 0, 1.0)
-        if out.data_ptr() == logits.data_ptr() and d.ld != a.ld:
-            raise ValueError("out: in place needs the logits' own row stride")
-        a.stats, a.top_ids, a.dlogprob, a.dentropy, a.dtop, a.dlogits, a.ldd = (_a(saved.stats), _a(saved.top_ids) if k else None, _a(dlogprob),
-                                                                                _a(dentropy), _a(dtop), _a(out), d.ld)
-        check(_lib.lib().dua_token_logprobs_bwd(ctypes.byref(a), _stream()), "dua_token_logprobs_bwd")
+    if out is None:
+        out = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
+    else:
+        _token_tensor(out, "out", (logits.dtype,), logits.shape, dev, contiguous=False)
+    ldd = _even_rows(out, "out")[1]
+    if out.data_ptr() == logits.data_ptr() and ldd != a.ld:
+        raise ValueError("out: in place needs the logits' own row stride")
+    a.stats, a.top_ids, a.dlogprob, a.dentropy, a.dtop, a.dlogits, a.ldd = (_a(saved.stats), _a(saved.top_ids) if k else None, _a(dlogprob),
+                                                                            _a(dentropy), _a(dtop), _a(out), ldd)
+    _launch(dev, _lib.lib().dua_token_logprobs_bwd, a, "dua_token_logprobs_bwd")
     return out

@@ -635,7 +635,8 @@ int dua_sandwich_norm_bwd(const dua_sandwich_norm_args* args_host, void* stream)
  * out_lo [B][heads][Tq][ch] = what out's rounding to bf16 / fp16 left, 16-byte aligned (NULL: not kept; the backward pass then takes out as it
  * is, and its gradients carry that rounding).  A query
  * without keys gives zeros (lse = -inf).  Keys behind klen are not read.  q, out [B][Tq][heads * ch], k, v [B][Tk][kv_heads * ch] with strides
- * of their own (elements); query head h reads kv head h / (heads / kv_heads); ch <= 128.  table [num_buckets][heads] (table_dtype: fp32 or
+ * of their own (elements); query head h reads kv head h / (heads / kv_heads);
+ * ch <= 128, a multiple of 8 (fp32: 4); row strides below 2^24.  table [num_buckets][heads] (table_dtype: fp32 or
  * dtype), bucket_map [2 radius + 1]: entries outside [0, num_buckets) add no bias; radius <= 1024.  Tq = 1 is decoding. */
 typedef struct {
     const void *q, *k, *v;

@@ -108,17 +108,19 @@ def test_rel_attention_lengths_offsets_and_empty_rows(dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("Tk,ch,H,Hk", [(1, 64, 2, 2), (257, 64, 4, 2), (1000, 128, 2, 1), (4100, 72, 1, 1), (130, 20, 3, 3), (63, 33, 2, 1)])
+@pytest.mark.parametrize("Tk,ch,H,Hk", [(1, 64, 2, 2), (257, 64, 4, 2), (1000, 128, 2, 1), (4100, 72, 1, 1), (130, 24, 3, 3), (63, 40, 34, 2)])
 def test_rel_attention_decoding(dt, Tk, ch, H, Hk):
     n = [Tk, max(Tk // 2, 1), 0]
     attention_case(dt, 3, 1, Tk, H, Hk, ch, True, klen=n, qstart=[max(x - 1, 0) for x in n], seed=Tk, grads=False)
     attention_case(dt, 3, 1, Tk, H, Hk, ch, False, klen=n, qstart=[5, 0, 3], seed=Tk, grads=False)
 
 
-@pytest.mark.parametrize("ch", [1, 4, 20, 33, 127])
-def test_rel_attention_odd_head_widths(ch):
+@pytest.mark.parametrize("ch", [8, 24, 40, 56, 88, 104, 120])
+def test_rel_attention_head_widths(ch):
     for dt in DTYPES:
         attention_case(dt, 1, 37, 67, 2, 1, ch, False, seed=ch)
+    for w in (ch - 4, ch + 4):
+        attention_case(torch.float32, 1, 37, 67, 2, 1, w, False, seed=w)
 
 
 def test_rel_attention_table_types_scale_and_wide_radius():
@@ -525,7 +527,8 @@ def test_token_operator_refusals():
            (ValueError, lambda: ops.rel_attention(q, q, q, table, torch.zeros(33), heads=2)),
            (TypeError, lambda: ops.rel_attention(q, q, q, table, bk, heads=2, klen=torch.zeros(1, device=dev, dtype=torch.int64))),
            (ValueError, lambda: ops.rel_attention(q, q, q, table, bk, heads=2, klen=torch.zeros(2, device=dev, dtype=torch.int32))),
-           (RuntimeError, lambda: ops.rel_attention(z(1, 4, 258), z(1, 4, 258), z(1, 4, 258), table, bk, heads=2)),
+           (RuntimeError, lambda: ops.rel_attention(z(1, 4, 272), z(1, 4, 272), z(1, 4, 272), table, bk, heads=2)),
+           (RuntimeError, lambda: ops.rel_attention(z(1, 4, 66), z(1, 4, 66), z(1, 4, 66), table, bk, heads=2)),
            (RuntimeError, lambda: ops.rel_attention(torch.zeros(1, 4, 64), q, q, table, bk, heads=2)),
            (TypeError, lambda: ops.rel_attention_bwd(q, q, q, table, bk, q, z(1, 2, 4), q, heads=2)),
            (ValueError, lambda: ops.rel_attention_bwd(q, q, q, table, bk, q, ops.RelAttentionSaved(z(1, 2, 5), None), q, heads=2)),

@@ -81,7 +81,7 @@ def test_argument_validation_without_gpu():
 
     assert L.dua_rel_attention(None, None) == -1 and L.dua_rel_attention_bwd(None, None) == -1
     for fn in (L.dua_rel_attention, L.dua_rel_attention_bwd):
-        for kw, text in ((dict(ch=0), "width"), (dict(ch=129), "width"), (dict(kv_heads=3), "kv_heads"), (dict(dtype=5), "dtype"), (dict(table_dtype=2), "dtype"),
+        for kw, text in ((dict(ch=0), "width"), (dict(ch=132), "width"), (dict(ch=30), "width"), (dict(ch=20, dtype=1), "width"), (dict(q_row=1 << 24), "strides"), (dict(k_row=-8), "strides"), (dict(kv_heads=3), "kv_heads"), (dict(dtype=5), "dtype"), (dict(table_dtype=2), "dtype"),
                          (dict(radius=0), "radius"), (dict(radius=1025), "radius"), (dict(num_buckets=0), "radius"), (dict(table=None), "table"),
                          (dict(bucket_map=None), "map"), (dict(k=None), "null"), (dict(q=None), "null"), (dict(Tk=1 << 29), "lengths"), (dict(Tq=-1), "lengths"),
                          (dict(B=1 << 22), "blocks")):
