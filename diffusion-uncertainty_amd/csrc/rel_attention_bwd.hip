@@ -134,10 +134,20 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float x = exp2_raw(s[i][n][r] - ls[i]);
-                        s[i][n][r] = masked && x == 0.f ? 0.f : x * (d[i][n][r] - D[i]);   // (masked places may hold anything)
-                        rest[i] += s[i][n][r];
-                        e[n][r] = s[i][n][r] * p.scale;
+                        s[i][n][r] = x;
+                        e[n][r] = x * (d[i][n][r] - D[i]);
                     }
+                if (masked) {                                               // (masked places may hold anything)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) e[n][r] = s[i][n][r] == 0.f ? 0.f : e[n][r];
+                }
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    rest[i] += (e[n][0] + e[n][1]) + (e[n][2] + e[n][3]);
+                    e[n] *= p.scale;
+                }
                 pf[i] = acc_frag<T>(e);
             }
 #pragma unroll
@@ -289,18 +299,39 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
                 const int key = kw + 16 * i + (lane & 15);
-                const float* lp = side ? lut0 : lut0 + (key - pmin - 4 * g);
+                if (side) {
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        const f32x4 L = b - *(const f32x4*)(row_ls + 16 * (n0 + n) + 4 * g);
+                        s[i][n] = s[i][n] * sl + L;
+                    }
+                } else {
+                    const float* lp = lut0 + (key - pmin - 4 * g);
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        const f32x4 L = *(const f32x4*)(row_ls + 16 * (n0 + n) + 4 * g);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[i][n][r] = s[i][n][r] * sl + (lp[-16 * n - r] - L[r]);
+                    }
+                }
 #pragma unroll
                 for (int n = 0; n < NP; ++n) {
-                    const f32x4 L = *(const f32x4*)(row_ls + 16 * (n0 + n) + 4 * g), Dr = *(const f32x4*)(row_d + 16 * (n0 + n) + 4 * g);
+                    const f32x4 Dr = *(const f32x4*)(row_d + 16 * (n0 + n) + 4 * g);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int qi = 16 * n + 4 * g + r;
-                        float e = exp2_raw(s[i][n][r] * sl + ((side ? b : lp[-16 * n - r]) - L[r]));
-                        if (masked && (key >= nk || (p.causal && key > pmin + qi))) e = 0.f;
-                        s[i][n][r] = e;
-                        d[i][n][r] = masked && e == 0.f ? 0.f : e * (d[i][n][r] - Dr[r]);
+                        s[i][n][r] = exp2_raw(s[i][n][r]);
+                        d[i][n][r] = s[i][n][r] * (d[i][n][r] - Dr[r]);
                     }
+                }
+                if (masked) {                                               // (masked places may hold anything)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool out = key >= nk || (p.causal && key > pmin + 16 * n + 4 * g + r);
+                            s[i][n][r] = out ? 0.f : s[i][n][r];
+                            d[i][n][r] = out || s[i][n][r] == 0.f ? 0.f : d[i][n][r];
+                        }
                 }
                 pf[i] = acc_frag<T>(s[i]);
             }
