@@ -322,13 +322,14 @@ __global__ __launch_bounds__(NTHR) void k_rel_attention_join(AttP p) {
 }
 
 // How the forward pass splits the keys: a few queries a kv head go to k_rel_attention_few; too few workgroups for the 256 CUs share a row's
-// keys - about 1024 workgroups of at least 128 keys (few queries: their time is the read), 512 of at least 256 (tiles of queries).
+// keys - about 512 workgroups of at least 128 keys (few queries) or 256 (tiles of queries).  Few queries, 2 x 30001 keys of 4 heads of 128: 30 us with
+// 512, 35 with 1024 workgroups; 4 x 2000 keys of 16 heads of 72 in fp32: 23 and 28 us.
 struct Plan { bool few; int splits; };
 Plan plan(const dua_rel_attention_args* a) {
     const long rep = a->heads / a->kv_heads, units = (long)a->B * a->kv_heads;
     Plan pl{rep * a->Tq <= 16, 1};
     const long wgs = pl.few ? units : units * rep * ((a->Tq + query_block(a->dtype) - 1) / query_block(a->dtype));
-    const long want = pl.few ? (1024 + wgs - 1) / wgs : (wgs < 256 ? (512 + wgs - 1) / wgs : 1), most = a->Tk / (pl.few ? 128 : 256);
+    const long want = pl.few ? (512 + wgs - 1) / wgs : (wgs < 256 ? (512 + wgs - 1) / wgs : 1), most = a->Tk / (pl.few ? 128 : 256);
     long s = want < most ? want : most;
     s = s < 1 ? 1 : (s > SMAX ? SMAX : s);
     pl.splits = (int)s;

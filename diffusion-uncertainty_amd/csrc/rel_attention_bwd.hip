@@ -36,7 +36,7 @@ __device__ __forceinline__ void flush_diagonals(float* diag, int nl, int R, int 
 
 // ------------------------------------------------------------------------------------------------------------------------ dq
 template <typename T, int CHP>
-__global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dq(AttP p) {
+__global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(AttP p) {
     typedef Shape<T, CHP> S;
     typedef typename Frag<T>::type frag;
     constexpr int KT = S::KT, NQ = S::NQ, KS = S::KS, CT = S::CT, P = S::PITCH, NP = S::NP;

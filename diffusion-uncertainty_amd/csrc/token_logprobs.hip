@@ -8,7 +8,7 @@
 // maxima is a lower bound of the row's k-th largest value; only groups that reach it are read again (about k of them), a thread whose
 // second value reaches it too is re-read whole (about k^2 / 512 of them), and the few candidates are ranked exactly.  Rows with many equal
 // values, NaN or +inf take an ordered scan of the row in the same kernel (select_ordered).
-// Any alignment: a row is walked in aligned 16-byte groups, its first and last group element by element.
+// A row may begin anywhere and be of any length.
 #include <float.h>
 #include "elem.h"
 
@@ -64,29 +64,31 @@ struct LogpP {
     long ldd;
 };
 
-// The 16-byte groups of elements [v0, v1) of a row: group g holds elements first + g * VEC ... ; only the first and the last may stick out.
+// The groups of VEC elements (16 bytes, at any address) of elements [v0, v1) of a row.  The last one is read up to v1 and overlaps the one before
+// where it would stick out: holds() says which elements are its own.  Every load is whole and unconditional.
 template <typename T> struct Groups {
     static constexpr int VEC = Elem<T>::VEC;
-    const T* base;                                           // of group 0 (16-byte aligned; may lie before the row)
+    typedef typename VecOf<T, VEC>::type Raw;
+    const T* base;                                           // element v0
     long first;
-    int lead, n, last;                                       // elements before v0 in group 0; groups; elements of the last group
-    __device__ Groups(const T* row, long v0, long v1) {
-        lead = (int)(((uintptr_t)(row + v0) & 15) / sizeof(T));
-        first = v0 - lead;
-        base = row + first;
-        n = (int)((v1 - first + VEC - 1) / VEC);
-        last = (int)(v1 - first - (long)(n - 1) * VEC);
-    }
-    __device__ __forceinline__ bool whole(int g) const { return (g > 0 || lead == 0) && (g < n - 1 || last == VEC); }
-    __device__ __forceinline__ bool holds(int g, int j) const { return (g > 0 || j >= lead) && (g < n - 1 || j < last); }
-    __device__ __forceinline__ void load(int g, float* f) const {                        // elements outside [v0, v1): -inf
-        const T* p = (const T*)((const char*)base + 16u * (unsigned)g);                  // (rows of less than 4 GB)
-        if (whole(g)) {
-            ld_elems<T, VEC>(p, f);
-        } else {
+    int len, n;
+    __device__ Groups(const T* row, long v0, long v1) : base(row + v0), first(v0), len((int)(v1 - v0)), n((len + VEC - 1) / VEC) {}
+    __device__ __forceinline__ int at(int g) const { return min(g * VEC, max(len - VEC, 0)); }
+    __device__ __forceinline__ bool whole(int g) const { return (g + 1) * VEC <= len; }
+    __device__ __forceinline__ bool holds(int g, int j) const { return at(g) + j >= g * VEC && at(g) + j < len; }
+    __device__ __forceinline__ long index(int g, int j) const { return first + at(g) + j; }
+    __device__ __forceinline__ const T* ptr(int g) const { return (const T*)((const char*)base + (unsigned)at(g) * (unsigned)sizeof(T)); }   // (rows of less than 4 GB)
+    __device__ __forceinline__ Raw raw(int g) const {
+        if (len >= VEC) return *(const typename MemVec<T, VEC>::type*)ptr(g);
+        Raw r;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f[j] = holds(g, j) ? (float)p[j] : -INFINITY;
-        }
+        for (int j = 0; j < VEC; ++j) r[j] = base[min(j, len - 1)];
+        return r;
+    }
+    __device__ __forceinline__ void load(int g, float* f) const {                        // elements that are not group g's own: -inf
+        const Raw r = raw(g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] = holds(g, j) ? (float)r[j] : -INFINITY;
     }
 };
 
@@ -125,7 +127,6 @@ __device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
     long have = 0;
     for (int g0 = 0; g0 < gr.n; g0 += NT) {
         const int g = g0 + tid;
-        const long e0 = gr.first + (long)g * VEC;
         float f[VEC];
         uint32_t best = 0;                                     // 0: below every float's key
         if (g < gr.n) {
@@ -148,7 +149,7 @@ __device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
                 if (gr.holds(g, j) && okey(f[j]) > bar) {
                     const int at = atomicAdd(&sh.ncand, 1);     // at most k * VEC <= 512: fits
                     sh.ck[at] = okey(f[j]);
-                    sh.ci[at] = (int)(e0 + j);
+                    sh.ci[at] = (int)gr.index(g, j);
                 }
         }
         __syncthreads();
@@ -216,20 +217,28 @@ __device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared&
     float b1 = -INFINITY, b2 = -INFINITY;                 // best value, best value outside the best pair of groups (g, g + NT)
     int bg = -1;
     const int n = gr.n;
-    for (int g = tid; g < n; g += 2 * NT) {
+    typename Groups<T>::Raw r0 = gr.raw(min(tid, n - 1)), r1 = gr.raw(min(tid + NT, n - 1));
+    for (int g0 = 0; g0 < n; g0 += 2 * NT) {
+        const int g = g0 + tid;
         float f[2 * VEC];
-        gr.load(g, f);
-        if (g + NT < n) {
-            gr.load(g + NT, f + VEC);
-        } else {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f[VEC + j] = -INFINITY;
+        for (int j = 0; j < VEC; ++j) { f[j] = (float)r0[j]; f[VEC + j] = (float)r1[j]; }
+        if (g0 + 2 * NT < n) {                             // (the next pair is in flight while this one is summed)
+            r0 = gr.raw(min(g + 2 * NT, n - 1));
+            r1 = gr.raw(min(g + 3 * NT, n - 1));
+        }
+        if (g0 + 2 * NT >= n) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                f[j] = g < n && gr.holds(g, j) ? f[j] : -INFINITY;
+                f[VEC + j] = g + NT < n && gr.holds(g + NT, j) ? f[VEC + j] : -INFINITY;
+            }
         }
         float vm = f[0];
 #pragma unroll
         for (int j = 1; j < 2 * VEC; ++j) vm = fmaxf(vm, f[j]);
         b2 = fmaxf(b2, fminf(b1, vm));
-        bg = vm > b1 || bg < 0 ? g : bg;
+        bg = g < n && (vm > b1 || bg < 0) ? g : bg;
         b1 = fmaxf(b1, vm);
         const float top = fminf(vm * c, REF_MAX);
         if (__any(top > a.ref + 16.f)) {
@@ -282,7 +291,7 @@ __device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared&
             for (int j = 0; j < VEC; ++j)
                 if (gr.holds(g, j) && okey(f[j]) >= tau) {
                     const int at = atomicAdd(&sh.ncand, 1);
-                    if (at < CAP) { sh.ck[at] = okey(f[j]); sh.ci[at] = (int)(gr.first + (long)g * VEC + j); }
+                    if (at < CAP) { sh.ck[at] = okey(f[j]); sh.ci[at] = (int)gr.index(g, j); }
                 }
         };
         if (bg >= 0 && mine >= tau) {
@@ -467,15 +476,14 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_bwd(LogpP p) {
         return none ? 0.f : p.t * (g - pr * (A + gH * (LN2 * fmaxf(l2, -300.f) + H)));      // 2^-300 = 0 in fp32: no 0 * inf
     };
     const Groups<T> gr(row, v0, v1);
-    T* const obase = out + gr.first;
     for (int g = tid; g < gr.n; g += NT) {
+        const typename Groups<T>::Raw raw = gr.raw(g);
         float f[VEC];
-        gr.load(g, f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = grad(f[j], 0.f);
-        T* const o = (T*)((char*)obase + 16u * (unsigned)g);
+        for (int j = 0; j < VEC; ++j) f[j] = grad((float)raw[j], 0.f);
+        T* const o = (T*)((char*)(out + v0) + (unsigned)gr.at(g) * (unsigned)sizeof(T));
         if (gr.whole(g)) {
-            st_elems<T, VEC>(o, f);                         // (rows of dx may lie at another alignment)
+            st_elems<T, VEC>(o, f);
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
