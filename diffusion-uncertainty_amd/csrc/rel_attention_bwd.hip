@@ -202,7 +202,7 @@ __global__ __launch_bounds__(1024) void k_rel_attention_dtable(AttP p) {
 
 // -------------------------------------------------------------------------------------------------------------------- dk, dv
 template <typename T, int CHP>
-__global__ __launch_bounds__(NTHR, 2) void k_rel_attention_dkv(AttP p) {
+__global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_rel_attention_dkv(AttP p) {
     typedef Shape<T, CHP> S;
     typedef typename Frag<T>::type frag;
     constexpr int QT = S::KT, NK = S::NK, KS = S::KS, CT = S::CT, P = S::PITCH, NP = S::NP;
