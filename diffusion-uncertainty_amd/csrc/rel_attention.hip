@@ -102,33 +102,43 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
         // far from the diagonal and whole: one multiply-add turns a raw score into the exponent (its maximum is the raw maximum's)
         const bool plain = side && !masked && sl > 0.f;
         const float b = side < 0 ? flo : fhi, mul = plain ? sl : 1.f, add = plain ? b : 0.f;
+        if (!plain) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) bias_mask<N16>(s[i], sl, lut0, side, b, masked, k0, nk, pmin + 16 * i + (lane & 15), p.causal, lane);
+        }
+        float mx[NQ], c0[NQ];
+        bool rise = false;
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
-            if (!plain) bias_mask<N16>(s[i], sl, lut0, side, b, masked, k0, nk, pmin + 16 * i + (lane & 15), p.causal, lane);
-            const float mx = max_of<N16>(s[i]) * mul + add;
-            if (__any(mx > m[i] + 8.f)) {
-                const float mn = fmaxf(m[i], col_max(mx)), f = exp2_raw(m[i] - (mn == -INFINITY ? 0.f : mn));
+            mx[i] = max_of<N16>(s[i]) * mul + add;
+            rise = rise || mx[i] > m[i] + 8.f;
+        }
+        if (__any(rise)) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const float mn = fmaxf(m[i], col_max(mx[i])), f = exp2_raw(m[i] - (mn == -INFINITY ? 0.f : mn));
                 m[i] = mn;
                 l[i] *= f;
 #pragma unroll
                 for (int c = 0; c < CT; ++c) o[i][c] *= f;
             }
-            const float c0 = add - (m[i] == -INFINITY ? 0.f : m[i]);
-            float sum = 0.f;
-#pragma unroll
-            for (int n = 0; n < N16; ++n)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[i][n][r] = exp2_raw(s[i][n][r] * mul + c0);
-                    sum += s[i][n][r];
-                }
-            l[i] += sum;
         }
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) c0[i] = add - (m[i] == -INFINITY ? 0.f : m[i]);
+        // the exponentials of one step beside the products of the one before
 #pragma unroll
         for (int kb = 0; kb < N16; kb += S::NP) {
             frag pf[NQ];
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) pf[i] = acc_frag<T>(&s[i][kb]);
+            for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+                for (int n = 0; n < S::NP; ++n) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[i][kb + n][r] = exp2_raw(s[i][kb + n][r] * mul + c0[i]);
+                    l[i] += (s[i][kb + n][0] + s[i][kb + n][1]) + (s[i][kb + n][2] + s[i][kb + n][3]);
+                }
+                pf[i] = acc_frag<T>(&s[i][kb]);
+            }
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 const frag a = col_frag<T>(Vt, P, 16 * kb, 16 * c, lane);
