@@ -88,13 +88,15 @@ __device__ __forceinline__ Where place(const AttP& p, int heads_inner, unsigned 
 __device__ __forceinline__ int keys_of(const AttP& p, int b) { return p.klen ? min(max(p.klen[b], 0), p.Tk) : p.Tk; }
 __device__ __forceinline__ int start_of(const AttP& p, int b) { return p.qstart ? min(max(p.qstart[b], -(1 << 30)), 1 << 30) : 0; }
 
-// Bias of head h at clipped distance index i in [0, 2R], in log2 units; a map entry outside [0, nb) adds nothing.
+// Bias of head h at clipped distance index i in [0, 2R], in log2 units; a map entry outside [0, nb) adds nothing, a value below -1e30 (a mask of the
+// type's lowest value) is -inf: in log2 units it would leave fp32's range, and beside it a score has no digits.
 __device__ __forceinline__ float bias_at(const AttP& p, int h, int i) {
     const int m = p.map[i];
     if (m < 0 || m >= p.nb) return 0.f;
     const long at = (long)m * p.H + h;
-    return LOG2E * (p.table_dtype == DUA_DTYPE_F32 ? ((const float*)p.table)[at]
-                                                   : (p.table_dtype == DUA_DTYPE_BF16 ? (float)((const bf16_t*)p.table)[at] : (float)((const f16_t*)p.table)[at]));
+    const float v = p.table_dtype == DUA_DTYPE_F32 ? ((const float*)p.table)[at]
+                                                   : (p.table_dtype == DUA_DTYPE_BF16 ? (float)((const bf16_t*)p.table)[at] : (float)((const f16_t*)p.table)[at]);
+    return v < -1e30f ? -INFINITY : LOG2E * v;
 }
 // lut[rel + R + pad], rel clipped to [-R, R]
 __device__ __forceinline__ void load_lut(const AttP& p, int h, int pad, float* lut) {

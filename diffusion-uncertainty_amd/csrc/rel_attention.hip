@@ -45,14 +45,14 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
     if (w.b >= p.B) return;
     const int blk = p.causal ? p.nblk - 1 - w.blk : w.blk;                 // long rows first
     const int q0 = blk * S::QB, nk = keys_of(p, w.b), qs = start_of(p, w.b);
-    const int kend = p.causal ? max(0, min(nk, qs + min(q0 + S::QB, p.Tq))) : nk;
+    const int kend = p.causal ? max(0, min(nk, qs + min(q0 + S::QB, p.Tq))) : nk;   // (what lies behind it is not read)
     const int nt = (kend + KT - 1) / KT, t0 = (int)((long)nt * split / p.splits), t1 = (int)((long)nt * (split + 1) / p.splits);
     const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
     Carrier<T, CHP, KT> ck(p.kr, p.ch, tid), cv(p.vr, p.ch, tid);
     if (t0 < t1) {
-        ck.fetch(kp + (long)t0 * KT * p.kr, p.kr, nk - t0 * KT, p.ch, tid);
-        cv.fetch(vp + (long)t0 * KT * p.vr, p.vr, nk - t0 * KT, p.ch, tid);
+        ck.fetch(kp + (long)t0 * KT * p.kr, p.kr, kend - t0 * KT, p.ch, tid);
+        cv.fetch(vp + (long)t0 * KT * p.vr, p.vr, kend - t0 * KT, p.ch, tid);
     }
     const int qw = q0 + wave * 16 * NQ, pmin = qs + qw, pmax = pmin + 16 * NQ - 1;
     const T* qp = (const T*)p.q + w.b * p.qb + (long)w.h * p.ch;
@@ -81,8 +81,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
         __syncthreads();                                                    // (the other pair of tiles is read until here)
         const int k0 = t * KT;
         if (t + 1 < t1) {
-            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, nk - k0 - KT, p.ch, tid);
-            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, nk - k0 - KT, p.ch, tid);
+            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, kend - k0 - KT, p.ch, tid);
+            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, kend - k0 - KT, p.ch, tid);
         }
         if (qw >= p.Tq || (p.causal && k0 > pmax)) continue;               // (a wave without queries, or past its last key)
         f32x4 s[NQ][N16];
@@ -182,14 +182,14 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
     auto fetch_k = [&](int t) {
 #pragma unroll
         for (int n = 0; n < N16; ++n) {
-            const int key = min(t * KT + 16 * n + col, nk - 1);
+            const int key = min(t * KT + 16 * n + col, kend - 1);
 #pragma unroll
             for (int s = 0; s < KS; ++s) kf[n][s] = load16<T>(kp + key * p.kr, S::KSTEP * s + Frag<T>::N * g, p.ch);
         }
     };
     if (t0 + wave < t1) {
         fetch_k(t0 + wave);
-        cv.fetch(vp + (long)(t0 + wave) * KT * p.vr, p.vr, nk - (t0 + wave) * KT, p.ch, lane);
+        cv.fetch(vp + (long)(t0 + wave) * KT * p.vr, p.vr, kend - (t0 + wave) * KT, p.ch, lane);
     }
     frag qf[KS];
 #pragma unroll
@@ -203,13 +203,13 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
     for (int t = t0 + wave; t < t1; t += NWAVE) {
         const int k0 = t * KT;
         f32x4 s[N16];
-        const bool whole = k0 + KT <= nk && p.ch == S::KW;
+        const bool whole = k0 + KT <= kend && p.ch == S::KW;
 #pragma unroll
         for (int n = 0; n < N16; ++n) {
             s[n] = ZERO4;
             if (!whole) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) kf[n][ks] = keep16<T>(kf[n][ks], S::KSTEP * ks + Frag<T>::N * g, p.ch, k0 + 16 * n + col < nk);
+                for (int ks = 0; ks < KS; ++ks) kf[n][ks] = keep16<T>(kf[n][ks], S::KSTEP * ks + Frag<T>::N * g, p.ch, k0 + 16 * n + col < kend);
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) s[n] = mma(kf[n][ks], qf[ks], s[n]);
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
         cv.put(Vt, p.ch, lane);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (t + NWAVE < t1) cv.fetch(vp + (long)(k0 + NWAVE * KT) * p.vr, p.vr, nk - k0 - NWAVE * KT, p.ch, lane);
+        if (t + NWAVE < t1) cv.fetch(vp + (long)(k0 + NWAVE * KT) * p.vr, p.vr, kend - k0 - NWAVE * KT, p.ch, lane);
         const int side = side_of(k0, KT, qs, qs + p.Tq - 1, p.R);
         if (side) {
             const float bias = side < 0 ? flo : fhi;

@@ -53,8 +53,8 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(Att
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
     Carrier<T, CHP, KT> ck(p.kr, p.ch, tid), cv(p.vr, p.ch, tid);
     if (kend > 0) {
-        ck.fetch(kp, p.kr, nk, p.ch, tid);
-        cv.fetch(vp, p.vr, nk, p.ch, tid);
+        ck.fetch(kp, p.kr, kend, p.ch, tid);
+        cv.fetch(vp, p.vr, kend, p.ch, tid);
     }
     load_lut(p, w.h, S::PAD, lut);
     const int qw = q0 + wave * 16 * NQ, pmin = qs + qw, pmax = pmin + 16 * NQ - 1;
@@ -99,8 +99,8 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(Att
         cv.put(Vt, p.ch, tid);
         __syncthreads();
         if (k0 + KT < kend) {
-            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, nk - k0 - KT, p.ch, tid);
-            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, nk - k0 - KT, p.ch, tid);
+            ck.fetch(kp + (long)(k0 + KT) * p.kr, p.kr, kend - k0 - KT, p.ch, tid);
+            cv.fetch(vp + (long)(k0 + KT) * p.vr, p.vr, kend - k0 - KT, p.ch, tid);
         }
         if (qw >= p.Tq) continue;
         // steps of 16 NP keys: scores, dP, dS, and dS straight into dq - few registers live
@@ -215,7 +215,8 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const Where w = place(p, 1, blockIdx.x);
     if (w.b >= p.B) return;
-    const int k0 = w.blk * S::KB, nk = keys_of(p, w.b), qs = start_of(p, w.b);
+    const int k0 = w.blk * S::KB, qs = start_of(p, w.b);
+    const int nk = p.causal ? max(0, min(keys_of(p, w.b), qs + p.Tq)) : keys_of(p, w.b);   // (what lies behind it is not read: no query sees it)
     const int kw = k0 + wave * 16 * NK;
     const T* kp = (const T*)p.k + w.b * p.kb + (long)w.hk * p.ch;
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;

@@ -331,19 +331,22 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return k == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((k >> 31) ? k & 0x7FFFFFFFu : ~k);
 }
 
-// log2 of p of a value from the row's reference and log2 s
-__device__ __forceinline__ float log2_p(float x, float ref, float logs, bool huge, float c) { return (huge ? (x - ref) * c : fmaf(x, c, -ref)) - logs; }
+// log p of a value from the row's reference and log2 s (a masked value near the type's lowest has no log2 units in fp32's range: natural ones)
+__device__ __forceinline__ float value_lp(float x, float ref, float logs, bool huge, float t) {
+    if (huge) return (x - ref) * t - LN2 * logs;
+    return fabsf(x) > 1e30f ? x * t - LN2 * (ref + logs) : LN2 * (fmaf(x, t * LOG2E, -ref) - logs);
+}
 
 // A row without any finite value has no distribution: log probabilities -inf, entropy 0.
 template <typename T>
 __device__ void finish_row(const LogpP& p, long r, Soft a, bool huge, const uint32_t* bk, const int* bi) {
-    const float c = p.t * LOG2E, logs = a.s > 0.f || a.s != a.s ? log2f(a.s) : -INFINITY;
+    const float logs = a.s > 0.f || a.s != a.s ? log2f(a.s) : -INFINITY;
     const bool none = logs == -INFINITY;
     if (threadIdx.x == 0) {
         const float H = none ? 0.f : LN2 * (logs - a.w / a.s);
         const int64_t id = p.ids ? p.ids[r] : -1;
         float lp = 0.f;
-        if (id >= 0 && id < p.V) lp = none ? -INFINITY : LN2 * log2_p((float)((const T*)p.x)[r * p.ld + id], a.ref, logs, huge, c);
+        if (id >= 0 && id < p.V) lp = none ? -INFINITY : value_lp((float)((const T*)p.x)[r * p.ld + id], a.ref, logs, huge, p.t);
         p.logprob[r] = lp;
         p.entropy[r] = H;
         p.lse[r] = none ? -INFINITY : (huge ? a.ref * p.t + LN2 * logs : LN2 * (a.ref + logs));
@@ -351,7 +354,7 @@ __device__ void finish_row(const LogpP& p, long r, Soft a, bool huge, const uint
     }
     for (int j = threadIdx.x; j < p.k; j += NT) {
         p.top_ids[r * p.k + j] = bi[j];
-        p.top_lp[r * p.k + j] = none ? -INFINITY : LN2 * log2_p(key_value(bk[j]), a.ref, logs, huge, c);
+        p.top_lp[r * p.k + j] = none ? -INFINITY : value_lp(key_value(bk[j]), a.ref, logs, huge, p.t);
     }
 }
 

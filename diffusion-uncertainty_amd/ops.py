@@ -1372,6 +1372,10 @@ def _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qst
     qb, qr, _ = q.stride()
     kb, kr, _ = k.stride()
     vb, vr, _ = v.stride()
+    if Tq <= 1:
+        qr = 0                                                # (a single row's stride may be any)
+    if k.shape[1] <= 1:
+        kr = vr = 0
     return RelAttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dt], B, Tq, k.shape[1], heads, kv_heads, ch, qb, qr, kb, kr, vb, vr,
                             table.data_ptr(), _DTYPES[table.dtype], buckets.map.data_ptr(), buckets.radius, buckets.num_buckets, _a(klen), _a(qstart),
                             int(bool(causal)), 1.0 / math.sqrt(ch) if scale is None else scale)
@@ -1385,7 +1389,8 @@ def rel_attention(q, k, v, table, buckets, heads, kv_heads=None, causal=False, s
     softmax(scale q k^T + table[bucket(j - p_i), h]) v, p_i = qstart[b] + i, over keys j < klen[b] and, if causal, j <= p_i -> [B, Tq, heads * ch].
     q [B, Tq, heads * ch], k / v [B, Tk, kv_heads * ch] (views with unit stride along the last dimension: thirds of a qkv projection, slots
     of a cache), head widths up to 128 in multiples of 8 (fp32: 4); query head h attends to kv head h // (heads // kv_heads); table [num_buckets, heads] in fp32 or q's
-    type; klen / qstart int32 [B].  A query without keys gives zeros; keys behind klen are not read.  Tq = 1 with qstart = klen - 1
+    type; klen / qstart int32 [B].  A query without keys gives zeros; keys behind klen (causal: or the last query)
+    are not read; a table value below -1e30 masks its distances.  Tq = 1 with qstart = klen - 1
     is decoding.  want_lse=True: also RelAttentionSaved(lse [B, heads, Tq] = log sum e^s, out_lo: what out's rounding left), for the backward pass."""
     a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
@@ -1415,8 +1420,8 @@ def rel_attention_bwd(q, k, v, table, buckets, out, saved, dout, heads, kv_heads
         _token_tensor(saved.out_lo, "saved.out_lo", (q.dtype,), (a.B, heads, a.Tq, a.ch), q.device)
     new = lambda t: torch.empty(t.shape, device=q.device, dtype=t.dtype)
     dq, dk, dv, dtable = new(q), new(k), new(v), new(table)
-    a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1), _a(saved.lse), _a(saved.out_lo)
-    a.dout, a.dout_batch, a.dout_row = _a(dout), dout.stride(0), dout.stride(1)
+    a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1) if a.Tq > 1 else 0, _a(saved.lse), _a(saved.out_lo)
+    a.dout, a.dout_batch, a.dout_row = _a(dout), dout.stride(0), dout.stride(1) if a.Tq > 1 else 0
     a.dq, a.dk, a.dv, a.dtable = _a(dq), _a(dk), _a(dv), _a(dtable)
     a.dq_batch, a.dq_row, a.dk_batch, a.dk_row, a.dv_batch, a.dv_row = (s for t in (dq, dk, dv) for s in t.stride()[:2])
     L = _lib.lib()

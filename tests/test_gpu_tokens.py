@@ -123,6 +123,49 @@ def test_rel_attention_head_widths(ch):
         attention_case(torch.float32, 1, 37, 67, 2, 1, w, False, seed=w)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+def test_rel_attention_few_queries_and_split_keys(dt):
+    """Several tokens a step in the 16 columns of a tile, shared kv heads; tiles of queries whose keys are split over workgroups; their gradients."""
+    for B, Tq, Tk, H, Hk, ch in [(2, 5, 700, 4, 2, 64), (1, 16, 300, 1, 1, 72), (3, 2, 33, 8, 1, 128), (1, 40, 1500, 2, 1, 64), (2, 17, 1030, 1, 1, 128)]:
+        n = [Tk, Tk // 2, Tk - 3][:B]
+        attention_case(dt, B, Tq, Tk, H, Hk, ch, True, klen=n, qstart=[x - Tq for x in n], seed=Tq)
+        attention_case(dt, B, Tq, Tk, H, Hk, ch, False, klen=n, qstart=[x - Tq for x in n], seed=Tq + 1, grads=Tq < 17)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_rel_attention_unwritten_slots_behind_the_last_query(dt):
+    """A cache without klen whose slots behind the last causal query hold anything: not read, by either pass."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(2)
+    for Tq, qs in ((1, 40), (3, 70), (50, 31)):
+        B, Tk, H, ch = 2, 128, 2, 64
+        q, k, v, do = rnd(g, B, Tq, H * ch, dtype=dt), rnd(g, B, Tk, H * ch, dtype=dt), rnd(g, B, Tk, H * ch, dtype=dt), rnd(g, B, Tq, H * ch, dtype=dt)
+        table, bk = rnd(g, 8, H, dtype=dt).to(dev), ops.RelativeBuckets(8, 16, False, device=dev)
+        qst = torch.full((B,), qs, dtype=torch.int32, device=dev)
+        kw = dict(heads=H, causal=True, qstart=qst)
+        res = []
+        for fill in (0.0, math.nan):
+            kk, vv = k.to(dev), v.to(dev)
+            kk[:, qs + Tq:], vv[:, qs + Tq:] = fill, fill
+            out, s = ops.rel_attention(q.to(dev), kk, vv, table, bk, want_lse=True, **kw)
+            res.append((out, *ops.rel_attention_bwd(q.to(dev), kk, vv, table, bk, out, s, do.to(dev), **kw)))
+        for a, b in zip(*res):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_rel_attention_table_of_the_lowest_value():
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(4)
+    q, k, v, do = (rnd(g, 1, 30, 64).to(dev) for _ in range(4))
+    bk = ops.RelativeBuckets(8, 16, True, device=dev)
+    t1, t2 = rnd(g, 8, 2).to(dev), None
+    t1[5] = torch.finfo(torch.float32).min
+    t2 = t1.clone()
+    t2[5] = -math.inf
+    for a, b in zip(*[(o, *ops.rel_attention_bwd(q, k, v, t, bk, o, s, do, heads=2)) for t in (t1, t2) for o, s in [ops.rel_attention(q, k, v, t, bk, heads=2, want_lse=True)]]):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
 def test_rel_attention_table_types_scale_and_wide_radius():
     attention_case(torch.bfloat16, 1, 80, 80, 2, 2, 64, True, table_dt=torch.float32, scale=0.3)
     attention_case(torch.float32, 1, 40, 1300, 1, 1, 16, False, radius=1024, nb=64, seed=4)
@@ -459,6 +502,37 @@ def test_token_logprobs_rows_without_a_distribution():
     assert (d[0] == 0).all() and d[1].isnan().all() and torch.isfinite(d[4]).all()
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+def test_token_logprobs_long_rows_in_parts(dt):
+    """Few long rows are cut into parts: parts without finite values, of the type's lowest value, with equal values, beside ordinary ones; NaN."""
+    g = torch.Generator().manual_seed(12)
+    V = 40000
+    x = rnd(g, 7, V, scale=2.0, dtype=dt)
+    low = torch.finfo(dt).min
+    x[0, 5000:] = -math.inf
+    x[1, 100:] = low                                   # a filter that kept a hundred tokens
+    x[2, :] = low
+    x[3, :] = 1.5
+    x[4, 30000:] = x[4, :10000]
+    x[5, :39990] = -math.inf
+    ids = torch.tensor([3, 39999, 20000, 39998, 30001, 39995, 12345])
+    logprob_case(x, ids, 20)
+    from diffusion_uncertainty_amd import ops
+    y = rnd(g, 4, V, scale=2.0, dtype=dt)
+    y[0, 33333] = math.nan
+    y[1, 22222] = math.inf
+    y[2] = -math.inf
+    o = ops.token_logprobs(y.to(dev), k=3)
+    assert o.lse[:2].isnan().all() and o.entropy[:2].isnan().all() and o.lse[2] == -math.inf and o.entropy[2] == 0 and torch.isfinite(o.lse[3])
+    assert o.top_ids[0, 0] == 33333 and o.top_ids[1, 0] == 22222 and o.top_ids[2].tolist() == [0, 1, 2]
+    if dt == torch.float32:                            # offsets past the floating reference, alone and beside ordinary parts
+        z = rnd(g, 3, V)
+        z[0] += 1e30
+        z[1, 35000:] -= 3e9
+        z[2, 10] = 2e9
+        logprob_case(z, torch.tensor([5, 6, 10]), 5)
+
+
 def test_token_logprobs_views_and_partial_gradients():
     """A slice of a padded vocabulary (row stride > V, rows not 16-byte aligned), leading dimensions, missing gradients, no ids, repeated ids."""
     from diffusion_uncertainty_amd import ops
@@ -620,6 +694,36 @@ def test_operators_together_against_autograd_in_64_bits():
         assert err < 1300 * U, (n, float(err))
     u = got["entropy"].cpu()
     assert torch.equal(got["mask"].cpu().bool(), u > torch.quantile(u, 0.9, dim=1, keepdim=True))
+
+
+def test_wide_heads_and_rows_in_a_graph():
+    """Kernels with more than 64 KB of LDS (heads of 128, backward norms of 8192 columns) captured and replayed."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(6)
+    q, k, v, do = (rnd(g, 1, 150, 256, dtype=torch.bfloat16).to(dev) for _ in range(4))
+    x, y, dr, dz = (rnd(g, 40, 8192).to(dev) for _ in range(4))
+    w = rnd(g, 8192).to(dev)
+    bk, table = ops.RelativeBuckets(8, 16, True, device=dev), rnd(g, 8, 2).to(dev)
+
+    def step():
+        out, s = ops.rel_attention(q, k, v, table, bk, heads=2, want_lse=True)
+        r, z, st = ops.sandwich_norm(x, y, post_w=w, pre_w=w, gate=w, want_stats=True)
+        return [out, *ops.rel_attention_bwd(q, k, v, table, bk, out, s, do, heads=2), r, z] + [
+            t for t in ops.sandwich_norm_bwd(x, y, st, dr, dz, post_w=w, pre_w=w, gate=w) if t is not None]
+
+    step()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        o = step()
+    for i in range(3):
+        q.mul_(0.9)
+        x.add_(0.1)
+        gr.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(o, want):
+            assert torch.equal(a, b), i
 
 
 def test_operators_on_another_stream_two_at_a_time_and_in_a_graph():
