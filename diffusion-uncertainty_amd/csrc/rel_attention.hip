@@ -354,13 +354,13 @@ template <typename T, int CHP> struct Fwd {
         typedef Shape<T, CHP> S;
         const long rows = (long)p.B * p.H * p.Tq;
         if (few) {
-            if (int rc = launch(k_rel_attention_few<T, CHP>, "dua_rel_attention", dim3((unsigned)(p.B * p.Hk * p.splits)), NTHR, 0, st, p)) return rc;
+            if (int rc = launch<k_rel_attention_few<T, CHP>>("dua_rel_attention", dim3((unsigned)(p.B * p.Hk * p.splits)), NTHR, 0, st, p)) return rc;
         } else {
             const unsigned grid = grid_of(p, p.H / p.Hk, (p.Tq + S::QB - 1) / S::QB);
             const size_t lds = 4 * S::TILE + (2 * (p.R + S::PAD) + 1) * sizeof(float);
-            if (int rc = launch(k_rel_attention<T, CHP>, "dua_rel_attention", dim3(grid, p.splits), NTHR, lds, st, p)) return rc;
+            if (int rc = launch<k_rel_attention<T, CHP>>("dua_rel_attention", dim3(grid, p.splits), NTHR, lds, st, p)) return rc;
         }
-        return p.splits > 1 ? launch(k_rel_attention_join<T>, "dua_rel_attention", dim3((unsigned)rows), NTHR, 0, st, p) : DUA_OK;
+        return p.splits > 1 ? launch<k_rel_attention_join<T>>("dua_rel_attention", dim3((unsigned)rows), NTHR, 0, st, p) : DUA_OK;
     }
 };
 }  // namespace

@@ -214,6 +214,7 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     float* const diag = lut + nl;                                          // [wave][nl]: a head's sums of dS along the diagonals
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const Where w = place(p, 1, blockIdx.x);
+    const int split = blockIdx.y;
     if (w.b >= p.B) return;
     const int k0 = w.blk * S::KB, qs = start_of(p, w.b);
     const int nk = p.causal ? max(0, min(keys_of(p, w.b), qs + p.Tq)) : keys_of(p, w.b);   // (what lies behind it is not read: no query sees it)
@@ -236,13 +237,13 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
         for (int c = 0; c < CT; ++c) { ak[i][c] = ZERO4; av[i][c] = ZERO4; }
     }
     const float sl = p.scale * LOG2E;
-    const int rep = p.H / p.Hk;
+    const int rep = p.H / p.Hk / p.splits, h0 = w.hk * (p.H / p.Hk) + split * rep;   // this workgroup's query heads
     // tiles of queries that see this block's first key (position >= k0), head after head of the group
     const int qbeg = p.causal ? max(0, k0 - qs) / QT : 0, per = max(0, (p.Tq + QT - 1) / QT - qbeg), total = k0 < nk ? per * rep : 0;
     Carrier<T, CHP, QT> cq(p.qr, p.ch, tid), cd(p.dr, p.ch, tid);
     float row_next = 0.f;
     auto fetch = [&](int t) {
-        const int h = w.hk * rep + t / per, q0 = (qbeg + t % per) * QT;
+        const int h = h0 + t / per, q0 = (qbeg + t % per) * QT;
         cq.fetch((const T*)p.q + w.b * p.qb + (long)h * p.ch + (long)q0 * p.qr, p.qr, p.Tq - q0, p.ch, tid);
         cd.fetch((const T*)p.dout + w.b * p.db + (long)h * p.ch + (long)q0 * p.dr, p.dr, p.Tq - q0, p.ch, tid);
         if (tid < 2 * QT) {
@@ -253,14 +254,14 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     };
     for (int i = tid; i < NWAVE * nl; i += NTHR) diag[i] = 0.f;
     float far_lo = 0.f, far_hi = 0.f;
-    float* const part = p.part + (((long)w.b * p.nblk + w.blk) * p.H + w.hk * rep) * (2 * p.R + 1);
+    float* const part = p.part + (((long)w.b * p.nblk + w.blk) * p.H + h0) * (2 * p.R + 1);
     if (total > 0) fetch(0);
     for (int t = 0; t < total; ++t) {
         if (t % per == 0) {
             __syncthreads();                                                // (the last head's bias is read until here)
             if (t > 0) flush_diagonals(diag, nl, p.R, S::PAD, far_lo, far_hi, part + (t / per - 1) * (2 * p.R + 1));
             far_lo = far_hi = 0.f;
-            load_lut(p, w.hk * rep + t / per, S::PAD, lut);
+            load_lut(p, h0 + t / per, S::PAD, lut);
         }
         T* const Qt = tiles + (t & 1) * 2 * QT * P;
         T* const Dt = Qt + QT * P;
@@ -390,6 +391,22 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     } else {
         for (int i = tid; i < rep * (2 * p.R + 1); i += NTHR) part[i] = 0.f;
     }
+    if (p.splits > 1) {
+        // [split][dk, dv][B][Tk][Hk ch]
+        const long row = (long)p.Hk * p.ch, all = (long)p.B * p.Tk * row;
+        float* const fk = p.kv_part + 2 * split * all + (long)w.b * p.Tk * row + w.hk * p.ch;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const int kk = kw + 16 * i + (lane & 15);
+            if (kk >= p.Tk) continue;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                store4<float>(fk + kk * row, 16 * c + 4 * g, p.ch, ak[i][c]);
+                store4<float>(fk + all + kk * row, 16 * c + 4 * g, p.ch, av[i][c]);
+            }
+        }
+        return;
+    }
     T* gk = (T*)p.dk + w.b * p.dkb + (long)w.hk * p.ch;
     T* gv = (T*)p.dv + w.b * p.dvb + (long)w.hk * p.ch;
 #pragma unroll
@@ -404,23 +421,42 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     }
 }
 
+// dk and dv of split groups: the splits' sums in their order, four elements a thread
+template <typename T>
+__global__ __launch_bounds__(NTHR) void k_rel_attention_kv_join(AttP p) {
+    const int row = p.Hk * p.ch, quads = row / 4;
+    const long all = (long)p.B * p.Tk * row, n = 2 * all / 4, stride = (long)gridDim.x * NTHR;
+    for (long i = (long)blockIdx.x * NTHR + threadIdx.x; i < n; i += stride) {
+        f32x4 a = ZERO4;
+        for (int s = 0; s < p.splits; ++s) a += *(const f32x4*)(p.kv_part + 2 * s * all + 4 * i);
+        const bool v = 4 * i >= all;
+        const long at = v ? i - all / 4 : i, r = at / quads, b = r / p.Tk;
+        T* dst = v ? (T*)p.dv + b * p.dvb + (r % p.Tk) * p.dvr : (T*)p.dk + b * p.dkb + (r % p.Tk) * p.dkr;
+        store4<T>(dst, 4 * (int)(at % quads), row, a);
+    }
+}
+
 template <typename T, int CHP> struct Bwd {
     static int run(AttP p, bool, hipStream_t st) {
         typedef Shape<T, CHP> S;
         const int nqb = (p.Tq + S::QB - 1) / S::QB, nl = 2 * (p.R + S::PAD) + 1;
         if (p.B > 0 && nqb > 0) {
             const unsigned grid = grid_of(p, p.H / p.Hk, nqb);
-            if (int rc = launch(k_rel_attention_dq<T, CHP>, "dua_rel_attention_bwd", dim3(grid), NTHR, 4 * S::TILE + nl * sizeof(float), st, p)) return rc;
+            if (int rc = launch<k_rel_attention_dq<T, CHP>>("dua_rel_attention_bwd", dim3(grid), NTHR, 4 * S::TILE + nl * sizeof(float), st, p)) return rc;
         }
         if (p.B > 0 && p.Tk > 0) {
             const unsigned grid = grid_of(p, 1, (p.Tk + S::KB - 1) / S::KB);
-            if (int rc = launch(k_rel_attention_dkv<T, CHP>, "dua_rel_attention_bwd", dim3(grid), NTHR, 4 * S::TILE + (4 * S::KT + (1 + NWAVE) * nl) * sizeof(float), st, p)) return rc;
+            if (int rc = launch<k_rel_attention_dkv<T, CHP>>("dua_rel_attention_bwd", dim3(grid, p.splits), NTHR, 4 * S::TILE + (4 * S::KT + (1 + NWAVE) * nl) * sizeof(float), st, p)) return rc;
+            if (p.splits > 1) {
+                const long quads = (long)p.B * p.Tk * p.Hk * p.ch / 2;
+                if (int rc = launch<k_rel_attention_kv_join<T>>("dua_rel_attention_bwd", dim3(stream_grid(quads, NTHR)), NTHR, 0, st, p)) return rc;
+            }
         }
         const int nparts = p.B * ((p.Tk + S::KB - 1) / S::KB);
-        if (int rc = launch(k_rel_attention_diag, "dua_rel_attention_bwd", dim3((2 * p.R + 64) / 64, p.H), 1024, 0, st, p, nparts)) return rc;
-        if (p.table_dtype == DUA_DTYPE_F32) return launch(k_rel_attention_dtable<float>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
-        if (p.table_dtype == DUA_DTYPE_BF16) return launch(k_rel_attention_dtable<bf16_t>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
-        return launch(k_rel_attention_dtable<f16_t>, "dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
+        if (int rc = launch<k_rel_attention_diag>("dua_rel_attention_bwd", dim3((2 * p.R + 64) / 64, p.H), 1024, 0, st, p, nparts)) return rc;
+        if (p.table_dtype == DUA_DTYPE_F32) return launch<k_rel_attention_dtable<float>>("dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
+        if (p.table_dtype == DUA_DTYPE_BF16) return launch<k_rel_attention_dtable<bf16_t>>("dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
+        return launch<k_rel_attention_dtable<f16_t>>("dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
     }
 };
 
@@ -432,9 +468,12 @@ extern "C" int dua_rel_attention_bwd(const dua_rel_attention_args* a, void* stre
     DUA_REQUIRE(a->B == 0 || a->Tq == 0 || (a->out && a->lse && a->dout && a->dq), "dua_rel_attention_bwd: null operand");
     DUA_REQUIRE(a->B == 0 || a->Tk == 0 || (a->dk && a->dv), "dua_rel_attention_bwd: null output");
     const size_t need = rel_attention_bwd_bytes(a);
-    DUA_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), "dua_rel_attention_bwd: workspace smaller than dua_rel_attention_workspace_bytes");
+    DUA_REQUIRE(need == 0 || (a->workspace && ((uintptr_t)a->workspace & 15) == 0 && a->workspace_bytes >= need),
+                "dua_rel_attention_bwd: workspace smaller than dua_rel_attention_workspace_bytes, or not 16-byte aligned");
     AttP p = pack(a);
     p.dsum = (float*)a->workspace;
+    p.splits = key_splits(a);
+    p.kv_part = p.dsum + rel_attention_bwd_floats(a);
     p.diag = p.dsum + (size_t)a->B * a->heads * a->Tq;
     p.part = p.diag + (size_t)a->heads * (2 * a->radius + 1);
     return dispatch<Bwd>(a->dtype, p, false, as_stream(stream));

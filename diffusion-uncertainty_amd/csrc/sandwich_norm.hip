@@ -6,6 +6,7 @@
 // need the whole row, so the lanes of one unit hold it in registers, 16 bytes a lane, and walk several rows;
 // the parameters of its columns stay in registers over the rows (read per row they would be L2 traffic of the size of the tensors' own).
 // All sums and statistics are fp32; variances are sums of squared differences from the mean (no E[x^2] - mean^2 cancellation).
+#include <atomic>
 #include "elem.h"
 
 namespace {
@@ -576,7 +577,13 @@ template <typename T, typename PT, int LANES, int W, int PL> struct LBwd {
         constexpr bool LDS = LANES == 0 && PL == 8 && W == 16;                 // the four parameters of a thread's columns in LDS: at most 128 KB
         const size_t lds = LDS ? 4 * PL * (size_t)block * sizeof(float) : (LANES ? 5 * (size_t)p.D * sizeof(float) : 0);
         auto* kernel = &k_sandwich_norm_bwd<T, PT, LANES, W, PL, LDS>;
-        if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (lds > 64 * 1024) {                                                 // asked for once a device; refused, the launch reports it
+            static std::atomic<unsigned> asked{0};
+            int dev = 0;
+            (void)hipGetDevice(&dev);
+            const unsigned bit = 1u << (dev & 31);
+            if (!(asked.load() & bit) && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024) == hipSuccess) asked.fetch_or(bit);
+        }
         hipLaunchKernelGGL(kernel, grid, block, lds, st, p);
     }
 };

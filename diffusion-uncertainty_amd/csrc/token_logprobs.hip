@@ -92,22 +92,31 @@ template <typename T> struct Groups {
     }
 };
 
-struct Shared {
-    Soft soft[NW];
+struct __attribute__((aligned(16))) Shared {
     uint32_t key[NT];
-    uint32_t ck[CAP];                     // candidates: key, index
-    int ci[CAP];
+    uint64_t cand[CAP];                   // candidates
     int rescan[RESCAN];
+    Soft soft[NW];
     uint32_t tau;                         // (candidates of the fast selection reach it)
     int ncand, nrescan, any;
-    uint32_t bk[2][KMAX];                 // running best of the ordered scan
-    int bi[2][KMAX];
+    uint64_t best[2][KMAX];               // the k best, sorted; running best of the ordered scan
 };
 
-// Number of entries of key[0, n) that beat (k, i); entries tie by the lower index.
-__device__ __forceinline__ int rank_of(const uint32_t* key, const int* idx, int n, uint32_t k, int i) {
+// A candidate as one whole number that orders by value, then by the lower index
+__device__ __forceinline__ uint64_t cand(uint32_t key, int idx) { return (uint64_t)key << 32 | (uint32_t)~idx; }
+__device__ __forceinline__ uint32_t cand_key(uint64_t c) { return (uint32_t)(c >> 32); }
+__device__ __forceinline__ int cand_idx(uint64_t c) { return (int)~(uint32_t)c; }
+// Number of entries of list[0, n) that beat c; list is 16-byte aligned
+__device__ __forceinline__ int rank_of(const uint64_t* list, int n, uint64_t c) {
     int r = 0;
-    for (int j = 0; j < n; ++j) r += key[j] > k || (key[j] == k && idx[j] < i);
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    const u64x2* two = (const u64x2*)list;
+#pragma unroll 4
+    for (int j = 0; j < n / 2; ++j) {
+        const u64x2 q = two[j];
+        r += (q[0] > c) + (q[1] > c);
+    }
+    if (n & 1) r += list[n - 1] > c;
     return r;
 }
 __device__ __forceinline__ int rank_of_thread(const uint32_t* key, uint32_t k, int t) {
@@ -118,7 +127,7 @@ __device__ __forceinline__ int rank_of_thread(const uint32_t* key, uint32_t k, i
 
 // Exact selection by one ordered scan: 256 groups at a time in index order; a chunk is looked at only if one of its values beats the k-th of
 // the best so far.  Of a chunk only the k threads with the best (largest, then leftmost) maxima can hold winners: every element of another
-// thread is beaten by those k maxima.  Leaves the k best, sorted, in sh.bk / sh.bi[return value].
+// thread is beaten by those k maxima.  Leaves the k best, sorted, in sh.best[return value].
 template <typename T>
 __device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
     constexpr int VEC = Elem<T>::VEC;
@@ -139,7 +148,7 @@ __device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
         if (tid == 0) { sh.any = 0; sh.ncand = 0; }
         sh.key[tid] = best;
         __syncthreads();
-        const uint32_t bar = have >= k ? sh.bk[cur][k - 1] : 0;
+        const uint32_t bar = have >= k ? cand_key(sh.best[cur][k - 1]) : 0;
         if (best > bar) sh.any = 1;
         __syncthreads();
         if (!sh.any) continue;
@@ -148,18 +157,16 @@ __device__ int select_ordered(const Groups<T>& gr, int k, Shared& sh) {
             for (int j = 0; j < VEC; ++j)
                 if (gr.holds(g, j) && okey(f[j]) > bar) {
                     const int at = atomicAdd(&sh.ncand, 1);     // at most k * VEC <= 512: fits
-                    sh.ck[at] = okey(f[j]);
-                    sh.ci[at] = (int)gr.index(g, j);
+                    sh.cand[at] = cand(okey(f[j]), (int)gr.index(g, j));
                 }
         }
         __syncthreads();
         const int n = sh.ncand, old = (int)min((long)k, have);
         // ranks within the union of the old best (all of them left of the chunk) and the new candidates
         for (int i = tid; i < n + old; i += NT) {
-            const uint32_t kk = i < n ? sh.ck[i] : sh.bk[cur][i - n];
-            const int ii = i < n ? sh.ci[i] : sh.bi[cur][i - n];
-            const int r = rank_of(sh.ck, sh.ci, n, kk, ii) + rank_of(sh.bk[cur], sh.bi[cur], old, kk, ii);
-            if (r < k) { sh.bk[cur ^ 1][r] = kk; sh.bi[cur ^ 1][r] = ii; }
+            const uint64_t c = i < n ? sh.cand[i] : sh.best[cur][i - n];
+            const int r = rank_of(sh.cand, n, c) + rank_of(sh.best[cur], old, c);
+            if (r < k) sh.best[cur ^ 1][r] = c;
         }
         have += n;
         cur ^= 1;
@@ -291,7 +298,7 @@ __device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared&
             for (int j = 0; j < VEC; ++j)
                 if (gr.holds(g, j) && okey(f[j]) >= tau) {
                     const int at = atomicAdd(&sh.ncand, 1);
-                    if (at < CAP) { sh.ck[at] = okey(f[j]); sh.ci[at] = (int)gr.index(g, j); }
+                    if (at < CAP) sh.cand[at] = cand(okey(f[j]), (int)gr.index(g, j));
                 }
         };
         if (bg >= 0 && mine >= tau) {
@@ -315,8 +322,9 @@ __device__ Soft scan_row(const T* row, long v0, long v1, float c, int k, Shared&
             const int nc = sh.ncand;
             if (nc <= CAP) {
                 for (int i = tid; i < nc; i += NT) {
-                    const int r = rank_of(sh.ck, sh.ci, nc, sh.ck[i], sh.ci[i]);
-                    if (r < k) { sh.bk[0][r] = sh.ck[i]; sh.bi[0][r] = sh.ci[i]; }
+                    const uint64_t c = sh.cand[i];
+                    const int r = rank_of(sh.cand, nc, c);
+                    if (r < k) sh.best[0][r] = c;
                 }
                 __syncthreads();
                 return t;
@@ -339,7 +347,7 @@ __device__ __forceinline__ float value_lp(float x, float ref, float logs, bool h
 
 // A row without any finite value has no distribution: log probabilities -inf, entropy 0.
 template <typename T>
-__device__ void finish_row(const LogpP& p, long r, Soft a, bool huge, const uint32_t* bk, const int* bi) {
+__device__ void finish_row(const LogpP& p, long r, Soft a, bool huge, const uint64_t* best) {
     const float logs = a.s > 0.f || a.s != a.s ? log2f(a.s) : -INFINITY;
     const bool none = logs == -INFINITY;
     if (threadIdx.x == 0) {
@@ -353,8 +361,8 @@ __device__ void finish_row(const LogpP& p, long r, Soft a, bool huge, const uint
         *(float4*)(p.stats + 4 * r) = make_float4(a.ref, logs, H, huge ? 1.f : 0.f);
     }
     for (int j = threadIdx.x; j < p.k; j += NT) {
-        p.top_ids[r * p.k + j] = bi[j];
-        p.top_lp[r * p.k + j] = none ? -INFINITY : value_lp(key_value(bk[j]), a.ref, logs, huge, p.t);
+        p.top_ids[r * p.k + j] = cand_idx(best[j]);
+        p.top_lp[r * p.k + j] = none ? -INFINITY : value_lp(key_value(cand_key(best[j])), a.ref, logs, huge, p.t);
     }
 }
 
@@ -365,7 +373,7 @@ __global__ __launch_bounds__(NT) void k_token_logprobs(LogpP p) {
     int set;
     bool huge;
     const Soft a = scan_row((const T*)p.x + r * p.ld, 0, p.V, p.t * LOG2E, p.k, sh, set, huge);
-    finish_row<T>(p, r, a, huge, sh.bk[set], sh.bi[set]);
+    finish_row<T>(p, r, a, huge, sh.best[set]);
 }
 
 // Few rows: `splits` workgroups a row, each with its part's sums and its k best; k_token_logprobs_join puts them together.
@@ -380,17 +388,14 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_part(LogpP p) {
     float* o = p.part + (long)blockIdx.x * (4 + 2 * p.k);
     if (threadIdx.x == 0) { o[0] = a.ref; o[1] = a.s; o[2] = a.w; o[3] = huge ? 1.f : 0.f; }
     for (int j = threadIdx.x; j < p.k; j += NT) {
-        o[4 + j] = __uint_as_float(sh.bk[set][j]);
-        o[4 + p.k + j] = __int_as_float(sh.bi[set][j]);
+        o[4 + j] = __uint_as_float(cand_key(sh.best[set][j]));
+        o[4 + p.k + j] = __int_as_float(cand_idx(sh.best[set][j]));
     }
 }
 
 template <typename T>
 __global__ __launch_bounds__(NT) void k_token_logprobs_join(LogpP p) {
-    __shared__ uint32_t ck[SMAX * KMAX];
-    __shared__ int ci[SMAX * KMAX];
-    __shared__ uint32_t bk[KMAX];
-    __shared__ int bi[KMAX];
+    __shared__ __attribute__((aligned(16))) uint64_t list[SMAX * KMAX], best[KMAX];
     __shared__ int n;
     __shared__ Soft soft[NW];
     const long r = blockIdx.x;
@@ -417,17 +422,16 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_join(LogpP p) {
         const uint32_t kk = __float_as_uint(o[4 + j % p.k]);
         if (kk >= tau) {
             const int at = atomicAdd(&n, 1);
-            ck[at] = kk;
-            ci[at] = __float_as_int(o[4 + p.k + j % p.k]);
+            list[at] = cand(kk, __float_as_int(o[4 + p.k + j % p.k]));
         }
     }
     __syncthreads();
     for (int j = threadIdx.x; j < n; j += NT) {
-        const int rk = rank_of(ck, ci, n, ck[j], ci[j]);
-        if (rk < p.k) { bk[rk] = ck[j]; bi[rk] = ci[j]; }
+        const int rk = rank_of(list, n, list[j]);
+        if (rk < p.k) best[rk] = list[j];
     }
     __syncthreads();
-    finish_row<T>(p, r, a, huge, bk, bi);
+    finish_row<T>(p, r, a, huge, best);
 }
 
 // One pass: reads a part of a row, writes its gradient.  The tokens that carry gradients of their own (the given one, the alternatives) are read
