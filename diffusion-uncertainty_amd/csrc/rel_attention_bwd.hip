@@ -22,17 +22,19 @@ __device__ __forceinline__ void flush_diagonals(float* diag, int nl, int R, int 
         diag[wave * nl + nl - 1] += far_hi;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i <= 2 * R; i += NTHR) {
-        const int lo = i == 0 ? 0 : i + pad, hi = i == 2 * R ? nl - 1 : i + pad;
+    for (int i = threadIdx.x; i < nl; i += NTHR) diag[i] = (diag[i] + diag[nl + i]) + (diag[2 * nl + i] + diag[3 * nl + i]);
+    __syncthreads();
+    for (int i = 1 + threadIdx.x; i < 2 * R; i += NTHR) out[i] = diag[i + pad];
+    if (wave < 2) {                                            // the two ends: all that lies beyond
         float t = 0.f;
-        for (int j = lo; j <= hi; ++j)
-#pragma unroll
-            for (int x = 0; x < NWAVE; ++x) t += diag[x * nl + j];
-        out[i] = t;
+        for (int i = lane; i <= pad; i += 64) t += diag[(wave ? nl - 1 - pad : 0) + i];
+        t = wave_sum(t);
+        if (lane == 0) out[wave ? 2 * R : 0] = t;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < NWAVE * nl; i += NTHR) diag[i] = 0.f;
 }
+static_assert(NWAVE == 4, "flush_diagonals adds four waves");
 
 // ------------------------------------------------------------------------------------------------------------------------ dq
 template <typename T, int CHP>

@@ -396,6 +396,7 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_part(LogpP p) {
 template <typename T>
 __global__ __launch_bounds__(NT) void k_token_logprobs_join(LogpP p) {
     __shared__ __attribute__((aligned(16))) uint64_t list[SMAX * KMAX], best[KMAX];
+    __shared__ uint64_t bound;
     __shared__ int n;
     __shared__ Soft soft[NW];
     const long r = blockIdx.x;
@@ -405,25 +406,31 @@ __global__ __launch_bounds__(NT) void k_token_logprobs_join(LogpP p) {
     const int i = threadIdx.x & 63;
     const float* o = q + (i < p.splits ? i : 0) * (4 + 2 * p.k);
     const float o0 = o[0], o1 = o[1], o2 = o[2], o3 = o[3];
-    uint32_t tau = p.k ? __float_as_uint(o[4 + p.k - 1]) : 0;  // the best of the parts' k-th values bounds the row's k-th from below
     const bool in = i < p.splits, odd = in && o3 != 0.f && o1 != 0.f, low = odd && o1 < INFINITY && o0 < 0.f;
     Soft a = in && o3 == 0.f ? Soft{o0, o1, o2} : Soft{-REF_MAX, 0.f, 0.f};
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) {
         a = soft_join(a, Soft{__shfl_xor(a.ref, x, 64), __shfl_xor(a.s, x, 64), __shfl_xor(a.w, x, 64)}, 1.f);
-        tau = max(tau, (uint32_t)__shfl_xor((int)tau, x, 64));
     }
     const bool huge = __any(odd && !low) || (__any(low) && a.ref < -0.5f * REF_MAX);
     if (huge) a = scan_huge(Groups<T>((const T*)p.x + r * p.ld, 0, p.V), c, soft);
+    if (p.k == 0) return finish_row<T>(p, r, a, huge, best);
+    // the k-th best of the first few of every part (at least 2 k in all) bounds the row's k-th from below: few candidates are left to rank
+    auto entry = [&](int part, int j) {
+        const float* e = q + part * (4 + 2 * p.k) + 4;
+        return cand(__float_as_uint(e[j]), __float_as_int(e[p.k + j]));
+    };
+    const int few = min(p.k, (2 * p.k + p.splits - 1) / p.splits + 1), nf = p.splits * few;
+    for (int j = threadIdx.x; j < nf; j += NT) list[j] = entry(j / few, j % few);
     if (threadIdx.x == 0) n = 0;
     __syncthreads();
+    for (int j = threadIdx.x; j < nf; j += NT)
+        if (rank_of(list, nf, list[j]) == p.k - 1) bound = list[j];
+    __syncthreads();
+    const uint64_t tau = bound;
     for (int j = threadIdx.x; j < p.splits * p.k; j += NT) {
-        const float* o = q + j / p.k * (4 + 2 * p.k);
-        const uint32_t kk = __float_as_uint(o[4 + j % p.k]);
-        if (kk >= tau) {
-            const int at = atomicAdd(&n, 1);
-            list[at] = cand(kk, __float_as_int(o[4 + p.k + j % p.k]));
-        }
+        const uint64_t c = entry(j / p.k, j % p.k);
+        if (c >= tau) list[atomicAdd(&n, 1)] = c;
     }
     __syncthreads();
     for (int j = threadIdx.x; j < n; j += NT) {

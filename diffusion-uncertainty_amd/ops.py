@@ -1304,8 +1304,10 @@ def sandwich_norm_bwd(x, y, stats, dr, dz, post="rms", post_w=None, post_b=None,
         _token_tensor(dz, "dz", (x.dtype,), x.shape, x.device)
     elif dz is not None:
         raise ValueError("dz: given without a pre norm")
-    like = lambda t: torch.empty_like(t) if t is not None else None
-    g = SandwichNormGrads(like(x), like(y), like(gate), like(post_w), like(post_b), like(pre_w), like(pre_b))
+    given = [t for t in (post_w, post_b, pre_w, pre_b) if t is not None]
+    cols = iter(torch.empty((len(given), a.D), device=x.device, dtype=given[0].dtype).unbind(0) if given else ())
+    g = SandwichNormGrads(torch.empty_like(x), torch.empty_like(y), torch.empty_like(gate) if gate is not None else None,
+                          *(next(cols) if t is not None else None for t in (post_w, post_b, pre_w, pre_b)))
     a.stats, a.dr, a.dz, a.dx, a.dy, a.dgate = _a(stats), _a(dr), _a(dz), _a(g.dx), _a(g.dy), _a(g.dgate)
     a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = _a(g.dpost_w), _a(g.dpost_b), _a(g.dpre_w), _a(g.dpre_b)
     L = _lib.lib()
