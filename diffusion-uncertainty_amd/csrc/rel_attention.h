@@ -3,12 +3,13 @@
 //   P = softmax(s), o = P v, lse_i = log sum_j e^s_ij;   a row without keys: o = 0, lse = -inf, no gradient
 //   dS = P (dO v^T - D), D_i = sum_c dO_ic o_ic;  dq = scale dS k;  dk = scale dS^T q;  dv = P^T dO;  dtable[n][h] = sum of dS where map = n
 // The bias is never materialised: a head's 2R + 1 values lie in LDS (padded so that a tile near the diagonal indexes them without a clamp), and a
-// tile farther than R from the diagonal sees one value.  All products run on 16x16 matrix instructions (K = 32 for sixteen-bit elements; fp32
-// as eight K = 4 steps on the same fragments), softmax and sums in fp32.  Every product is arranged so that its result's columns are the axis the
+// tile farther than R from the diagonal sees one value.  All products run on 16x16 matrix instructions (K = 32 for sixteen-bit elements, four
+// K = 4 steps for fp32), softmax and sums in fp32.  Every product is arranged so that its result's columns are the axis the
 // wave owns (queries in the forward and dq passes, keys in the dk / dv pass): scores come out with a query's keys in one lane's registers, and go
 // straight back in as the next product's right operand - P and dS never pass through LDS.  Their key order inside a K = 32 step
 // (16 (j / 4) + 4 (lane / 16) + j % 4) is matched by reading the other operand transposed from its row-major tile.
-// dk / dv and dq are two passes (scores computed twice, 14 instead of 10 products' flops): no atomics, the same bits in every run.
+// dk / dv and dq are two passes (S and dP computed twice: 14 ch operations a pair of query and key instead of 10): dq stays in registers, nothing is
+// added by atomics from several workgroups, the bits are the same in every run.
 #pragma once
 #include <atomic>
 #include "elem.h"
@@ -323,7 +324,8 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
 [[maybe_unused]] static int key_block(int dtype, int ch) { return (dtype == DUA_DTYPE_F32 || chp_of(ch) > 64 ? 16 : 32) * NWAVE; }   // Shape::KB
 
 // dk / dv of shared kv heads: where the blocks of keys alone do not fill the chip, a group's query heads are dealt to `splits` workgroups whose sums
-// (fp32) are added in order afterwards.  2 x 8 kv heads of 4 query heads, 940 tokens of 16 bf16: 128 workgroups, 344 us a training step; 512: see below.
+// (fp32) are added in order afterwards.  2 x 8 kv heads of 4 query heads, 940 tokens of 16 bf16, forward and backward: 344 us with one workgroup a
+// block of keys (128 in all), 180 with four.
 [[maybe_unused]] static int key_splits(const dua_rel_attention_args* a) {
     const int rep = a->heads / a->kv_heads, nkb = (a->Tk + key_block(a->dtype, a->ch) - 1) / key_block(a->dtype, a->ch);
     const long wgs = (long)a->B * a->kv_heads * nkb;

@@ -696,6 +696,38 @@ def test_operators_together_against_autograd_in_64_bits():
     assert torch.equal(got["mask"].cpu().bool(), u > torch.quantile(u, 0.9, dim=1, keepdim=True))
 
 
+def test_offsets_past_32_bits():
+    """Slots of a cache and rows of logits 2^23 elements apart, a stream of more than 2^31 elements: the same bits as from small tensors."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(12)
+    T, far = 300, 1 << 23
+    base = torch.empty(T * far, device=dev, dtype=torch.bfloat16)
+    at = lambda c, w: base.as_strided((1, T, w), (T * far, far, 1), c)
+    k, v, q, do = (rnd(g, 1, T, 128, dtype=torch.bfloat16).to(dev) for _ in range(4))
+    kf, vf = at(0, 128).copy_(k), at(128, 128).copy_(v)
+    bk, table = ops.RelativeBuckets(8, 16, True, device=dev), rnd(g, 8, 2).to(dev)
+    for n in (1, T):
+        assert torch.equal(ops.rel_attention(q[:, :n], kf, vf, table, bk, heads=2), ops.rel_attention(q[:, :n], k, v, table, bk, heads=2))
+    out, s = ops.rel_attention(q, k, v, table, bk, heads=2, want_lse=True)
+    for a, b in zip(ops.rel_attention_bwd(q, kf, vf, table, bk, out, s, do, heads=2), ops.rel_attention_bwd(q, k, v, table, bk, out, s, do, heads=2)):
+        assert torch.equal(a, b)
+    x, ids, gl = rnd(g, T, 1000, dtype=torch.bfloat16).to(dev), torch.randint(0, 1000, (T,), generator=g).to(dev), rnd(g, T).to(dev)
+    xf, into = at(256, 1000)[0].copy_(x), at(1264, 1000)[0]
+    a, b = ops.token_logprobs(xf, ids, k=4), ops.token_logprobs(x, ids, k=4)
+    for m, n in zip(a, b):
+        assert torch.equal(m, n)
+    assert torch.equal(ops.token_logprobs_bwd(xf, ids, a, dlogprob=gl, out=into), ops.token_logprobs_bwd(x, ids, b, dlogprob=gl))
+    del base, kf, vf, xf, into
+    rows, D = (1 << 18) + 5, 8192
+    x, y = (torch.empty(rows, D, device=dev, dtype=torch.bfloat16).normal_() for _ in range(2))
+    r, z, st = ops.sandwich_norm(x, y, want_stats=True)
+    r8, z8, st8 = ops.sandwich_norm(x[-8:], y[-8:], want_stats=True)
+    assert torch.equal(r[-8:], r8) and torch.equal(z[-8:], z8) and torch.equal(st[-8:], st8)
+    del r, z
+    d, d8 = ops.sandwich_norm_bwd(x, y, st, y, x), ops.sandwich_norm_bwd(x[-8:], y[-8:], st8, y[-8:], x[-8:])
+    assert torch.equal(d.dx[-8:], d8.dx) and torch.equal(d.dy[-8:], d8.dy)
+
+
 def test_wide_heads_and_rows_in_a_graph():
     """Kernels with more than 64 KB of LDS (heads of 128, backward norms of 8192 columns) captured and replayed."""
     from diffusion_uncertainty_amd import ops
