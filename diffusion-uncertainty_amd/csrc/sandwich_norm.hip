@@ -114,7 +114,10 @@ template <int LANES> struct UnitSum {
     }
 };
 
-// Where a thread stands in its unit, and the columns it holds: 16-byte chunks of V elements, threads side by side, PL elements in all.  A chunk that
+// Elements of one access: 16 bytes, or all that a thread holds
+template <typename T, int PL> constexpr int chunk_of() { return PL < Elem<T>::VEC ? PL : Elem<T>::VEC; }
+
+// Where a thread stands in its unit, and the columns it holds: chunks of V elements, threads side by side, PL elements in all.  A chunk that
 // would stick out of the row lies at its end instead (the elements it shares with the chunk before do not count: valid), and so does one past
 // the row: every load is a whole, unconditional one.  (Loads behind a lane's own condition, zeros otherwise, cost half the bandwidth: the zeros wait for
 // the loads into the same registers.  16512 rows of 1152 floats: 82 us, 1024: 45 us.)
@@ -137,7 +140,7 @@ template <int V, int PL, int LANES> struct Cols {
 
 // This thread's part of a row as it lies in memory (rows may begin anywhere); elements that are not valid hold others of the row
 template <typename T, typename C, int PL> struct Part {
-    static constexpr int V = Elem<T>::VEC, N = PL / V;
+    static constexpr int V = chunk_of<T, PL>(), N = PL / V;
     typename VecOf<T, V>::type x[N];
     __device__ __forceinline__ void load(const T* p, int D) {
         if (D >= V) {
@@ -169,7 +172,7 @@ __device__ __forceinline__ void store_row(T* p, int D, const float* f) {
 // Parameters of this thread's columns; `dflt` where there are none.
 template <typename T, typename PT, typename C, int PL>
 __device__ __forceinline__ void load_param(const void* p, int D, float dflt, float* f) {
-    constexpr int V = Elem<T>::VEC;
+    constexpr int V = chunk_of<T, PL>();
 #pragma unroll
     for (int e = 0; e < PL; e += V) {
         if (!p) {
@@ -242,7 +245,7 @@ __device__ __forceinline__ void row_stats(const float* f, int D, int kind, float
 // flight while one is reduced (of the next two: no faster, 5 - 20 % slower where the registers then hold fewer waves).
 template <typename T, typename PT, int LANES, int WAVES, int PL>
 __global__ __launch_bounds__(64 * WAVES) void k_sandwich_norm(NormP p) {
-    constexpr int V = Elem<T>::VEC;
+    constexpr int V = chunk_of<T, PL>();
     typedef Cols<V, PL, LANES> C;
     __shared__ float buf[4 * MAX_WAVES];
     UnitSum<LANES> us(buf);
@@ -298,7 +301,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sandwich_norm(NormP p) {
 // sums in every run.
 template <typename T, typename PT, int LANES, int WAVES, int PL, bool LDS>
 __global__ __launch_bounds__(64 * WAVES) void k_sandwich_norm_bwd(NormP p) {
-    constexpr int V = Elem<T>::VEC;
+    constexpr int V = chunk_of<T, PL>();
     typedef Cols<V, PL, LANES> C;
     __shared__ float buf[4 * MAX_WAVES];
     extern __shared__ __attribute__((aligned(16))) float dyn[];
@@ -512,22 +515,25 @@ NormP pack(const dua_sandwich_norm_args* a) {
 
 bool aligned16(const void* q) { return ((uintptr_t)q & 15) == 0; }
 
-// The unit of a row: 16 bytes a lane up to D = 4096 (sixteen-bit elements: 8, fp32: 4), beyond it 16 waves with 8 elements a lane.
-struct Unit { int lanes, waves, per_block; };
-Unit unit_of(const dua_sandwich_norm_args* a) {
-    const int pl = a->dtype == DUA_DTYPE_F32 && a->D <= 4096 ? 4 : 8, threads = (a->D + pl - 1) / pl;
-    if (threads <= 16) return {16, 4, 16};
-    if (threads <= 32) return {32, 4, 8};
-    if (threads <= 64) return {64, 4, 4};
-    return {0, (threads + 63) / 64, 1};
+// The unit of a row: 16 bytes a lane up to D = 4096 (sixteen-bit elements: 8, fp32: 4), beyond it 16 waves with 8 elements a lane.  Backward, sixteen-bit
+// rows take 4 elements a lane too: with 8 the registers leave two waves a SIMD, and a unit of few waves leaves some of those empty (65536 rows
+// of 128 bf16 43 -> 32 us, 16512 of 1152 75 -> 57, 8192 of 2560 67 -> 57) - but units of 7 and 8 waves fill them (8192 rows of 3584: 76 us
+// against 81, of 4096: 82 against 84).
+struct Unit { int pl, lanes, waves, per_block; };
+Unit unit_of(const dua_sandwich_norm_args* a, bool backward) {
+    const bool eight = a->D > 4096 || (a->dtype != DUA_DTYPE_F32 && (!backward || (a->D + 511) / 512 >= 7));
+    const int pl = eight ? 8 : 4, threads = (a->D + pl - 1) / pl;
+    if (threads <= 16) return {pl, 16, 4, 16};
+    if (threads <= 32) return {pl, 32, 4, 8};
+    if (threads <= 64) return {pl, 64, 4, 4};
+    return {pl, 0, (threads + 63) / 64, 1};
 }
 // How the rows are dealt: the same number of workgroups to every CU (half a round more cost a third: 3 against 2 workgroups of 8 waves on 8192 rows of
 // 4096 bf16, 55 against 47 us), `waves` wavefronts a CU; each unit takes at least `least` rows where there are that many.
 struct Deal { long units, per_sample, blocks; };
-Deal deal(const dua_sandwich_norm_args* a, int waves, long least) {
+Deal deal(const dua_sandwich_norm_args* a, const Unit& u, int waves, long least) {
     Deal d{0, 1, 0};
     if (a->rows == 0) return d;
-    const Unit u = unit_of(a);
     const long most = 256L * (waves / u.waves > 1 ? waves / u.waves : 1) * u.per_block, g = a->gate ? a->gate_rows : 1, t = a->rows / g;
     long each = (a->rows + most - 1) / most;
     if (each < least) each = least;
@@ -542,27 +548,33 @@ Deal deal(const dua_sandwich_norm_args* a, int waves, long least) {
     d.blocks = (d.units + u.per_block - 1) / u.per_block;
     return d;
 }
-// Wavefronts that the kernels' registers let a CU hold (fp32 rows keep half the elements a lane).  Forward: 16512 rows of 1152 floats 54 us with 20
-// waves, 60 with 16, 67 with 24 (uneven); 8192 rows of 4096 bf16 47 us with 16.  Backward: the partial sums, 5 rows of floats a workgroup, want
-// few; 65536 rows of 128 bf16 43 us with 8 waves, 66 with 12; 16512 rows of 1152 bf16 74 us with 12, 86 with 8.
-Deal deal_fwd(const dua_sandwich_norm_args* a) { return deal(a, a->dtype == DUA_DTYPE_F32 ? 20 : 16, 1); }
-Deal deal_bwd(const dua_sandwich_norm_args* a) { return deal(a, a->dtype == DUA_DTYPE_F32 || !unit_of(a).lanes ? 12 : 8, 4); }
+// Wavefronts that the kernels' registers let a CU hold.  Forward (fp32 rows keep half the elements a lane): 16512 rows of 1152 floats 74 us with 20 or 24
+// waves, 83 with 16; 8192 rows of 4096 bf16 47 us with 16 to 24.  Backward (the partial sums, 5 rows of floats a workgroup, want few): 16512 rows
+// of 1152 floats 117 us with 12, 135 with 16; bf16 57 us with 16, 64 with 12; 8192 rows of 4096 bf16 82 us with 12, 87 with 16.
+Deal deal_fwd(const dua_sandwich_norm_args* a) { return deal(a, unit_of(a, false), a->dtype == DUA_DTYPE_F32 ? 20 : 16, 1); }
+Deal deal_bwd(const dua_sandwich_norm_args* a) {
+    const Unit u = unit_of(a, true);
+    return deal(a, u, a->dtype == DUA_DTYPE_F32 || u.pl == 8 ? 12 : 16, 4);
+}
 size_t gate_floats(const dua_sandwich_norm_args* a, const Deal& d) { return a->gate && a->gate_rows > 1 && d.per_sample > 0 ? (size_t)d.units * a->D : 0; }
 
-template <template <typename, typename, int, int, int> class L>
+template <template <typename, typename, int, int, int> class L, bool BWD>
 void dispatch(const dua_sandwich_norm_args* a, const NormP& p, unsigned grid, hipStream_t st) {
-    const Unit u = unit_of(a);
+    const Unit u = unit_of(a, BWD);
     const bool pf = a->param_dtype == DUA_DTYPE_F32;
+    const unsigned block = 64 * u.waves;
 #define GO(T, PT)                                                                                        \
     {                                                                                                    \
-        constexpr int PL = Elem<T>::VEC;                                                                 \
-        const unsigned block = 64 * u.waves;                                                             \
-        if (u.lanes == 16) L<T, PT, 16, 4, PL>::run(p, grid, block, st);                                 \
+        constexpr int PL = BWD ? 4 : Elem<T>::VEC;                                                       \
+        if (a->D > 4096) L<T, PT, 0, 16, 8>::run(p, grid, block, st);                                    \
+        else if (u.lanes == 16) L<T, PT, 16, 4, PL>::run(p, grid, block, st);                            \
         else if (u.lanes == 32) L<T, PT, 32, 4, PL>::run(p, grid, block, st);                            \
         else if (u.lanes == 64) L<T, PT, 64, 4, PL>::run(p, grid, block, st);                            \
-        else if (a->D > 4096) L<T, PT, 0, 16, 8>::run(p, grid, block, st);                               \
-        else if (u.waves > 8) L<T, PT, 0, 16, PL>::run(p, grid, block, st);                              \
-        else L<T, PT, 0, 8, PL>::run(p, grid, block, st);                                                \
+        else if (u.pl == 8) L<T, PT, 0, 8, Elem<T>::VEC>::run(p, grid, block, st);                       \
+        else if constexpr (PL == 4) {                                                                    \
+            if (u.waves > 8) L<T, PT, 0, 16, 4>::run(p, grid, block, st);                                \
+            else L<T, PT, 0, 8, 4>::run(p, grid, block, st);                                             \
+        }                                                                                                \
     }
     if (a->dtype == DUA_DTYPE_F32) GO(float, float)
     else if (a->dtype == DUA_DTYPE_BF16) { if (pf) GO(bf16_t, float) else GO(bf16_t, bf16_t) }
@@ -599,7 +611,7 @@ extern "C" int dua_sandwich_norm(const dua_sandwich_norm_args* a, void* stream) 
     const Deal d = deal_fwd(a);
     p.units = d.units;
     p.per_sample = d.per_sample;
-    dispatch<LFwd>(a, p, (unsigned)d.blocks, as_stream(stream));
+    dispatch<LFwd, false>(a, p, (unsigned)d.blocks, as_stream(stream));
     return dua_check_launch("dua_sandwich_norm");
 }
 
@@ -625,7 +637,7 @@ extern "C" int dua_sandwich_norm_bwd(const dua_sandwich_norm_args* a, void* stre
     p.part = (float*)a->workspace;
     p.gate_part = p.part + (size_t)d.blocks * 5 * a->D;
     hipStream_t st = as_stream(stream);
-    if (a->rows > 0) dispatch<LBwd>(a, p, (unsigned)d.blocks, st);
+    if (a->rows > 0) dispatch<LBwd, true>(a, p, (unsigned)d.blocks, st);
     ColsP q{};
     q.part = p.part; q.gate_part = p.gate_part; q.D = a->D; q.blocks = d.blocks;
     q.dst[0] = a->dgate; q.dst[1] = a->dpost_w; q.dst[2] = a->dpost_b; q.dst[3] = a->dpre_w; q.dst[4] = a->dpre_b;
