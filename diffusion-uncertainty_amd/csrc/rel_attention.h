@@ -54,6 +54,8 @@ struct AttP {
 // Shapes of the tiles of a type and a padded head width (a multiple of 16).
 template <typename T, int CHP> struct Shape {
     static constexpr bool F32 = sizeof(T) == 4;
+    // dS times the scale before it is rounded for its products, where the type's range asks for it (fp16); else dq and dk at the end (1 - 3 % faster)
+    static constexpr bool EARLY = __is_same(T, f16_t);
     static constexpr int KSTEP = 4 * Frag<T>::N, NP = KSTEP / 16;   // summed elements of one product; result tiles that feed one
     static constexpr int KW = (CHP + KSTEP - 1) / KSTEP * KSTEP, KS = KW / KSTEP, CT = CHP / 16;
     static constexpr int KT = F32 ? 32 : 64;              // rows of a staged tile

@@ -37,6 +37,11 @@ __device__ __forceinline__ void flush_diagonals(float* diag, int nl, int R, int 
 static_assert(NWAVE == 4, "flush_diagonals adds four waves");
 
 // ------------------------------------------------------------------------------------------------------------------------ dq
+// dq: 6 ch matrix operations a pair; a wave holds 32 queries' q, dO and dq, the keys and values pass through LDS, and every fragment read from there
+// feeds two products.  Bound by three units that take turns more than they overlap: a step of 32 x 32 pairs is 384 cycles of matrix
+// instructions, about as many of LDS reads (four waves), some 600 of vector instructions (exponentials at a quarter of the rate).  Three waves a SIMD at head
+// widths up to 64 (20 bytes of spill): 4 x 16 heads of 64, 4096 tokens bf16 1282 us a backward pass, 1356 with two.  8 x 16 heads, 1024 tokens of 64 bf16
+// in a padded batch: 83 us.
 template <typename T, int CHP>
 __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(AttP p) {
     typedef Shape<T, CHP> S;
@@ -148,7 +153,7 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(Att
 #pragma unroll
                 for (int n = 0; n < NP; ++n) {
                     rest[i] += (e[n][0] + e[n][1]) + (e[n][2] + e[n][3]);
-                    e[n] *= p.scale;
+                    if (S::EARLY) e[n] *= p.scale;
                 }
                 pf[i] = acc_frag<T>(e);
             }
@@ -170,7 +175,7 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(Att
         if (q >= p.Tq) continue;
         if (g == 0) p.dsum[row0 + q] = dt;
 #pragma unroll
-        for (int c = 0; c < CT; ++c) store4<T>(gp + q * p.dqr, 16 * c + 4 * g, p.ch, a[i][c]);
+        for (int c = 0; c < CT; ++c) store4<T>(gp + q * p.dqr, 16 * c + 4 * g, p.ch, S::EARLY ? a[i][c] : a[i][c] * p.scale);
     }
 }
 
@@ -192,17 +197,51 @@ __global__ __launch_bounds__(1024) void k_rel_attention_diag(AttP p, int nparts)
 }
 // ... and dtable[n][h]: the distances of bucket n, a wave a bucket.
 template <typename TT>
-__global__ __launch_bounds__(1024) void k_rel_attention_dtable(AttP p) {
-    const int lane = threadIdx.x & 63, h = blockIdx.x, nd = 2 * p.R + 1;
+__device__ __forceinline__ void sum_buckets(const AttP& p, int h, const float* diag) {
+    const int lane = threadIdx.x & 63, nd = 2 * p.R + 1;
     for (int n = threadIdx.x >> 6; n < p.nb; n += 16) {
         float t = 0.f;
-        for (int i = lane; i < nd; i += 64) t += p.map[i] == n ? p.diag[h * nd + i] : 0.f;
+        for (int i = lane; i < nd; i += 64) t += p.map[i] == n ? diag[i] : 0.f;
         t = wave_sum(t);
         if (lane == 0) ((TT*)p.dtable)[(long)n * p.H + h] = (TT)t;
     }
 }
+template <typename TT>
+__global__ __launch_bounds__(1024) void k_rel_attention_dtable(AttP p) { sum_buckets<TT>(p, blockIdx.x, p.diag + blockIdx.x * (2 * p.R + 1)); }
+
+// Both at once where there are few parts, a workgroup a head: runs of parts side by side (together at most 1024 sums, or one run of 2R + 1), a thread
+// a distance; the runs added in order.  A launch less: 1.5 us on the GPU, 5 us of host time; backward of 32 parts of 257 distances 78.3 us against
+// 79.8 with two kernels, of 64 parts 136.3 against 135.5.
+constexpr int FEW_PARTS = 32;
+template <typename TT>
+__global__ __launch_bounds__(1024) void k_rel_attention_dtable_few(AttP p, int nparts) {
+    __shared__ float sm[2 * RMAX + 1];
+    const int h = blockIdx.x, nd = 2 * p.R + 1, runs = max(1, 1024 / nd), per = (nparts + runs - 1) / runs;
+    for (int at = threadIdx.x; at < runs * nd; at += 1024) {
+        const int run = at / nd, i = at % nd, j0 = run * per, j1 = min(j0 + per, nparts);
+        float t = 0.f;
+#pragma unroll 8
+        for (int j = j0; j < j1; ++j) t += p.part[((long)j * p.H + h) * nd + i];
+        sm[at] = t;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nd; i += 1024)
+        for (int run = 1; run < runs; ++run) sm[i] += sm[run * nd + i];
+    __syncthreads();
+    sum_buckets<TT>(p, h, sm);
+}
+template <typename TT>
+int table_gradient(const AttP& p, int nparts, hipStream_t st) {
+    if (nparts <= FEW_PARTS) return launch<k_rel_attention_dtable_few<TT>>("dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p, nparts);
+    if (int rc = launch<k_rel_attention_diag>("dua_rel_attention_bwd", dim3((2 * p.R + 64) / 64, p.H), 1024, 0, st, p, nparts)) return rc;
+    return launch<k_rel_attention_dtable<TT>>("dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
+}
 
 // -------------------------------------------------------------------------------------------------------------------- dk, dv
+// dk, dv and the diagonal sums: 8 ch matrix operations a pair; a wave holds 32 keys' k, v, dk and dv (wide heads and fp32: 16), the queries and dO pass
+// through LDS, read as rows for the scores and as columns for the sums.  Bound by those reads: 16 keys a wave on three waves a SIMD read twice as much and
+// take 286 us a backward pass, on four 309, where 32 keys on two take 247 (8 x 16 heads, 1024 tokens of 64 bf16; 164 us are this kernel).  The sums along
+// the diagonals cost there 210 -> 246 us at radius 128, 369 at radius 512: where a tile is nearer than the radius every dS is shifted to its diagonal.
 template <typename T, int CHP>
 __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_rel_attention_dkv(AttP p) {
     typedef Shape<T, CHP> S;
@@ -373,7 +412,8 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
 #pragma unroll
-                for (int n = 0; n < NP; ++n) d[i][n] *= p.scale;
+                for (int n = 0; n < NP; ++n)
+                    if (S::EARLY) d[i][n] *= p.scale;
                 sf[i] = acc_frag<T>(d[i]);
             }
 #pragma unroll
@@ -392,6 +432,12 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
         flush_diagonals(diag, nl, p.R, S::PAD, far_lo, far_hi, part + (rep - 1) * (2 * p.R + 1));
     } else {
         for (int i = tid; i < rep * (2 * p.R + 1); i += NTHR) part[i] = 0.f;
+    }
+    if (!S::EARLY) {
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) ak[i][c] *= p.scale;
     }
     if (p.splits > 1) {
         // [split][dk, dv][B][Tk][Hk ch]
@@ -455,10 +501,9 @@ template <typename T, int CHP> struct Bwd {
             }
         }
         const int nparts = p.B * ((p.Tk + S::KB - 1) / S::KB);
-        if (int rc = launch<k_rel_attention_diag>("dua_rel_attention_bwd", dim3((2 * p.R + 64) / 64, p.H), 1024, 0, st, p, nparts)) return rc;
-        if (p.table_dtype == DUA_DTYPE_F32) return launch<k_rel_attention_dtable<float>>("dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
-        if (p.table_dtype == DUA_DTYPE_BF16) return launch<k_rel_attention_dtable<bf16_t>>("dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
-        return launch<k_rel_attention_dtable<f16_t>>("dua_rel_attention_bwd", dim3(p.H), 1024, 0, st, p);
+        if (p.table_dtype == DUA_DTYPE_F32) return table_gradient<float>(p, nparts, st);
+        if (p.table_dtype == DUA_DTYPE_BF16) return table_gradient<bf16_t>(p, nparts, st);
+        return table_gradient<f16_t>(p, nparts, st);
     }
 };
 

@@ -9,6 +9,8 @@
 // second value reaches it too is re-read whole (about k^2 / 512 of them), and the few candidates are ranked exactly.  Rows with many equal
 // values, NaN or +inf take an ordered scan of the row in the same kernel (select_ordered).
 // A row may begin anywhere and be of any length.
+// Measured: 2048 rows of 128000 bf16 110 us without alternatives (4.8 TB/s: an exponential and some six more vector instructions an element bound it), 117 with
+// 20; 4112 rows of 16385 fp32 44 us (6.1 TB/s), 53 with 8; gradients 113 us (4.8 TB/s; a copy takes 103); 4 rows of 32000: 8 + 4 us in parts.
 #include <float.h>
 #include "elem.h"
 

@@ -1420,7 +1420,7 @@ def rel_attention_bwd(q, k, v, table, buckets, out, saved, dout, heads, kv_heads
     _token_tensor(saved.lse, "saved.lse", (torch.float32,), (a.B, heads, a.Tq), q.device)
     if saved.out_lo is not None:
         _token_tensor(saved.out_lo, "saved.out_lo", (q.dtype,), (a.B, heads, a.Tq, a.ch), q.device)
-    new = lambda t: torch.empty(t.shape, device=q.device, dtype=t.dtype)
+    new = lambda t: t.new_empty(t.shape)
     dq, dk, dv, dtable = new(q), new(k), new(v), new(table)
     a.out, a.out_batch, a.out_row, a.lse, a.out_lo = _a(out), out.stride(0), out.stride(1) if a.Tq > 1 else 0, _a(saved.lse), _a(saved.out_lo)
     a.dout, a.dout_batch, a.dout_row = _a(dout), dout.stride(0), dout.stride(1) if a.Tq > 1 else 0

@@ -203,6 +203,12 @@ def test_rel_attention_custom_map_and_minus_infinite_bias():
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+def test_rel_attention_table_gradient_of_many_sequences(dt):
+    """18 sequences of three or five blocks of keys: the table's gradient is added up in two launches instead of one."""
+    attention_case(dt, 18, 40, 260, 2, 1, 16, radius=40, klen=[260 - 7 * b for b in range(18)], qstart=[11 * b for b in range(18)], seed=14)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 def test_rel_attention_strided_views(dt):
     """Thirds of a qkv projection, slots of a larger cache, rows that are not 16-byte aligned: the same bits as from contiguous copies."""
     from diffusion_uncertainty_amd import ops
