@@ -47,7 +47,7 @@ struct AttP {
     long qb, qr, kb, kr, vb, vr, ob, orow, db, dr, dqb, dqr, dkb, dkr, dvb, dvr;      // batch and row strides, elements
     const int32_t *map, *klen, *qstart;
     float *lse, *dsum, *diag, *part, *part_ml, *kv_part;
-    int B, Tq, Tk, H, Hk, ch, R, nb, causal, table_dtype, splits, nblk, swz;
+    int B, Tq, Tk, H, Hk, ch, R, nb, causal, table_dtype, splits, qsplits, nblk, swz;
     float scale;
 };
 
@@ -325,26 +325,34 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
 [[maybe_unused]] static int query_block(int dtype) { return (dtype == DUA_DTYPE_F32 ? 16 : 32) * NWAVE; }        // Shape::QB
 [[maybe_unused]] static int key_block(int dtype, int ch) { return (dtype == DUA_DTYPE_F32 || chp_of(ch) > 64 ? 16 : 32) * NWAVE; }   // Shape::KB
 
-// dk / dv of shared kv heads: where the blocks of keys alone do not fill the chip, a group's query heads are dealt to `splits` workgroups whose sums
-// (fp32) are added in order afterwards.  2 x 8 kv heads of 4 query heads, 940 tokens of 16 bf16, forward and backward: 344 us with one workgroup a
-// block of keys (128 in all), 180 with four.
-[[maybe_unused]] static int key_splits(const dua_rel_attention_args* a) {
+// dk / dv where the blocks of keys alone do not fill the chip: a group's query heads are dealt to `heads` workgroups, and of single heads the tiles of
+// queries to `tiles`; their sums (fp32) are added in order afterwards.  2 x 8 kv heads of 4 query heads, 940 tokens of 16 bf16, forward and backward: 344 us
+// with one workgroup a block of keys (128 in all), 180 with four.  @@
+struct KeySplits { int heads, tiles; };
+[[maybe_unused]] static KeySplits key_splits(const dua_rel_attention_args* a) {
     const int rep = a->heads / a->kv_heads, nkb = (a->Tk + key_block(a->dtype, a->ch) - 1) / key_block(a->dtype, a->ch);
     const long wgs = (long)a->B * a->kv_heads * nkb;
-    int s = 1;
-    for (int d = 2; d <= rep && wgs * s < 512; ++d)
-        if (rep % d == 0) s = d;
+    KeySplits s{1, 1};
+    for (int d = 2; d <= rep && wgs * s.heads < 512; ++d)
+        if (rep % d == 0) s.heads = d;
+    const long now = wgs * s.heads, tiles = a->Tq / (a->dtype == DUA_DTYPE_F32 ? 64 : 128);        // two of Shape::KT
+    if (s.heads == rep && now > 0 && now < 256) {
+        const long t = (512 + now - 1) / now;
+        s.tiles = (int)(t < tiles ? t : (tiles > 1 ? tiles : 1));
+    }
     return s;
 }
 
-// Workspace of the backward pass: D of every row, the diagonal sums of every head, and of every block of keys and head; dk and dv of split groups.
+// Workspace of the backward pass: D of every row, the diagonal sums of every head, and of every block of keys (and share of the queries) and head; dk
+// and dv of the shares.
 [[maybe_unused]] static size_t rel_attention_bwd_floats(const dua_rel_attention_args* a) {
     const size_t rows = (size_t)a->B * a->heads * a->Tq, nkb = (a->Tk + key_block(a->dtype, a->ch) - 1) / key_block(a->dtype, a->ch);
-    return (rows + (1 + a->B * nkb) * a->heads * (2 * a->radius + 1) + 3) / 4 * 4;
+    return (rows + (1 + a->B * nkb * key_splits(a).tiles) * a->heads * (2 * a->radius + 1) + 3) / 4 * 4;
 }
 
 [[maybe_unused]] static size_t rel_attention_bwd_bytes(const dua_rel_attention_args* a) {
-    const int s = key_splits(a);
+    const KeySplits k = key_splits(a);
+    const int s = k.heads * k.tiles;
     return (rel_attention_bwd_floats(a) + (s > 1 ? 2 * (size_t)s * a->B * a->Tk * a->kv_heads * a->ch : 0)) * sizeof(float);
 }
 

@@ -255,7 +255,7 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     float* const diag = lut + nl;                                          // [wave][nl]: a head's sums of dS along the diagonals
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
     const Where w = place(p, 1, blockIdx.x);
-    const int split = blockIdx.y;
+    const int split = blockIdx.y, qsplit = split % p.qsplits;
     if (w.b >= p.B) return;
     const int k0 = w.blk * S::KB, qs = start_of(p, w.b);
     const int nk = p.causal ? max(0, min(keys_of(p, w.b), qs + p.Tq)) : keys_of(p, w.b);   // (what lies behind it is not read: no query sees it)
@@ -278,9 +278,11 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
         for (int c = 0; c < CT; ++c) { ak[i][c] = ZERO4; av[i][c] = ZERO4; }
     }
     const float sl = p.scale * LOG2E;
-    const int rep = p.H / p.Hk / p.splits, h0 = w.hk * (p.H / p.Hk) + split * rep;   // this workgroup's query heads
-    // tiles of queries that see this block's first key (position >= k0), head after head of the group
-    const int qbeg = p.causal ? max(0, k0 - qs) / QT : 0, per = max(0, (p.Tq + QT - 1) / QT - qbeg), total = k0 < nk ? per * rep : 0;
+    const int rep = p.H / p.Hk / (p.splits / p.qsplits), h0 = w.hk * (p.H / p.Hk) + split / p.qsplits * rep;   // this workgroup's query heads
+    // tiles of queries that see this block's first key (position >= k0), head after head of the group; of a single head (qsplits > 1) a share of them
+    const int qmin = p.causal ? max(0, k0 - qs) / QT : 0, all_tiles = max(0, (p.Tq + QT - 1) / QT - qmin);
+    const int qbeg = qmin + (int)((long)all_tiles * qsplit / p.qsplits), per = qmin + (int)((long)all_tiles * (qsplit + 1) / p.qsplits) - qbeg;
+    const int total = k0 < nk ? per * rep : 0;
     Carrier<T, CHP, QT> cq(p.qr, p.ch, tid), cd(p.dr, p.ch, tid);
     float row_next = 0.f;
     auto fetch = [&](int t) {
@@ -295,7 +297,7 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     };
     for (int i = tid; i < NWAVE * nl; i += NTHR) diag[i] = 0.f;
     float far_lo = 0.f, far_hi = 0.f;
-    float* const part = p.part + (((long)w.b * p.nblk + w.blk) * p.H + h0) * (2 * p.R + 1);
+    float* const part = p.part + ((((long)w.b * p.nblk + w.blk) * p.qsplits + qsplit) * p.H + h0) * (2 * p.R + 1);
     if (total > 0) fetch(0);
     for (int t = 0; t < total; ++t) {
         if (t % per == 0) {
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     }
 }
 
-// dk and dv of split groups: the splits' sums in their order, four elements a thread
+// dk and dv of split blocks: the splits' sums in their order, four elements a thread
 template <typename T>
 __global__ __launch_bounds__(NTHR) void k_rel_attention_kv_join(AttP p) {
     const int row = p.Hk * p.ch, quads = row / 4;
@@ -500,7 +502,7 @@ template <typename T, int CHP> struct Bwd {
                 if (int rc = launch<k_rel_attention_kv_join<T>>("dua_rel_attention_bwd", dim3(stream_grid(quads, NTHR)), NTHR, 0, st, p)) return rc;
             }
         }
-        const int nparts = p.B * ((p.Tk + S::KB - 1) / S::KB);
+        const int nparts = p.B * ((p.Tk + S::KB - 1) / S::KB) * p.qsplits;
         if (p.table_dtype == DUA_DTYPE_F32) return table_gradient<float>(p, nparts, st);
         if (p.table_dtype == DUA_DTYPE_BF16) return table_gradient<bf16_t>(p, nparts, st);
         return table_gradient<f16_t>(p, nparts, st);
@@ -519,7 +521,9 @@ extern "C" int dua_rel_attention_bwd(const dua_rel_attention_args* a, void* stre
                 "dua_rel_attention_bwd: workspace smaller than dua_rel_attention_workspace_bytes, or not 16-byte aligned");
     AttP p = pack(a);
     p.dsum = (float*)a->workspace;
-    p.splits = key_splits(a);
+    const KeySplits ks = key_splits(a);
+    p.splits = ks.heads * ks.tiles;
+    p.qsplits = ks.tiles;
     p.kv_part = p.dsum + rel_attention_bwd_floats(a);
     p.diag = p.dsum + (size_t)a->B * a->heads * a->Tq;
     p.part = p.diag + (size_t)a->heads * (2 * a->radius + 1);

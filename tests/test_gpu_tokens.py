@@ -209,6 +209,14 @@ def test_rel_attention_table_gradient_of_many_sequences(dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("Tq,Tk,H,Hk,ch,causal,klen,qstart", [(520, 150, 2, 2, 64, False, None, None), (333, 333, 4, 2, 16, True, [300], None),
+                                                              (300, 140, 1, 1, 128, True, [130], [-100]), (400, 3, 2, 1, 72, False, [0], None)])
+def test_rel_attention_gradients_of_one_sequence(dt, Tq, Tk, H, Hk, ch, causal, klen, qstart):
+    """Few blocks of keys: dk and dv summed over shares of the queries, some of which see none of a block's keys."""
+    attention_case(dt, 1, Tq, Tk, H, Hk, ch, causal, klen=klen, qstart=qstart, seed=15)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 def test_rel_attention_strided_views(dt):
     """Thirds of a qkv projection, slots of a larger cache, rows that are not 16-byte aligned: the same bits as from contiguous copies."""
     from diffusion_uncertainty_amd import ops
