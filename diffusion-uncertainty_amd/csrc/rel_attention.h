@@ -327,7 +327,9 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
 
 // dk / dv where the blocks of keys alone do not fill the chip: a group's query heads are dealt to `heads` workgroups, and of single heads the tiles of
 // queries to `tiles`; their sums (fp32) are added in order afterwards.  2 x 8 kv heads of 4 query heads, 940 tokens of 16 bf16, forward and backward: 344 us
-// with one workgroup a block of keys (128 in all), 180 with four.  @@
+// with one workgroup a block of keys (128 in all), 180 with four.  Shares of the queries, backward: 1 x 8 heads, 1024 tokens of 64
+// fp32 (128 workgroups) 207 -> 154 us, 2 heads, 2048 tokens of 128 bf16 (64) 190 -> 133, 2 x 12 heads, 1024 tokens of 72 fp32 (384) 392 -> 338; 4 x 8 heads,
+// 1024 tokens of 64 bf16 (256) 106 -> 109: the sums' way through memory is all that is left there.
 struct KeySplits { int heads, tiles; };
 [[maybe_unused]] static KeySplits key_splits(const dua_rel_attention_args* a) {
     const int rep = a->heads / a->kv_heads, nkb = (a->Tk + key_block(a->dtype, a->ch) - 1) / key_block(a->dtype, a->ch);
@@ -336,7 +338,7 @@ struct KeySplits { int heads, tiles; };
     for (int d = 2; d <= rep && wgs * s.heads < 512; ++d)
         if (rep % d == 0) s.heads = d;
     const long now = wgs * s.heads, tiles = a->Tq / (a->dtype == DUA_DTYPE_F32 ? 64 : 128);        // two of Shape::KT
-    if (s.heads == rep && now > 0 && now < 256) {
+    if (s.heads == rep && now > 0 && now < 512) {
         const long t = (512 + now - 1) / now;
         s.tiles = (int)(t < tiles ? t : (tiles > 1 ? tiles : 1));
     }
