@@ -54,8 +54,9 @@ struct AttP {
 // Shapes of the tiles of a type and a padded head width (a multiple of 16).
 template <typename T, int CHP> struct Shape {
     static constexpr bool F32 = sizeof(T) == 4;
-    // dS times the scale before it is rounded for its products, where the type's range asks for it (fp16); else dq and dk at the end (1 - 3 % faster)
-    static constexpr bool EARLY = __is_same(T, f16_t);
+    // fp16 ends at 2^-24 and 65504: the backward passes take P and dS times powers of two there (P_SHIFT, in_range); bf16 and fp32 hold them as they are
+    static constexpr bool NARROW = __is_same(T, f16_t);
+    static constexpr float P_SHIFT = NARROW ? 14.f : 0.f;   // log2
     static constexpr int KSTEP = 4 * Frag<T>::N, NP = KSTEP / 16;   // summed elements of one product; result tiles that feed one
     static constexpr int KW = (CHP + KSTEP - 1) / KSTEP * KSTEP, KS = KW / KSTEP, CT = CHP / 16;
     static constexpr int KT = F32 ? 32 : 64;              // rows of a staged tile
@@ -240,6 +241,33 @@ __device__ __forceinline__ float col_max(float v) {
 __device__ __forceinline__ float col_sum(float v) {
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
+}
+
+// dS as fp16 operands.  Its size is the incoming gradient's, from 1e-9 (a mean over many tokens) to past 65504 (loss scaling), so it is multiplied by a
+// power of two f of the result column's own (a query of dq, a key of dk), whose accumulators carry the same factor until they are stored: exact, and every
+// operand is rounded relative to the column's largest one (to 2^-11 of its own size down to 2^-21 of that, to 2^-32 of the largest below).  f falls when a
+// value would pass 2^15, to where the largest is in [2^7, 2^8): with the first values that count, then hardly ever.  Rounded unscaled, a dO of 1e-5 lost
+// half of dq.
+constexpr float F_START = 0x1p100f;
+__device__ __forceinline__ float pow2_inverse(float f) { return __int_as_float(0x7F000000 - __float_as_int(f)); }
+template <int NP, int CT>
+__device__ __forceinline__ void in_range(f32x4* e, float& f, f32x4* acc) {
+    float mx = 0.f;
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, fabsf(e[n][r]));
+    if (__any(mx * f > 32768.f)) {
+        const float top = col_max(mx);
+        if (top * f > 32768.f) {                                            // (then top > 2^-85, or infinite: exponents stay in [-120, 92])
+            const float nf = __int_as_float((127 + 8 - __builtin_amdgcn_frexp_expf(top)) << 23), by = nf * pow2_inverse(f);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) acc[c] *= by;
+            f = nf;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NP; ++n) e[n] *= f;
 }
 
 // Where a tile of keys [k0, k0 + n) lies for queries at positions [pmin, pmax]: -1 / 1: all of it at least R to the left / right (one bias value), 0: near.

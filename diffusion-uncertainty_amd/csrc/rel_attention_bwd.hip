@@ -12,8 +12,8 @@ __device__ __forceinline__ void diagonals(f32x4 x, float& a, float& b) {
 }
 
 // The four waves' sums along the diagonals (diag [wave][nl], distance 0 at R + pad) clipped to 2R + 1 distances, into this workgroup's row of the
-// partial sums; then zeros again.
-__device__ __forceinline__ void flush_diagonals(float* diag, int nl, int R, int pad, float far_lo, float far_hi, float* out) {
+// partial sums, times `unit`; then zeros again.
+__device__ __forceinline__ void flush_diagonals(float* diag, int nl, int R, int pad, float far_lo, float far_hi, float unit, float* out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
@@ -24,12 +24,12 @@ __device__ __forceinline__ void flush_diagonals(float* diag, int nl, int R, int 
     __syncthreads();
     for (int i = threadIdx.x; i < nl; i += NTHR) diag[i] = (diag[i] + diag[nl + i]) + (diag[2 * nl + i] + diag[3 * nl + i]);
     __syncthreads();
-    for (int i = 1 + threadIdx.x; i < 2 * R; i += NTHR) out[i] = diag[i + pad];
+    for (int i = 1 + threadIdx.x; i < 2 * R; i += NTHR) out[i] = diag[i + pad] * unit;
     if (wave < 2) {                                            // the two ends: all that lies beyond
         float t = 0.f;
         for (int i = lane; i <= pad; i += 64) t += diag[(wave ? nl - 1 - pad : 0) + i];
         t = wave_sum(t);
-        if (lane == 0) out[wave ? 2 * R : 0] = t;
+        if (lane == 0) out[wave ? 2 * R : 0] = t * unit;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < NWAVE * nl; i += NTHR) diag[i] = 0.f;
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(Att
     const T* dp = (const T*)p.dout + w.b * p.db + (long)w.h * p.ch;
     const long row0 = ((long)w.b * p.H + w.h) * p.Tq;
     frag qf[NQ][KS], df[NQ][KS];
-    float ls[NQ], D[NQ], rest[NQ];
+    float ls[NQ], D[NQ], rest[NQ], f[NQ];
     f32x4 a[NQ][CT];
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
@@ -93,6 +93,7 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(Att
         ls[i] = there ? p.lse[row0 + q] * LOG2E : INFINITY;
         if (ls[i] == -INFINITY) ls[i] = INFINITY;                          // a row without keys: P = 0
         rest[i] = 0.f;
+        f[i] = F_START;
 #pragma unroll
         for (int c = 0; c < CT; ++c) a[i][c] = ZERO4;
     }
@@ -151,10 +152,8 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(Att
                         for (int r = 0; r < 4; ++r) e[n][r] = s[i][n][r] == 0.f ? 0.f : e[n][r];
                 }
 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    rest[i] += (e[n][0] + e[n][1]) + (e[n][2] + e[n][3]);
-                    if (S::EARLY) e[n] *= p.scale;
-                }
+                for (int n = 0; n < NP; ++n) rest[i] += (e[n][0] + e[n][1]) + (e[n][2] + e[n][3]);
+                if constexpr (S::NARROW) in_range<NP, CT>(e, f[i], a[i]);
                 pf[i] = acc_frag<T>(e);
             }
 #pragma unroll
@@ -175,7 +174,7 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(Att
         if (q >= p.Tq) continue;
         if (g == 0) p.dsum[row0 + q] = dt;
 #pragma unroll
-        for (int c = 0; c < CT; ++c) store4<T>(gp + q * p.dqr, 16 * c + 4 * g, p.ch, S::EARLY ? a[i][c] : a[i][c] * p.scale);
+        for (int c = 0; c < CT; ++c) store4<T>(gp + q * p.dqr, 16 * c + 4 * g, p.ch, S::NARROW ? a[i][c] * p.scale * pow2_inverse(f[i]) : a[i][c] * p.scale);
     }
 }
 
@@ -264,9 +263,12 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     const T* vp = (const T*)p.v + w.b * p.vb + (long)w.hk * p.ch;
     frag kf[NK][KS], vf[NK][KS];
     f32x4 ak[NK][CT], av[NK][CT];
+    float f[NK];
+    constexpr float UNIT = S::NARROW ? 0x1p-14f : 1.f;                       // 2^-P_SHIFT: P, and dS with it, are 2^P_SHIFT times themselves here
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
         const int kk = kw + 16 * i + (lane & 15);
+        f[i] = F_START;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int c = S::KSTEP * s + Frag<T>::N * g;
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     for (int t = 0; t < total; ++t) {
         if (t % per == 0) {
             __syncthreads();                                                // (the last head's bias is read until here)
-            if (t > 0) flush_diagonals(diag, nl, p.R, S::PAD, far_lo, far_hi, part + (t / per - 1) * (2 * p.R + 1));
+            if (t > 0) flush_diagonals(diag, nl, p.R, S::PAD, far_lo, far_hi, UNIT, part + (t / per - 1) * (2 * p.R + 1));
             far_lo = far_hi = 0.f;
             load_lut(p, h0 + t / per, S::PAD, lut);
         }
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
         float* const row_ls = rows + (t & 1) * 2 * QT, *const row_d = row_ls + QT;
         cq.put(Qt, p.ch, tid);
         cd.put(Dt, p.ch, tid);
-        if (tid < QT) row_ls[tid] = row_next == -INFINITY ? INFINITY : row_next * LOG2E;   // no keys, no query: P = 0
+        if (tid < QT) row_ls[tid] = row_next == -INFINITY ? INFINITY : row_next * LOG2E - S::P_SHIFT;   // no keys, no query: P = 0
         else if (tid < 2 * QT) row_ls[tid] = row_next;
         __syncthreads();
         if (t + 1 < total) fetch(t + 1);
@@ -413,9 +415,7 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
             }
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
-#pragma unroll
-                for (int n = 0; n < NP; ++n)
-                    if (S::EARLY) d[i][n] *= p.scale;
+                if constexpr (S::NARROW) in_range<NP, CT>(d[i], f[i], ak[i]);
                 sf[i] = acc_frag<T>(d[i]);
             }
 #pragma unroll
@@ -431,16 +431,20 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_r
     }
     __syncthreads();
     if (total > 0) {
-        flush_diagonals(diag, nl, p.R, S::PAD, far_lo, far_hi, part + (rep - 1) * (2 * p.R + 1));
+        flush_diagonals(diag, nl, p.R, S::PAD, far_lo, far_hi, UNIT, part + (rep - 1) * (2 * p.R + 1));
     } else {
         for (int i = tid; i < rep * (2 * p.R + 1); i += NTHR) part[i] = 0.f;
     }
-    if (!S::EARLY) {
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+    for (int i = 0; i < NK; ++i)
 #pragma unroll
-            for (int c = 0; c < CT; ++c) ak[i][c] *= p.scale;
-    }
+        for (int c = 0; c < CT; ++c) {
+            ak[i][c] *= p.scale;
+            if constexpr (S::NARROW) {
+                ak[i][c] = ak[i][c] * UNIT * pow2_inverse(f[i]);
+                av[i][c] *= UNIT;
+            }
+        }
     if (p.splits > 1) {
         // [split][dk, dv][B][Tk][Hk ch]
         const long row = (long)p.Hk * p.ch, all = (long)p.B * p.Tk * row;

@@ -281,6 +281,71 @@ def test_rel_attention_gradient_against_differences():
         assert abs(diff - have) < 1e-5 * size + 1e-6, (n, diff, have)
 
 
+def fp16_gradient_case(q, k, v, table, bk, do, H, Hk, scale, causal=False, qstart=None):
+    """Gradients in fp16 against 64 bits where nothing but the operands' rounding is allowed for: every dS and P counts relative to the largest one that goes
+    into the same sum, whatever the size of dO.
+
+    dS is multiplied by a power of two that keeps the largest dS of a sum at 2^7 or above before it is rounded: one that then falls below 2^-14 is off by
+    at most 2^-25, that is 2^-32 of the largest; P is multiplied by 2^14, off by at most 2^-39 there.  Nothing else is absolute (close() adds the
+    result's own half step below 2^-14)."""
+    from diffusion_uncertainty_amd import ops
+    B, Tq, ch, Tk = q.shape[0], q.shape[1], q.shape[2] // H, k.shape[1]
+    D = lambda t: None if t is None else t.to(dev)
+    r = oracle.rel_attention(q, k, v, table, bk.map.cpu(), H, Hk, causal, scale, None, qstart, do)
+    e = half_step(torch.float16)
+    w = (2 * ((ch + 8) * r["logit"] + 8) * U + (Tk + 8) * U).max()
+    ds = w + (ch + 4) * U + e * e + e
+    size = lambda t: t.double().abs().max()
+    ds_max = 2 * do.double().abs().reshape(B, Tq, H, ch).sum(3).max() * size(v)                       # |dP| + |D| at most
+    sc = abs(scale)
+    kw = dict(heads=H, kv_heads=Hk, causal=causal, scale=scale, qstart=D(qstart))
+    a = (D(q), D(k), D(v), D(table), bk)
+    out, s = ops.rel_attention(*a, want_lse=True, **kw)
+    got = dict(zip(("dq", "dk", "dv", "dtable"), ops.rel_attention_bwd(*a, out, s, D(do), **kw)))
+    n = H // Hk * Tq
+    assert r["dq"].abs().max() < 65504 and r["dk"].abs().max() < 65504 and r["dv"].abs().max() < 65504
+    close(got["dq"], r["dq"], r["adq"] * (ds + (Tk + 8) * U) + e * r["dq"].abs() + Tk * 2.0 ** -32 * ds_max * size(k) * sc, "dq")
+    close(got["dk"], r["dk"], r["adk"] * (ds + (n + 8) * U) + e * r["dk"].abs() + n * 2.0 ** -32 * ds_max * size(q) * sc, "dk")
+    close(got["dv"], r["dv"], r["adv"] * (w + e + (n + 8) * U) + e * r["dv"].abs() + n * 2.0 ** -39 * size(do), "dv")
+    return got, r
+
+
+@pytest.mark.parametrize("dout", [1e3, 1.0, 1e-3, 1e-5])
+@pytest.mark.parametrize("Tq,Tk,H,Hk,ch", [(1, 300, 2, 1, 64), (130, 200, 2, 1, 64), (400, 400, 1, 1, 40), (200, 70, 2, 2, 128)])
+def test_rel_attention_fp16_gradients_of_any_size(dout, Tq, Tk, H, Hk, ch):
+    """Gradients of a mean over many tokens (far below 1) and loss-scaled ones: dq, dk, dv lose no more than their type forces."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(31)
+    h = torch.float16
+    q, k, v, do = rnd(g, 1, Tq, H * ch, dtype=h), rnd(g, 1, Tk, Hk * ch, dtype=h), rnd(g, 1, Tk, Hk * ch, dtype=h), rnd(g, 1, Tq, H * ch, dtype=h, scale=dout)
+    do[:, ::3] *= 2.0 ** -6                                                            # rows of different size share a key
+    bk = ops.RelativeBuckets(8, 16, True, device=dev)
+    fp16_gradient_case(q, k, v, rnd(g, 8, H, dtype=h), bk, do, H, Hk, 1.0 / math.sqrt(ch))
+
+
+def test_rel_attention_fp16_gradients_past_the_types_range():
+    """dS times the scale beyond 65504 with gradients that fp16 holds; a key that every query gives a probability near 2^-27; queries whose dS vary by 2^40."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(32)
+    h, ch = torch.float16, 64
+    bk = ops.RelativeBuckets(8, 16, True, device=dev)
+    zero = torch.zeros(8, 1, dtype=h)
+    q, k = rnd(g, 1, 90, ch, dtype=h, scale=2.0 ** -9), rnd(g, 1, 8, ch, dtype=h, scale=2.0 ** -9)
+    v, do = rnd(g, 1, 8, ch, dtype=h, scale=8.0), rnd(g, 1, 90, ch, dtype=h, scale=256.0)
+    got, r = fp16_gradient_case(q, k, v, zero, bk, do, 1, 1, 64.0)
+    assert r["dq"].abs().max() > 100
+    q, k, v, do = (rnd(g, 1, 150, ch, dtype=h) for _ in range(4))
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[:, 5::7, 0] = -14.0                                                              # scores 14 below the rest: P about 2^-27
+    got, r = fp16_gradient_case(q, k, v, rnd(g, 8, 1, dtype=h), bk, do, 1, 1, 0.125)
+    assert r["dv"][:, 5::7].abs().max() < 1e-3
+    q, k, v, do = (rnd(g, 1, 150, ch, dtype=h) for _ in range(4))
+    do[:, :75] *= 2.0 ** -20
+    do[:, 75:] *= 2.0 ** 10
+    do[:, 100] *= 2.0 ** 4
+    fp16_gradient_case(q, k, v, rnd(g, 8, 1, dtype=h), bk, do, 1, 1, 0.125, causal=True)
+
+
 # ---------------------------------------------------------------------------------------------------------- sandwich norm
 def norm_case(dt, shape, post, pre, gate_rows, param_dt=torch.float32, weights=True, shifts=True, res_scale=0.7, seed=0, offset=0.0, grads=True):
     from diffusion_uncertainty_amd import ops
