@@ -94,14 +94,18 @@ __device__ __forceinline__ int keys_of(const AttP& p, int b) { return p.klen ? m
 __device__ __forceinline__ int start_of(const AttP& p, int b) { return p.qstart ? min(max(p.qstart[b], -(1 << 30)), 1 << 30) : 0; }
 
 // Bias of head h at clipped distance index i in [0, 2R], in log2 units; a map entry outside [0, nb) adds nothing, a value below -1e30 (a mask of the
-// type's lowest value) is -inf: in log2 units it would leave fp32's range, and beside it a score has no digits.
+// type's lowest value) is -inf: in log2 units it would leave fp32's range.  Finite values are taken as between -BIAS_MAX and BIAS_MAX, the range of fp16:
+// beside -1e9 a score, the row's maximum and lse have no digits left, P as the gradients compute it again would be 2^(+-64), and what such a bias says -
+// not to be seen beside any other key - -BIAS_MAX says as well.
+constexpr float BIAS_MAX = 65504.f;
 __device__ __forceinline__ float bias_at(const AttP& p, int h, int i) {
     const int m = p.map[i];
     if (m < 0 || m >= p.nb) return 0.f;
     const long at = (long)m * p.H + h;
     const float v = p.table_dtype == DUA_DTYPE_F32 ? ((const float*)p.table)[at]
                                                    : (p.table_dtype == DUA_DTYPE_BF16 ? (float)((const bf16_t*)p.table)[at] : (float)((const f16_t*)p.table)[at]);
-    return v < -1e30f ? -INFINITY : LOG2E * v;
+    if (v < -1e30f) return -INFINITY;
+    return LOG2E * (v < -BIAS_MAX ? -BIAS_MAX : (v > BIAS_MAX && v < INFINITY ? BIAS_MAX : v));       // (+inf and NaN stay)
 }
 // lut[rel + R + pad], rel clipped to [-R, R]
 __device__ __forceinline__ void load_lut(const AttP& p, int h, int pad, float* lut) {

@@ -1392,8 +1392,8 @@ def rel_attention(q, k, v, table, buckets, heads, kv_heads=None, causal=False, s
     q [B, Tq, heads * ch], k / v [B, Tk, kv_heads * ch] (views with unit stride along the last dimension: thirds of a qkv projection, slots
     of a cache), head widths up to 128 in multiples of 8 (fp32: 4); query head h attends to kv head h // (heads // kv_heads); table [num_buckets, heads] in fp32 or q's
     type; klen / qstart int32 [B].  A query without keys gives zeros; keys behind klen (causal: or the last query)
-    are not read; a table value below -1e30 masks its distances.  Tq = 1 with qstart = klen - 1
-    is decoding.  want_lse=True: also RelAttentionSaved(lse [B, heads, Tq] = log sum e^s, out_lo: what out's rounding left), for the backward pass."""
+    are not read; a table value below -1e30 masks its distances, other finite ones are taken as between -65504 and 65504 (beside a larger one
+    a score has no digits in fp32).  Tq = 1 with qstart = klen - 1 is decoding.  want_lse=True: also RelAttentionSaved(lse [B, heads, Tq] = log sum e^s, out_lo: what out's rounding left), for the backward pass."""
     a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lse = lo = None

@@ -635,7 +635,7 @@ int dua_sandwich_norm_bwd(const dua_sandwich_norm_args* args_host, void* stream)
  * out_lo [B][heads][Tq][ch] = what out's rounding to bf16 / fp16 left, 16-byte aligned (NULL: not kept; the backward pass then takes out as it
  * is, and its gradients carry that rounding).  A query
  * without keys gives zeros (lse = -inf).  Keys behind klen or, with causal,
- * behind the last query are not read; a table value below -1e30 masks its distances.  q, out [B][Tq][heads * ch], k, v [B][Tk][kv_heads * ch] with strides
+ * behind the last query are not read; a table value below -1e30 masks its distances, other finite ones are taken as between -65504 and 65504.  q, out [B][Tq][heads * ch], k, v [B][Tk][kv_heads * ch] with strides
  * of their own (elements); query head h reads kv head h / (heads / kv_heads);
  * ch <= 128, a multiple of 8 (fp32: 4); row strides below 2^24.  table [num_buckets][heads] (table_dtype: fp32 or
  * dtype), bucket_map [2 radius + 1]: entries outside [0, num_buckets) add no bias; radius <= 1024.  Tq = 1 is decoding. */

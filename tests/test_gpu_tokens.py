@@ -166,6 +166,57 @@ def test_rel_attention_table_of_the_lowest_value():
         assert torch.isfinite(a).all() and torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("mask", [-65504.0, -1e6, -1e9, -9e29, 1e9])
+def test_rel_attention_masks_of_large_finite_values(dt, mask):
+    """A bias of +-1e9: a query that sees nothing else has the softmax of its scores alone (a common shift), queries that see other keys too do not see
+    those of -1e9.  Beside 65504 a score is rounded to half a step of 65504 log2 e, 2^-8 log2 units; so are the row's maximum with its sum, and lse (2^-9
+    and once more 2^-8 on its way back): P is off by 3 2^-8 ln 2 + 2^-9 = 0.011 at most, before normalising and after."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(41)
+    x = 2 * 0.011
+    bk = ops.RelativeBuckets(8, 16, True, device=dev)
+    far = int(bk.map[0])                                                             # the bucket of keys 16 and more to the left
+    for B, Tq, Tk, H, Hk, ch in ((2, 70, 100, 2, 1, 64), (1, 1, 100, 4, 2, 64), (1, 2, 1000, 2, 2, 40), (1, 40, 900, 1, 1, 128)):
+        q, k, v, do = rnd(g, B, Tq, H * ch, dtype=dt), rnd(g, B, Tk, Hk * ch, dtype=dt), rnd(g, B, Tk, Hk * ch, dtype=dt), rnd(g, B, Tq, H * ch, dtype=dt)
+        table = rnd(g, 8, H)
+        table[far] = mask
+        D = lambda t: t.to(dev)
+        for start, causal in ((5000, False), (5000, True), (Tk - Tq, True), (Tk // 2, False)):
+            alone = start == 5000
+            qs = torch.full((B,), start, dtype=torch.int32)
+            t0 = table.clone()
+            if alone:
+                t0[far] = 0.0
+            elif mask > 0:
+                continue
+            r = oracle.rel_attention(q, k, v, t0, bk.map.cpu(), H, Hk, causal, None, None, qs, do)
+            tol = attention_bounds(r, dt, ch, Tk, Tq, H // Hk)
+            kw = dict(heads=H, kv_heads=Hk, causal=causal, qstart=D(qs))
+            out, s = ops.rel_attention(D(q), D(k), D(v), D(table), bk, want_lse=True, **kw)
+            got = ops.rel_attention_bwd(D(q), D(k), D(v), D(table), bk, out, s, D(do), **kw)
+            y = x if alone else 0.0
+            close(out, r["out"], tol["out"] + y * r["pv"], "out")
+            for n, t in zip(("dq", "dk", "dv", "dtable"), got):
+                close(t, r[n], tol[n] + y * r["a" + n] + 1e-30, n)
+
+
+def test_rel_attention_table_without_a_value():
+    """+inf and NaN in the table are not clipped: a query that sees them has no result."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(42)
+    q, k, v = (rnd(g, 1, 40, 64).to(dev) for _ in range(3))
+    bk = ops.RelativeBuckets(8, 16, True, device=dev)
+    near = min(d for d in range(17) if bk.map[16 - d] == bk.map[0])                  # the bucket's nearest distance
+    for bad in (math.inf, math.nan):
+        table = rnd(g, 8, 2)
+        table[int(bk.map[0]), 1] = bad
+        for n in (1, 40):
+            out = ops.rel_attention(q[:, :n], k, v, table.to(dev), bk, heads=2, qstart=torch.full((1,), 39 if n == 1 else 0, dtype=torch.int32, device=dev)).view(n, 2, 32)
+            sees = torch.arange(40 - n, 40) >= near
+            assert torch.isfinite(out[:, 0]).all() and out[:, 1].isnan().all(1).cpu().tolist() == sees.tolist()
+
+
 def test_rel_attention_table_types_scale_and_wide_radius():
     attention_case(torch.bfloat16, 1, 80, 80, 2, 2, 64, True, table_dt=torch.float32, scale=0.3)
     attention_case(torch.float32, 1, 40, 1300, 1, 1, 16, False, radius=1024, nb=64, seed=4)
