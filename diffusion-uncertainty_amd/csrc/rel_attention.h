@@ -316,7 +316,7 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- host
-[[maybe_unused]] static int check_common(const dua_rel_attention_args* a, const char* who) {
+[[maybe_unused]] static int check_common(const dua_rel_attention_args* a, const char* who, bool backward) {
     DUA_REQUIRE(a, "%s: null arguments", who);
     DUA_REQUIRE(dua_dtype_ok(a->dtype) && dua_dtype_ok(a->table_dtype) && (a->table_dtype == DUA_DTYPE_F32 || a->table_dtype == a->dtype),
                 "%s: dtype must be fp32, bf16 or fp16 and the table's fp32 or the same", who);
@@ -329,7 +329,9 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
         DUA_REQUIRE(r >= 0 && r < (1L << 24), "%s: row strides must be in [0, 2^24) elements", who);
     DUA_REQUIRE(a->table && a->bucket_map, "%s: null table / bucket map", who);
     DUA_REQUIRE((a->B == 0 || a->Tq == 0 || a->q) && (a->B == 0 || a->Tk == 0 || (a->k && a->v)), "%s: null operand", who);
-    DUA_REQUIRE((long)a->B * a->heads * ((a->Tq > a->Tk ? a->Tq : a->Tk) / 64 + 1) < (1L << 23), "%s: too many blocks for one launch", who);
+    // workgroups of a launch: at most one for 64 queries of a head, in the backward pass for 64 keys too (the factors one by one: no overflow)
+    const long heads = (long)a->B * a->heads, blocks = (backward && a->Tk > a->Tq ? a->Tk : a->Tq) / 64 + 1;
+    DUA_REQUIRE(heads < (1L << 23) && heads * blocks < (1L << 23), "%s: too many blocks for one launch", who);
     return DUA_OK;
 }
 

@@ -371,7 +371,7 @@ template <typename T, int CHP> struct Fwd {
 }  // namespace
 
 extern "C" size_t dua_rel_attention_workspace_bytes(const dua_rel_attention_args* a, int backward) {
-    if (!a || check_common(a, "dua_rel_attention_workspace_bytes")) return 0;
+    if (!a || check_common(a, "dua_rel_attention_workspace_bytes", backward != 0)) return 0;
     const size_t rows = (size_t)a->B * a->heads * a->Tq;
     if (backward) return rel_attention_bwd_bytes(a);
     if (rows == 0) return 0;
@@ -380,7 +380,7 @@ extern "C" size_t dua_rel_attention_workspace_bytes(const dua_rel_attention_args
 }
 
 extern "C" int dua_rel_attention(const dua_rel_attention_args* a, void* stream) {
-    if (int rc = check_common(a, "dua_rel_attention")) return rc;
+    if (int rc = check_common(a, "dua_rel_attention", false)) return rc;
     if (a->B == 0 || a->Tq == 0) return DUA_OK;
     DUA_REQUIRE(a->out, "dua_rel_attention: null output");
     const Plan pl = plan(a);

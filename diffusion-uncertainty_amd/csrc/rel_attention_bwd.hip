@@ -516,7 +516,7 @@ template <typename T, int CHP> struct Bwd {
 }  // namespace
 
 extern "C" int dua_rel_attention_bwd(const dua_rel_attention_args* a, void* stream) {
-    if (int rc = check_common(a, "dua_rel_attention_bwd")) return rc;
+    if (int rc = check_common(a, "dua_rel_attention_bwd", true)) return rc;
     DUA_REQUIRE(a->dtable, "dua_rel_attention_bwd: null dtable");
     DUA_REQUIRE(a->B == 0 || a->Tq == 0 || (a->out && a->lse && a->dout && a->dq), "dua_rel_attention_bwd: null operand");
     DUA_REQUIRE(a->B == 0 || a->Tk == 0 || (a->dk && a->dv), "dua_rel_attention_bwd: null output");

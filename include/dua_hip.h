@@ -638,7 +638,8 @@ int dua_sandwich_norm_bwd(const dua_sandwich_norm_args* args_host, void* stream)
  * behind the last query are not read; a table value below -1e30 masks its distances, other finite ones are taken as between -65504 and 65504.  q, out [B][Tq][heads * ch], k, v [B][Tk][kv_heads * ch] with strides
  * of their own (elements); query head h reads kv head h / (heads / kv_heads);
  * ch <= 128, a multiple of 8 (fp32: 4); row strides below 2^24.  table [num_buckets][heads] (table_dtype: fp32 or
- * dtype), bucket_map [2 radius + 1]: entries outside [0, num_buckets) add no bias; radius <= 1024.  Tq = 1 is decoding. */
+ * dtype), bucket_map [2 radius + 1]: entries outside [0, num_buckets) add no bias; radius <= 1024.  Tq = 1 is decoding.
+ * B * heads * (Tq / 64 + 1), in the backward pass with the larger of Tq and Tk, stays below 2^23. */
 typedef struct {
     const void *q, *k, *v;
     int dtype, B, Tq, Tk, heads, kv_heads, ch;

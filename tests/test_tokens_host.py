@@ -113,3 +113,22 @@ def test_argument_validation_without_gpu():
     refuses(L.dua_token_logprobs_bwd, lp(dtop=None), "null operand")
     refuses(L.dua_token_logprobs_bwd, lp(dlogits=P, ldd=128), "in place")
     assert L.dua_token_logprobs(ctypes.byref(lp(rows=0, logits=None)), None) == 0
+
+
+def test_rel_attention_block_count():
+    """B * heads * blocks of 64 rows stay below 2^23 whatever the factors (their product may pass 2^64), and the forward pass counts queries alone: a
+    long cache is no reason to refuse a decoding step."""
+    from diffusion_uncertainty_amd import _lib
+    L = _lib.lib()
+    P = 4096
+    att = lambda **kw: _lib.RelAttentionArgs(**{**dict(q=P, k=P, v=P, B=1, Tq=4, Tk=4, heads=2, kv_heads=1, ch=32, table=P, bucket_map=P, radius=16, num_buckets=8,
+                                                       scale=1.0, out=P, lse=P, dout=P, dq=P, dk=P, dv=P, dtable=P), **kw})
+    T = (1 << 25) - 64
+    for kw in (dict(B=1 << 30, heads=1 << 15, kv_heads=1 << 15, Tq=T, Tk=T), dict(B=1 << 23), dict(B=(1 << 31) - 1, heads=65535, kv_heads=1)):
+        for fn in (L.dua_rel_attention, L.dua_rel_attention_bwd):
+            assert fn(ctypes.byref(att(**kw)), None) == -1 and "blocks" in L.dua_last_error().decode(), L.dua_last_error()
+        assert L.dua_rel_attention_workspace_bytes(ctypes.byref(att(**kw)), 0) == 0
+    cache = att(B=8, Tq=1, Tk=600000, heads=128, kv_heads=8, ch=128, dtype=1)
+    assert L.dua_rel_attention_workspace_bytes(ctypes.byref(cache), 0) > 0                       # split keys
+    assert L.dua_rel_attention_workspace_bytes(ctypes.byref(cache), 1) == 0
+    assert L.dua_rel_attention_bwd(ctypes.byref(cache), None) == -1 and "blocks" in L.dua_last_error().decode()
