@@ -633,7 +633,8 @@ extern "C" int dua_sandwich_norm_bwd(const dua_sandwich_norm_args* a, void* stre
     const Deal d = deal_bwd(a);
     DUA_REQUIRE(a->rows == 0 || (a->workspace && a->workspace_bytes >= dua_sandwich_norm_bwd_workspace_bytes(a)),
                 "dua_sandwich_norm_bwd: workspace smaller than dua_sandwich_norm_bwd_workspace_bytes");
-    DUA_REQUIRE(!a->gate || a->gate_rows <= 65000 || d.per_sample == 0, "dua_sandwich_norm_bwd: more than 65000 gate rows of many rows each");
+    // (k_sandwich_cols' grid; with rows there are at most as many gate rows with sums of their own as units on the chip)
+    DUA_REQUIRE(!a->gate || a->gate_rows <= 65000 || d.per_sample == 0, "dua_sandwich_norm_bwd: an empty call's gate has at most 65000 rows");
     NormP p = pack(a);
     p.units = d.units;
     p.per_sample = d.per_sample;

@@ -1271,8 +1271,10 @@ def _sandwich_args(x, y, post, post_w, post_b, gate, res_scale, pre, pre_w, pre_
         if gate.shape[-1:] != (D,):
             raise ValueError(f"gate: expected [D] or [rows, D] with D = {D}, got {tuple(gate.shape)}")
         gate_rows = gate.numel() // D
-        if gate_rows < 1 or rows % gate_rows:
+        if rows % gate_rows if gate_rows else rows:
             raise ValueError(f"gate: its {gate_rows} rows must divide the {rows} rows of x")
+        if not gate_rows:
+            gate = None                                       # (an empty batch of gated samples)
     return SandwichNormArgs(x.data_ptr(), y.data_ptr(), _DTYPES[dt], _DTYPES[pt], rows, D, _NORMS[post], _NORMS[pre], _a(post_w), _a(post_b),
                             _a(pre_w), _a(pre_b), _a(gate), gate_rows, res_scale, eps)
 

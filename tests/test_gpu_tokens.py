@@ -531,6 +531,18 @@ def test_sandwich_norm_in_place_and_empty():
     assert torch.equal(x, r) and torch.equal(y, z)
 
 
+def test_sandwich_norm_empty_batch_with_a_gate_for_each_sample():
+    """No samples, no gate rows: nothing to do, zeros for the parameters' gradients."""
+    from diffusion_uncertainty_amd import ops
+    x, gate, w = torch.zeros(0, 7, 64, device=dev), torch.zeros(0, 64, device=dev), torch.ones(64, device=dev)
+    r, z, st = ops.sandwich_norm(x, x, post_w=w, pre_w=w, gate=gate, want_stats=True)
+    assert r.shape == z.shape == (0, 7, 64) and st.shape == (0, 4)
+    g = ops.sandwich_norm_bwd(x, x, st, x, x, post_w=w, pre_w=w, gate=gate)
+    assert g.dx.shape == (0, 7, 64) and g.dgate.shape == (0, 64) and (g.dpost_w == 0).all() and (g.dpre_w == 0).all()
+    with pytest.raises(ValueError):
+        ops.sandwich_norm(torch.zeros(2, 64, device=dev), torch.zeros(2, 64, device=dev), gate=gate)
+
+
 # --------------------------------------------------------------------------------------------------------- token logprobs
 def logprob_case(x, ids, k, t=1.0, grads=True, seed=0):
     """x [rows, V] on the CPU in its type.  A row's sums: chains of V / 256 / parts groups of up to 8 and trees of depth 14; each exponential is good
