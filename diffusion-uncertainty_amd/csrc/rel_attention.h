@@ -361,9 +361,10 @@ __device__ __forceinline__ float max_of(const f32x4* s) {
 
 // dk / dv where the blocks of keys alone do not fill the chip: a group's query heads are dealt to `heads` workgroups, and of single heads the tiles of
 // queries to `tiles`; their sums (fp32) are added in order afterwards.  2 x 8 kv heads of 4 query heads, 940 tokens of 16 bf16, forward and backward: 344 us
-// with one workgroup a block of keys (128 in all), 180 with four.  Shares of the queries, backward: 1 x 8 heads, 1024 tokens of 64
-// fp32 (128 workgroups) 207 -> 154 us, 2 heads, 2048 tokens of 128 bf16 (64) 190 -> 133, 2 x 12 heads, 1024 tokens of 72 fp32 (384) 392 -> 338; 4 x 8 heads,
-// 1024 tokens of 64 bf16 (256) 106 -> 109: the sums' way through memory is all that is left there.
+// with one workgroup a block of keys (128 in all), 180 with four.  Shares of the queries, backward, 64 wide, 8 heads of 1024 tokens
+// a sequence: fp32 (three workgroups a CU) 1 / 2 / 3 sequences (128 / 256 / 384 workgroups) 205 / 208 / 313 us without, 149 / 192 / 273 with 4 / 2 / 2
+// shares; bf16 (two workgroups a CU) 64 / 128 workgroups 98 / 101 without, 78 / 88 with 8 / 4 shares; 192 / 256: 101 / 103 and 102 / 104 (256 of 4096
+// tokens: 285 and 243) with 2.  Past 512 workgroups they lose: 192 in 3 shares 111, 320 / 384 / 448 in 2 142 / 157 / 167 us, 132 / 132 / 133 without.
 struct KeySplits { int heads, tiles; };
 [[maybe_unused]] static KeySplits key_splits(const dua_rel_attention_args* a) {
     const int rep = a->heads / a->kv_heads, nkb = (a->Tk + key_block(a->dtype, a->ch) - 1) / key_block(a->dtype, a->ch);
@@ -373,7 +374,7 @@ struct KeySplits { int heads, tiles; };
         if (rep % d == 0) s.heads = d;
     const long now = wgs * s.heads, tiles = a->Tq / (a->dtype == DUA_DTYPE_F32 ? 64 : 128);        // two of Shape::KT
     if (s.heads == rep && now > 0 && now < 512) {
-        const long t = (512 + now - 1) / now;
+        const long t = a->dtype == DUA_DTYPE_F32 ? (512 + now - 1) / now : 512 / now;
         s.tiles = (int)(t < tiles ? t : (tiles > 1 ? tiles : 1));
     }
     return s;

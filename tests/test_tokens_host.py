@@ -132,3 +132,22 @@ def test_rel_attention_block_count():
     assert L.dua_rel_attention_workspace_bytes(ctypes.byref(cache), 0) > 0                       # split keys
     assert L.dua_rel_attention_workspace_bytes(ctypes.byref(cache), 1) == 0
     assert L.dua_rel_attention_bwd(ctypes.byref(cache), None) == -1 and "blocks" in L.dua_last_error().decode()
+
+
+def test_rel_attention_shares_of_the_queries_fill_the_chip_once():
+    """Backward, one query head a kv head: a share of the queries costs fp32 sums of dk and dv in the workspace.  Sixteen-bit types take as many whole shares as
+    512 workgroups have room for (none at 320), fp32 one more where that leaves places empty."""
+    from diffusion_uncertainty_amd import _lib
+    L = _lib.lib()
+    P = 4096
+
+    def shares(dtype, B, T=1024, H=8, ch=64):
+        a = _lib.RelAttentionArgs(q=P, k=P, v=P, dtype=dtype, B=B, Tq=T, Tk=T, heads=H, kv_heads=H, ch=ch, table=P, table_dtype=dtype, bucket_map=P, radius=1,
+                                  num_buckets=2, scale=1.0, out=P, lse=P, dout=P, dq=P, dk=P, dv=P, dtable=P)
+        n = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 1)
+        one = 2 * B * T * H * ch * 4                                                 # dk and dv of a share
+        return n // one
+
+    assert [shares(1, B) for B in (1, 2, 3, 4, 5, 6, 7, 8)] == [8, 4, 2, 2, 0, 0, 0, 0]
+    assert [shares(2, B) for B in (3, 5)] == [2, 0]
+    assert [shares(0, B) for B in (1, 2, 3, 4)] == [4, 2, 2, 0]
