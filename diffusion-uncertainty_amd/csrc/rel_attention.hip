@@ -338,14 +338,23 @@ __global__ __launch_bounds__(NTHR) void k_rel_attention_join(AttP p) {
 
 // How the forward pass splits the keys: a few queries a kv head go to k_rel_attention_few; too few workgroups for the 256 CUs share a row's
 // keys - about 512 workgroups of at least 128 keys (few queries) or 256 (tiles of queries).  Few queries, 2 x 30001 keys of 4 heads of 128: 30 us with
-// 512, 35 with 1024 workgroups; 4 x 2000 keys of 16 heads of 72 in fp32: 23 and 28 us.
+// 512, 35 with 1024 workgroups; 4 x 2000 keys of 16 heads of 72 in fp32: 23 and 28 us.  Tiles of queries, bf16, whole and split: 8 workgroups of 2000 keys
+// 44 and 20 us, 64 of 4096 (64 wide) 80 and 38, of 1024 27 and 26.  More workgroups than 64 fill enough of the chip that the sums' way through memory costs
+// more than the rest of it gives, but for long rows: 128 of 1024 keys 28 and 40 us, 192 28 and 51, 216 of 2048 47 and 61; 128 of 4096 79 and 51, 160 (128 wide)
+// 116 and 88, 192 of 8192 152 and 132 - in as many whole shares as 512 workgroups hold (160 in four instead of three: 100).  fp32, slower a key and three workgroups
+// a CU: 128 of 1024 58 and 42, 240 of 2048 111 and 103, 240 of 4096 211 and 173.
 struct Plan { bool few; int splits; };
 Plan plan(const dua_rel_attention_args* a) {
     const long rep = a->heads / a->kv_heads, units = (long)a->B * a->kv_heads;
     Plan pl{rep * a->Tq <= 16, 1};
     const long wgs = pl.few ? units : units * rep * ((a->Tq + query_block(a->dtype) - 1) / query_block(a->dtype));
-    const long want = pl.few ? (512 + wgs - 1) / wgs : (wgs < 256 ? (512 + wgs - 1) / wgs : 1), most = a->Tk / (pl.few ? 128 : 256);
-    long s = want < most ? want : most;
+    const long up = (512 + wgs - 1) / wgs, most = a->Tk / (pl.few ? 128 : 256);
+    long s = up;
+    if (!pl.few) {
+        if (wgs >= 256) s = 1;
+        else if (a->dtype != DUA_DTYPE_F32 && wgs > 64) s = a->Tk >= 4096 ? 512 / wgs : 1;
+    }
+    if (s > most) s = most;
     s = s < 1 ? 1 : (s > SMAX ? SMAX : s);
     pl.splits = (int)s;
     return pl;

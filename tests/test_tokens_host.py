@@ -151,3 +151,23 @@ def test_rel_attention_shares_of_the_queries_fill_the_chip_once():
     assert [shares(1, B) for B in (1, 2, 3, 4, 5, 6, 7, 8)] == [8, 4, 2, 2, 0, 0, 0, 0]
     assert [shares(2, B) for B in (3, 5)] == [2, 0]
     assert [shares(0, B) for B in (1, 2, 3, 4)] == [4, 2, 2, 0]
+
+
+def test_rel_attention_splits_keys_where_the_chip_is_empty():
+    """Forward, tiles of queries: the number of shares of the keys by the workspace they take (ch sums, a maximum and a sum a row and share)."""
+    from diffusion_uncertainty_amd import _lib
+    L = _lib.lib()
+    P = 4096
+
+    def shares(dtype, B, Tq, Tk, H=8, ch=64):
+        a = _lib.RelAttentionArgs(q=P, k=P, v=P, dtype=dtype, B=B, Tq=Tq, Tk=Tk, heads=H, kv_heads=H, ch=ch, table=P, table_dtype=dtype, bucket_map=P, radius=1,
+                                  num_buckets=2, scale=1.0, out=P)
+        n = L.dua_rel_attention_workspace_bytes(ctypes.byref(a), 0)
+        one = B * H * Tq * (ch + 2) * 4
+        assert n % one == 0
+        return n // one                                                              # 0: none
+
+    assert [shares(1, 1, 128, 2000), shares(1, 1, 1024, 1024), shares(1, 1, 1024, 4096)] == [7, 4, 8]
+    assert [shares(1, 2, 1024, 1024), shares(2, 3, 1024, 1024), shares(1, 3, 1024, 2048)] == [0, 0, 0]
+    assert [shares(1, 2, 1024, 4096), shares(2, 3, 1024, 4096), shares(1, 4, 1024, 4096)] == [4, 2, 0]
+    assert [shares(0, 1, 1024, 1024), shares(0, 1, 1920, 2048), shares(0, 2, 1024, 1024)] == [4, 3, 0]
