@@ -520,10 +520,14 @@ int check_common(const dua_token_logprobs_args* a, const char* who) {
     return DUA_OK;
 }
 
-// Parts of a row: enough workgroups for the chip, at least 4096 elements (more than k) each.
-int plan_splits(long rows, long V) {
-    if (rows >= 256 || rows == 0) return 1;
-    long s = (512 + rows - 1) / rows, most = V / 4096;
+// Parts of a row: enough workgroups for the chip, at least 4096 elements (more than k) each.  Rows from 192 KB on are dealt up to 512 rows, where a workgroup a
+// row still leaves CUs waiting for the last ones: 256 / 384 / 512 rows of 128000 bf16 27 / 38 / 39 us whole, 21 / 29 / 33 in 4 / 3 / 2 parts, of 65536 fp32
+// (384) 29 and 26; 600 rows of 128000 fp32 60 and 61.  Shorter rows only below 256 (256 / 512 rows of 65536 bf16 18 / 18 us whole, 20 / 21 in parts).
+int plan_splits(long rows, long V, int dtype) {
+    const bool big = V * (long)dua_dtype_size(dtype) >= 192 * 1024;
+    if (rows == 0 || rows > (big ? 512 : 255)) return 1;
+    const long want = rows < 256 ? 512 : 1024;
+    long s = (want + rows - 1) / rows, most = V / 4096;
     if (s > most) s = most;
     if (s > SMAX) s = SMAX;
     return s < 1 ? 1 : (int)s;
@@ -539,7 +543,7 @@ LogpP pack(const dua_token_logprobs_args* a) {
 
 extern "C" size_t dua_token_logprobs_workspace_bytes(const dua_token_logprobs_args* a) {
     if (!a || a->rows < 0 || a->V < 1 || a->k < 0) return 0;
-    const int s = plan_splits(a->rows, a->V);
+    const int s = plan_splits(a->rows, a->V, a->dtype);
     return s > 1 ? (size_t)a->rows * s * (4 + 2 * a->k) * sizeof(float) : 0;
 }
 
@@ -548,7 +552,7 @@ extern "C" int dua_token_logprobs(const dua_token_logprobs_args* a, void* stream
     if (a->rows == 0) return DUA_OK;
     DUA_REQUIRE(a->logprob && a->entropy && a->lse && (a->k == 0 || (a->top_ids && a->top_logprobs)), "dua_token_logprobs: null output");
     LogpP p = pack(a);
-    p.splits = plan_splits(a->rows, a->V);
+    p.splits = plan_splits(a->rows, a->V, a->dtype);
     p.part = (float*)a->workspace;
     DUA_REQUIRE(p.splits == 1 || (a->workspace && a->workspace_bytes >= dua_token_logprobs_workspace_bytes(a)),
                 "dua_token_logprobs: workspace smaller than dua_token_logprobs_workspace_bytes");

@@ -675,6 +675,28 @@ def test_token_logprobs_long_rows_in_parts(dt):
         logprob_case(z, torch.tensor([5, 6, 10]), 5)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+def test_token_logprobs_many_long_rows_in_parts(dt):
+    """More than 255 rows of 192 KB and beyond, cut into parts: equal rows give equal bits."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(13)
+    V = 100003 if dt != torch.float32 else 50003
+    base = rnd(g, 8, V, scale=2.0, dtype=dt)
+    base[1, 40000:] = -math.inf
+    ids = torch.randint(0, 40000, (8,), generator=g)
+    logprob_case(base, ids, 8, grads=False)
+    few = ops.token_logprobs(base.to(dev), ids.to(dev), k=8)
+    r = torch.arange(260) % 8
+    many = ops.token_logprobs(base.to(dev)[r.to(dev)], ids[r].to(dev), k=8)
+    lp, ent, lse, top, tlp, l = oracle.token_logprobs(base.double(), ids, 8, 1.0)
+    assert torch.equal(many.top_ids.cpu(), top[r])
+    for a, b in ((many.logprob, lp), (many.entropy, ent), (many.lse, lse)):
+        assert torch.equal(a.cpu()[:8].repeat(33)[:260], a.cpu()), "equal rows, equal bits"
+        # two orders of a sum of V / 1024 terms a thread and trees: V / 256 + 30 half steps, 4 for each unit of the largest logit that counts (40)
+        close(a, b[r], (V / 256 + 30 + 160) * U * (2 + 2 * b[r].abs()), "many")
+    assert (many.logprob - few.logprob[r.to(dev)]).abs().max() < 1e-4
+
+
 def test_token_logprobs_views_and_partial_gradients():
     """A slice of a padded vocabulary (row stride > V, rows not 16-byte aligned), leading dimensions, missing gradients, no ids, repeated ids."""
     from diffusion_uncertainty_amd import ops

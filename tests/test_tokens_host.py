@@ -171,3 +171,18 @@ def test_rel_attention_splits_keys_where_the_chip_is_empty():
     assert [shares(1, 2, 1024, 1024), shares(2, 3, 1024, 1024), shares(1, 3, 1024, 2048)] == [0, 0, 0]
     assert [shares(1, 2, 1024, 4096), shares(2, 3, 1024, 4096), shares(1, 4, 1024, 4096)] == [4, 2, 0]
     assert [shares(0, 1, 1024, 1024), shares(0, 1, 1920, 2048), shares(0, 2, 1024, 1024)] == [4, 3, 0]
+
+
+def test_token_logprobs_parts_have_no_cliff():
+    """Long rows are dealt in parts up to 512 of them, short ones below 256: the number of parts by the workspace (4 sums and k pairs each)."""
+    from diffusion_uncertainty_amd import _lib
+    L = _lib.lib()
+
+    def parts(rows, V, dtype, k=5):
+        a = _lib.TokenLogprobsArgs(rows=rows, V=V, ld=V, k=k, dtype=dtype, inv_temperature=1.0)
+        return L.dua_token_logprobs_workspace_bytes(ctypes.byref(a)) // (rows * (4 + 2 * k) * 4)
+
+    assert [parts(r, 128000, 1) for r in (4, 255, 256, 384, 512, 513)] == [31, 3, 4, 3, 2, 0]
+    assert [parts(r, 65536, 0) for r in (255, 256, 512)] == [3, 4, 2]
+    assert [parts(r, 65536, 2) for r in (255, 256, 512)] == [3, 0, 0]
+    assert parts(4, 8191, 0) == 0 and parts(4, 8192, 0) == 2
