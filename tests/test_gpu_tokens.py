@@ -332,6 +332,106 @@ def test_rel_attention_gradient_against_differences():
         assert abs(diff - have) < 1e-5 * size + 1e-6, (n, diff, have)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,Hk", [(2, 4), (13, 5)])
+def test_rel_attention_kv_heads_on_eight_dies(dt, B, Hk):
+    """8 and 65 kv heads: their blocks are dealt to the eight XCDs, the last round of 65 partly filled."""
+    attention_case(dt, B, 40, 70, 2 * Hk, Hk, 16, True, qstart=[30 - b for b in range(B)], seed=16)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_rel_attention_joins_of_more_than_64_splits(dt):
+    """One head over 20000 keys: 128 splits (one query), 78 (a tile of queries); two wavefronts hold the splits' weights."""
+    attention_case(dt, 1, 1, 20000, 1, 1, 16, True, klen=[19990], qstart=[19989], seed=17, grads=False)
+    attention_case(dt, 1, 40, 20000, 1, 1, 16, False, klen=[19990], qstart=[10000], seed=18)
+
+
+FORMS = [(70, 150), (3, 100), (1, 3000), (40, 1500)]                   # tiles of queries, few queries, and both with split keys
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Tq,Tk", FORMS)
+def test_rel_attention_keeps_what_the_outputs_rounding_left(dt, Tq, Tk):
+    """Equal keys and no bias: every P is 1 and rounds to itself, so out + out_lo is the mean of the values (3 + a normal number) but for fp32's roundings -
+    a logit's in P and in their sum, 32 in an instruction and one for every 16 keys in the sums - and out_lo's own (e^2; fp16: half a subnormal step)."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(51)
+    H, ch, e = 2, 64, half_step(dt)
+    q, v = rnd(g, 1, Tq, H * ch, dtype=dt, scale=0.1), (3.0 + rnd(g, 1, Tk, H * ch)).to(dt)
+    k = rnd(g, 1, 1, H * ch, dtype=dt).repeat(1, Tk, 1)
+    bk = ops.RelativeBuckets(8, 16, True, device=dev)
+    out, s = ops.rel_attention(q.to(dev), k.to(dev), v.to(dev), torch.zeros(8, H, device=dev), bk, heads=H, want_lse=True)
+    r = oracle.rel_attention(q, k, v, torch.zeros(8, H), bk.map.cpu(), H, H)
+    tol = r["pv"] * 2 * ((ch + 8) * r["logit"].max() + 8 + 40 + Tk / 16) * U + e * e * r["out"].abs() + (2.0 ** -25 if dt == torch.float16 else 0.0)
+    lo = s.out_lo.permute(0, 2, 1, 3).reshape(1, Tq, H * ch)
+    close(out.double() + lo.double(), r["out"], tol, "out + out_lo")
+    bare = (r["out"].to(dt).double() - r["out"]).abs()
+    assert (bare > 4 * tol).any(), "the bound would not tell out from out + out_lo"
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Tq,Tk", FORMS)
+def test_rel_attention_gradients_of_decided_queries(dt, Tq, Tk):
+    """Queries that all find two equal keys whose values are a step or two of their type apart: the output lies between two numbers, dS = P (dP - D) is the
+    small difference of large terms, and D = dO . o has to be better than the rounded output.
+
+    Bounds, one query: dS is off by its own rounding e |dS| and by P times (dP's and D's chains of ch products, (ch + 4) u each of |dO| . |v| and |dO| . |o|;
+    what out_lo's rounding leaves of D, e^2 |dO| . |o| and in fp16 2^-25 |dO|; the forward's rounding of the other keys' P, e |dO| . sum P |v|; P's own
+    relative error w times |dP - D|).  dk and the table take D corrected by the row's sum of dS: what is left of the output's errors drops out, with
+    out_lo or without; the table takes dS unrounded."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(52)
+    H, ch, e, F = 8, 16, half_step(dt), torch.float64
+    q, k = rnd(g, 1, Tq, H, ch, scale=0.3), rnd(g, 1, Tk, H, ch, scale=0.3)
+    best = Tk // 3
+    q[..., 0], k[..., 0], k[:, best, :, 0] = 8.0, 0.0, 8.0
+    k[:, best + 1] = k[:, best]
+    v, do = rnd(g, 1, Tk, H * ch, dtype=dt), rnd(g, 1, Tq, H * ch, dtype=dt)
+    v[:, best + 1] = (v[:, best].float() * (1 + 2 * e)).to(dt)
+    q, k = q.to(dt).view(1, Tq, H * ch), k.to(dt).view(1, Tk, H * ch)
+    m = ops.RelativeBuckets(8, 16, True, device="cpu").map
+    qs, scale = Tk // 2, 0.25
+    cell = m.long()[(torch.arange(Tk)[None] - (torch.arange(Tq)[:, None] + qs)).clamp(-16, 16) + 16].reshape(-1)
+    table = lambda t: torch.zeros(8, dtype=F).index_add_(0, cell, t.reshape(-1))
+    want, tol, seen = {n: [] for n in ("dq", "dk", "dtable")}, {n: [] for n in ("dq", "dk", "dtable")}, []
+    for h in range(H):
+        Q, K, V, G = (t[0].view(-1, H, ch)[:, h].to(F) for t in (q, k, v, do))
+        P = torch.softmax(scale * Q @ K.T, 1)
+        others = P * ((torch.arange(Tk) != best) & (torch.arange(Tk) != best + 1))
+        assert others.sum(1).max() < 2.0 ** -8                                        # (the two keys' own P are 1 before they are normalised)
+        O, dP = P @ V, G @ V.T
+        dP_D = dP - (G * O).sum(1, keepdim=True)
+        dS = P * dP_D
+        w = 2 * ((ch + 8) * (scale * Q.abs() @ K.abs().T * (P > 1e-12)).max() + 8) * U + (Tk + 8) * U
+        GO = (G.abs() * O.abs()).sum(1, keepdim=True)
+        chains = (ch + 4) * U * (G.abs() @ V.abs().T + GO) + w * dP_D.abs()
+        rest = e * e * GO + (2.0 ** -25 if dt == torch.float16 else 0.0) * G.abs().sum(1, keepdim=True) + e * (G.abs() * (others @ V.abs())).sum(1, keepdim=True)
+        far = 2.0 ** -32 * dS.abs().max() if dt == torch.float16 else 0.0              # fp16 operands far below their column's largest
+        err_q, err_k = e * dS.abs() + P * (chains + rest) + far, e * dS.abs() + P * chains + far
+        want["dq"].append(scale * dS @ K)
+        want["dk"].append(scale * dS.T @ Q)
+        want["dtable"].append(table(dS))
+        tol["dq"].append(e * want["dq"][h].abs() + scale * (err_q + (Tk + 8) * U * dS.abs()) @ K.abs())
+        tol["dk"].append(e * want["dk"][h].abs() + scale * (err_k + (Tq + 8) * U * dS.abs()).T @ Q.abs())
+        tol["dtable"].append(U * want["dtable"][h].abs() + table(P * chains + (600 + Tq + Tk) * U * dS.abs()) + 1e-30)
+        # what a D of the rounded output alone would do to dq and, uncorrected, to the table
+        off = (G * (O.to(dt).to(F) - O)).sum(1, keepdim=True)
+        seen.append([bool((scale * off * (P @ K)).abs().gt(4 * tol["dq"][h]).any()), bool(table(off * P).abs().gt(4 * tol["dtable"][h]).any())])
+        if dt == torch.float16:
+            tol["dq"][h], tol["dk"][h] = tol["dq"][h] + 2.0 ** -25, tol["dk"][h] + 2.0 ** -25
+    assert all(any(x) for x in zip(*seen)), "the bounds would not tell"
+    want, tol = ({n: torch.stack(t, -1 if n == "dtable" else 1) for n, t in d.items()} for d in (want, tol))
+    bk = ops.RelativeBuckets.from_map(m.to(dev), 8)
+    kw = dict(heads=H, scale=scale, qstart=torch.full((1,), qs, dtype=torch.int32, device=dev))
+    a = (q.to(dev), k.to(dev), v.to(dev), torch.zeros(8, H, device=dev), bk)
+    out, s = ops.rel_attention(*a, want_lse=True, **kw)
+    for saved, names in ((s, ("dq", "dk", "dtable")), (s._replace(out_lo=None), ("dk", "dtable"))):
+        got = dict(zip(("dq", "dk", "dv", "dtable"), ops.rel_attention_bwd(*a, out, saved, do.to(dev), **kw)))
+        for n in names:
+            close(got[n].double().view(want[n].shape), want[n], tol[n], n)
+    assert ((got["dq"].cpu().double().view(want["dq"].shape) - want["dq"]).abs() > 2 * tol["dq"]).any(), "dq without out_lo"
+
+
 def fp16_gradient_case(q, k, v, table, bk, do, H, Hk, scale, causal=False, qstart=None):
     """Gradients in fp16 against 64 bits where nothing but the operands' rounding is allowed for: every dS and P counts relative to the largest one that goes
     into the same sum, whatever the size of dO.
