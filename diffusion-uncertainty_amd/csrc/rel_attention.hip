@@ -161,6 +161,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
 // Few queries (a kv head's query heads times Tq at most 16 - decoding): they are the 16 columns of one tile, so the group's heads share one
 // read of the keys and values.  Bound by that read: the waves split the keys, key fragments go from memory straight to the matrix unit, values
 // through the wave's own LDS tile to be read transposed; workgroups split the keys further and k_rel_attention_join adds up.
+// The matrix unit waits for memory here, so P goes into its product with v twice, rounded and what the rounding left: the output is off by its own rounding
+// alone (bf16 1.66e-3 of its size against 2.3e-3, fp16 2.1e-4 against 2.9e-4; 48.1 -> 48.4 and 26.5 -> 27.0 us in the first two examples).
 // 32 sequences of 4096 keys, 4 kv heads of 128 bf16: 48 us, 5.6 TB/s; 2 of 30001 fp16: 25 + 4 us, 4.2 TB/s; 8 of 1000, 16 heads of 64: 11 + 4 us, where
 // the launches and the dependent loads of three tiles count.
 template <typename T, int CHP>
@@ -262,8 +264,17 @@ __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(At
 #pragma unroll
         for (int kb = 0; kb < N16; kb += S::NP) {
             const frag pf = acc_frag<T>(&s[kb]);
+            frag pl;                                                        // P as two numbers of the tensors' type
+            if constexpr (!S::F32) {
+                const f32x4 lo[2] = {rest4<T>(s[kb]), rest4<T>(s[kb + 1])};
+                pl = acc_frag<T>(lo);
+            }
 #pragma unroll
-            for (int c = 0; c < CT; ++c) o[c] = mma(col_frag<T>(Vt, P, 16 * kb, 16 * c, lane), pf, o[c]);
+            for (int c = 0; c < CT; ++c) {
+                const frag x = col_frag<T>(Vt, P, 16 * kb, 16 * c, lane);
+                o[c] = mma(x, pf, o[c]);
+                if constexpr (!S::F32) o[c] = mma(x, pl, o[c]);
+            }
         }
     }
     l = col_sum(l);

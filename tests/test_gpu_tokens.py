@@ -153,6 +153,25 @@ def test_rel_attention_unwritten_slots_behind_the_last_query(dt):
             assert torch.isfinite(a).all() and torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Tq,Tk,H,Hk,ch", [(1, 1000, 4, 4, 64), (1, 3000, 16, 2, 128), (4, 333, 4, 1, 72), (2, 90, 2, 1, 40)])
+def test_rel_attention_few_queries_are_off_by_their_own_rounding(dt, Tq, Tk, H, Hk, ch):
+    """Decoding: P is not rounded to the tensors' type but to two numbers of it (e^2; fp16: half a subnormal step of the second, beside a largest P of at least
+    1), so nothing of e is left but the output's own rounding."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(19)
+    e = half_step(dt)
+    q, k, v = rnd(g, 3, Tq, H * ch, dtype=dt), rnd(g, 3, Tk, Hk * ch, dtype=dt), rnd(g, 3, Tk, Hk * ch, dtype=dt)
+    table, bk = rnd(g, 8, H, dtype=dt), ops.RelativeBuckets(8, 16, True, device=dev)
+    n = torch.tensor([Tk, Tk - 7, Tk // 2], dtype=torch.int32)
+    r = oracle.rel_attention(q, k, v, table, bk.map.cpu(), H, Hk, True, None, n, n - Tq)
+    out = ops.rel_attention(q.to(dev), k.to(dev), v.to(dev), table.to(dev), bk, heads=H, kv_heads=Hk, causal=True, klen=n.to(dev), qstart=(n - Tq).to(dev))
+    dp = 2 * ((ch + 8) * r["logit"] + 8) * U + (Tk + 8) * U
+    rows = dp.permute(0, 2, 1).repeat_interleave(ch, 2)
+    sub = 2.0 ** -25 * Tk * v.abs().max().double() if dt == torch.float16 else 0.0
+    close(out, r["out"], r["pv"] * (rows + e * e + Tk * U) + e * r["out"].abs() + sub, "out")
+
+
 def test_rel_attention_table_of_the_lowest_value():
     from diffusion_uncertainty_amd import ops
     g = torch.Generator().manual_seed(4)
