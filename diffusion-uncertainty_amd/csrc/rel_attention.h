@@ -4,7 +4,11 @@
 //   dS = P (dO v^T - D), D_i = sum_c dO_ic o_ic;  dq = scale dS k;  dk = scale dS^T q;  dv = P^T dO;  dtable[n][h] = sum of dS where map = n
 // The bias is never materialised: a head's 2R + 1 values lie in LDS (padded so that a tile near the diagonal indexes them without a clamp), and a
 // tile farther than R from the diagonal sees one value.  All products run on 16x16 matrix instructions (K = 32 for sixteen-bit elements, four
-// K = 4 steps for fp32), softmax and sums in fp32.  Every product is arranged so that its result's columns are the axis the
+// K = 4 steps for fp32), softmax statistics and sums in fp32.  The matrix unit takes both operands in one type, so P (before P v and P^T dO) and dS (before
+// dS k and dS^T q) are rounded to the tensors' sixteen-bit type, relative to the largest of their column: off by half a step of each, which averages out
+// over the keys - the output is then off by 1.3 to 1.5 times its own rounding.  Two numbers of the type instead of one cost another product each: free where
+// the kernel waits for memory (few queries, which does that), a third of the products in the others.  The softmax's sum, D and the table's
+// gradient take P and dS unrounded.  Every product is arranged so that its result's columns are the axis the
 // wave owns (queries in the forward and dq passes, keys in the dk / dv pass): scores come out with a query's keys in one lane's registers, and go
 // straight back in as the next product's right operand - P and dS never pass through LDS.  Their key order inside a K = 32 step
 // (16 (j / 4) + 4 (lane / 16) + j % 4) is matched by reading the other operand transposed from its row-major tile.

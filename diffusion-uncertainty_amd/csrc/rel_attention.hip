@@ -31,9 +31,11 @@ __device__ __forceinline__ void finish_query(const AttP& p, int b, int h, int q,
 
 // Online softmax with a lazy maximum: the sums are moved to a new maximum only when a score exceeds the old one by more than 2^8 - fp32 sums and
 // the rounded P (relative) lose nothing, and after a row's first tile it hardly ever happens.
-// Bound by the vector unit beside the matrix unit: a step of 32 keys x 32 queries is 256 cycles of matrix instructions at ch = 64, as many of LDS
-// reads, and some 450 of vector instructions, most of them the exponentials.  4 x 16 heads of 64, 4096 tokens bf16: 370 us, 740 TFLOP/s (a
-// large matrix product: 1120); 4 x 16 heads of 128 on 4, 4001 tokens causal: 378 us, 695; 16 x 16 heads of 72, 258 tokens fp32: 80 us, 61 (154).
+// Sixteen bit: no unit is full - two waves a SIMD take turns on products, softmax and the products that wait for it.  Busy of the CUs' time: vector unit 44 %
+// (128 wide) to 57 % (64), LDS 45 % (18 of them bank conflicts) and 32 %, matrix unit 35 % and 22 %; a wave waits a third of its time for data, a quarter to
+// issue.  fp32: matrix unit 54 %, half of a wave's time waiting for it; 72 channels run as 80, 258 queries as 320, 1280 workgroups in two rounds of
+// 768 places.  4 x 16 heads of 64, 4096 tokens bf16: 370 us, 740 TFLOP/s (a large matrix product: 1120); 4 x 16 heads of 128 on 4, 4001 tokens
+// causal: 362 us, 725 (402 in an unbroken run of such calls); 16 x 16 heads of 72, 258 tokens fp32: 80 us, 61 (154).
 template <typename T, int CHP>
 __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
     typedef Shape<T, CHP> S;

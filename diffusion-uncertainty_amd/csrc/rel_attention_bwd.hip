@@ -38,10 +38,9 @@ static_assert(NWAVE == 4, "flush_diagonals adds four waves");
 
 // ------------------------------------------------------------------------------------------------------------------------ dq
 // dq: 6 ch matrix operations a pair; a wave holds 32 queries' q, dO and dq, the keys and values pass through LDS, and every fragment read from there
-// feeds two products.  Bound by three units that take turns more than they overlap: a step of 32 x 32 pairs is 384 cycles of matrix
-// instructions, about as many of LDS reads (four waves), some 600 of vector instructions (exponentials at a quarter of the rate).  Three waves a SIMD at head
-// widths up to 64 (20 bytes of spill): 4 x 16 heads of 64, 4096 tokens bf16 1282 us a backward pass, 1356 with two.  8 x 16 heads, 1024 tokens of 64 bf16
-// in a padded batch: 83 us.
+// feeds two products.  Bound by three units that take turns more than they overlap: at 64 bf16 the vector unit is busy 55 % of the CUs' time, LDS 32, the
+// matrix unit 25, and a wave waits 40 % of its time for data.  Three waves a SIMD at head widths up to 64 (20 bytes of spill, fp16 40): 4 x 16 heads of 64,
+// 4096 tokens bf16 1282 us a backward pass, 1356 with two.  8 x 16 heads, 1024 tokens of 64 bf16 in a padded batch: 77 us.  fp32: matrix unit 58 %.
 template <typename T, int CHP>
 __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 3) void k_rel_attention_dq(AttP p) {
     typedef Shape<T, CHP> S;
@@ -238,9 +237,11 @@ int table_gradient(const AttP& p, int nparts, hipStream_t st) {
 
 // -------------------------------------------------------------------------------------------------------------------- dk, dv
 // dk, dv and the diagonal sums: 8 ch matrix operations a pair; a wave holds 32 keys' k, v, dk and dv (wide heads and fp32: 16), the queries and dO pass
-// through LDS, read as rows for the scores and as columns for the sums.  Bound by those reads: 16 keys a wave on three waves a SIMD read twice as much and
-// take 286 us a backward pass, on four 309, where 32 keys on two take 247 (8 x 16 heads, 1024 tokens of 64 bf16; 164 us are this kernel).  The sums along
-// the diagonals cost there 210 -> 246 us at radius 128, 369 at radius 512: where a tile is nearer than the radius every dS is shifted to its diagonal.
+// through LDS, read as rows for the scores and as columns for the sums.  LDS, busy 51 % of the CUs' time (vector unit 31, matrix unit 17), is the fullest unit
+// and a wave waits 40 % of its time: 16 keys a wave on three waves a SIMD read twice as much and take 286 us a backward pass, on four 309, where 32 keys on two
+// take 243 (8 x 16 heads, 1024 tokens of 64 bf16; 152 us are this kernel in a padded batch).  The sums along the diagonals cost there 210 -> 246 us at
+// radius 128, 369 at radius 512: where a tile is nearer than the radius every dS is shifted to its diagonal.  fp32: matrix unit 47 %, LDS 38; at 65 to
+// 80 wide three waves a SIMD spill 17 registers (72 bytes a lane: addresses and the like, written once, read again by every tile).
 template <typename T, int CHP>
 __global__ __launch_bounds__(NTHR, sizeof(T) == 4 && CHP <= 80 ? 3 : 2) void k_rel_attention_dkv(AttP p) {
     typedef Shape<T, CHP> S;

@@ -242,9 +242,11 @@ __device__ __forceinline__ void row_stats(const float* f, int D, int kind, float
 }
 
 // LANES: a unit's lanes (16, 32, 64), 0: the workgroup of at most WAVES wavefronts.  PL: elements of a row a thread.  The loads of the next row are in
-// flight while one is reduced (of the next two: no faster, 5 - 20 % slower where the registers then hold fewer waves).  Bound by memory: 5.2 - 6.3 TB/s at
-// widths that fill their waves (8192 rows of 4096 bf16 47 us, 16384 of 1024 fp32 43 us; a copy of 512 MB: 5.3); rows whose last wave is mostly empty wait
-// for their barriers (16512 rows of 1152 fp32, 4.5 of 5 waves: 74 us, 4.1 TB/s; bf16, 2.25 of 3: 34 - 49 us, 3.1 - 4.4).
+// flight while one is reduced (of the next two: no faster, 5 - 20 % slower where the registers then hold fewer waves).  Bound by memory: called over and
+// over on the same rows, partly from the 256 MB cache, 5.2 - 6.3 TB/s at widths that fill their waves (8192 rows of 4096 bf16 47 us, 16384 of 1024 fp32
+// 43 us; a copy of 512 MB: 5.3), in a training step 56 us (4.8 TB/s) for the first; the vector unit is busy two thirds of the time.  Rows whose last wave is
+// mostly empty wait for their barriers (16512 rows of 1152 fp32, 4.5 of 5 waves: 74 us, 4.1 TB/s, in a training step 88; bf16, 2.25 of 3:
+// 34 - 49 us, 3.1 - 4.4).
 template <typename T, typename PT, int LANES, int WAVES, int PL>
 __global__ __launch_bounds__(64 * WAVES) void k_sandwich_norm(NormP p) {
     constexpr int V = chunk_of<T, PL>();
@@ -300,7 +302,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sandwich_norm(NormP p) {
 //   t = dr + pre'(dz);  dx = a t;  du = g t;  dgate = sum t u;  dy = post'(du);  dpost_w = sum du hy;  dpost_b = sum du;  dpre_w = sum dz hr.
 // r is not read: it is x, y and the saved statistics again, in fp32 (reading it would replace x and bring its rounding into hr).
 // A unit sums its rows' columns in registers, a workgroup its units in their order, k_sandwich_cols the workgroups in theirs: the same
-// sums in every run.  Bound by memory and by the registers of five column sums: 8192 rows of 4096 bf16 82 us, 4.9 TB/s; 16512 of 1152 fp32 117 us, 3.9;
+// sums in every run.  Bound by memory and by the registers of five column sums: 8192 rows of 4096 bf16 82 us, 4.9 TB/s; 16512 of 1152 fp32 114 us, 4.0;
 // rows of more than 4096 elements spill (4096 rows of 8192 fp32 294 us, 2.7; bf16 rows of 8192 3.3).
 template <typename T, typename PT, int LANES, int WAVES, int PL, bool LDS>
 __global__ __launch_bounds__(64 * WAVES) void k_sandwich_norm_bwd(NormP p) {

@@ -1,16 +1,21 @@
 // Log probabilities of given tokens with the entropy of each row's distribution and its k best alternatives, and their gradient.
 //   l = t x;  lse = log sum e^l;  logprob = l_id - lse;  H = -sum p l^  (l^ = l - lse, p = e^l^);  top k by (value descending, index ascending)
 //   dx = t [ glp (d_id - p) + sum_j gtop_j (d_top_j - p) - gH p (l^ + H) ]
-// Memory bound: the row is read once (backward: read once, written once).  One pass keeps, per thread, the running maximum m and the sums
-// s = sum e^(l-m), w = sum e^(l-m) (l-m), all fp32 and rescaled when m moves; lse = m + log s, H = log s - w / s.  Differences x - m are
-// formed BEFORE the temperature and the base change, so huge common offsets and masks of the type's lowest value keep their meaning.
-// The alternatives ride along: a thread remembers its best 16-byte group and the best value outside it.  The k-th largest of the threads'
-// maxima is a lower bound of the row's k-th largest value; only groups that reach it are read again (about k of them), a thread whose
-// second value reaches it too is re-read whole (about k^2 / 512 of them), and the few candidates are ranked exactly.  Rows with many equal
-// values, NaN or +inf take an ordered scan of the row in the same kernel (select_ordered).
+// Memory bound: the row is read once (backward: read once, written once).  One pass keeps, per thread, s = sum 2^(L - ref) and w = sum 2^(L - ref) (L - ref)
+// of the logits in log2 units, L = x t log2 e, in fp32; ref is any float near the largest L and moves when a value passes it by 2^16, so lse =
+// ln 2 (ref + log2 s), H = ln 2 (log2 s - w / s).  L - ref is one fused multiply-add, exact but for its rounding: offsets common to a row keep their digits
+// as far as L has them.  Rows beyond +-2^28 (offsets of 1e30, masks of the type's lowest value everywhere) are summed again relative to their largest logit,
+// x - m formed before the temperature and the base change (scan_huge).
+// The alternatives ride along: a thread remembers the best value of its pairs of 16-byte groups (g, g + 256) with its pair, and the best value outside
+// that pair.  The smallest of the k largest maxima of 64, 128 or 256 sets of threads (k up to 16, 32, 64) is a lower bound of the row's k-th largest value;
+// only pairs that reach it are read again, a thread whose second value reaches it too is re-read whole, and the few candidates are ranked exactly.
+// Rows with many equal values, NaN or +inf take an ordered scan of the row in the same kernel (select_ordered).
 // A row may begin anywhere and be of any length.
-// Measured: 2048 rows of 128000 bf16 110 us without alternatives (4.8 TB/s: an exponential and some six more vector instructions an element bound it), 117 with
-// 20; 4112 rows of 16385 fp32 44 us (6.1 TB/s), 53 with 8; gradients 113 us (4.8 TB/s; a copy takes 103); 4 rows of 32000: 8 + 4 us in parts.
+// Measured: 2048 rows of 128000 bf16, 20 alternatives 118 us (4.5 TB/s; the vector unit is busy three quarters of the time: an exponential and some six more
+// instructions an element), 106 without.  4112 rows of 16385 fp32 in a training step, inputs from memory: 88 us with 8 alternatives (3.1 TB/s: the waves wait
+// three quarters of the time, and a row of 64 KB ends in reductions and the ranking, under which no load of its own runs; called over and over on
+// one input, mostly from the 256 MB cache, 53), gradients 98 us (5.5 TB/s; 120 if the forward pass was long ago; 2048 rows of 128000 bf16 226, 4.7).
+// 4 rows of 32000: 8 + 4 us in parts.
 #include <float.h>
 #include "elem.h"
 

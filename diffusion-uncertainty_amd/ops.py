@@ -1394,8 +1394,10 @@ def rel_attention(q, k, v, table, buckets, heads, kv_heads=None, causal=False, s
     q [B, Tq, heads * ch], k / v [B, Tk, kv_heads * ch] (views with unit stride along the last dimension: thirds of a qkv projection, slots
     of a cache), head widths up to 128 in multiples of 8 (fp32: 4); query head h attends to kv head h // (heads // kv_heads); table [num_buckets, heads] in fp32 or q's
     type; klen / qstart int32 [B].  A query without keys gives zeros; keys behind klen (causal: or the last query)
-    are not read; a table value below -1e30 masks its distances, other finite ones are taken as between -65504 and 65504 (beside a larger one
-    a score has no digits in fp32).  Tq = 1 with qstart = klen - 1 is decoding.  want_lse=True: also RelAttentionSaved(lse [B, heads, Tq] = log sum e^s, out_lo: what out's rounding left), for the backward pass."""
+    are not read, others have to be finite also where a query does not see them; a table value below -1e30 masks its distances, other finite ones are taken as between -65504 and 65504 (beside a larger one
+    a score has no digits in fp32).  Tq = 1 with qstart = klen - 1 is decoding.  want_lse=True: also RelAttentionSaved(lse [B, heads, Tq] = log sum e^s, out_lo: what out's rounding left), for the backward pass.
+    bf16 / fp16: softmax statistics and sums in fp32, the probabilities rounded to that type before their product with v (not where the query heads of a
+    kv head times Tq are at most 16)."""
     a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lse = lo = None
@@ -1413,7 +1415,8 @@ def rel_attention(q, k, v, table, buckets, heads, kv_heads=None, causal=False, s
 
 def rel_attention_bwd(q, k, v, table, buckets, out, saved, dout, heads, kv_heads=None, causal=False, scale=None, klen=None, qstart=None):
     """Gradients of rel_attention (same arguments, `out` and `saved` of the forward call with want_lse) given that of out -> dq, dk, dv, dtable (in their
-    operands' types; shared kv heads and the table summed over all that read them; zeros for keys behind klen)."""
+    operands' types; shared kv heads and the table summed over all that read them; zeros for keys behind klen).  bf16 / fp16: probabilities and the
+    scores' gradients are rounded to that type before their products, relative to the largest of a sum - fp16 gradients of any size keep their digits."""
     a = _rel_args(q, k, v, table, buckets, heads, kv_heads, causal, scale, klen, qstart)
     _token_tensor(out, "out", (q.dtype,), q.shape, q.device, contiguous=False)
     _token_tensor(dout, "dout", (q.dtype,), q.shape, q.device, contiguous=False)
@@ -1494,7 +1497,7 @@ def token_logprobs(logits, ids=None, k=0, inv_temperature=1.0):
 
 def token_logprobs_bwd(logits, ids, saved, dlogprob=None, dentropy=None, dtop=None, inv_temperature=1.0, out=None):
     """Gradient of token_logprobs' logprob, entropy and top_logprobs (any of them None: no gradient) with respect to the logits; `saved`: the
-    forward call's TokenLogprobs.  out: where to (like logits; logits itself: in place).  Rows without a finite logit get zeros."""
+    forward call's TokenLogprobs.  out: where to (like logits; logits itself: in place; else not overlapping them).  Rows without a finite logit get zeros."""
     k = saved.top_ids.shape[-1] if dtop is not None and saved.top_ids is not None else 0
     if dtop is not None and not k:
         raise ValueError("dtop: the forward call kept no alternatives")

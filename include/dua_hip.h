@@ -599,7 +599,10 @@ int dua_mc_var_grad(const float* stack, float* grad, int M, size_t n, float scal
 
 /* ---------------- token operators: transformers over tokens, their training and their answers ----------------
  * The pieces a denoiser / language model over TOKENS needs next to the image path above; each with its gradient.  Tensors of one of three
- * types; sums, softmax statistics and norms in fp32.  Results of a call do not depend on the run (no unordered sums). */
+ * types; sums, softmax statistics and norms in fp32.  Results of a call do not depend on the run (no unordered sums).
+ * Attention in bf16 / fp16 rounds its probabilities and, in the backward pass, the scores' gradients dS to that type before their products with
+ * v, dout, k and q (relative to the largest of a sum, whatever their size: fp16 gradients neither underflow nor overflow inside); the forward pass of few
+ * queries (heads / kv_heads * Tq <= 16) does not. */
 #define DUA_DTYPE_F32 0
 #define DUA_DTYPE_BF16 1
 #define DUA_DTYPE_F16 2
@@ -635,7 +638,8 @@ int dua_sandwich_norm_bwd(const dua_sandwich_norm_args* args_host, void* stream)
  * out_lo [B][heads][Tq][ch] = what out's rounding to bf16 / fp16 left, 16-byte aligned (NULL: not kept; the backward pass then takes out as it
  * is, and its gradients carry that rounding).  A query
  * without keys gives zeros (lse = -inf).  Keys behind klen or, with causal,
- * behind the last query are not read; a table value below -1e30 masks its distances, other finite ones are taken as between -65504 and 65504.  q, out [B][Tq][heads * ch], k, v [B][Tk][kv_heads * ch] with strides
+ * behind the last query are not read; others have to be finite also where a query does not see them (0 times infinity); a table value below -1e30 masks its
+ * distances, other finite ones are taken as between -65504 and 65504.  q, out [B][Tq][heads * ch], k, v [B][Tk][kv_heads * ch] with strides
  * of their own (elements); query head h reads kv head h / (heads / kv_heads);
  * ch <= 128, a multiple of 8 (fp32: 4); row strides below 2^24.  table [num_buckets][heads] (table_dtype: fp32 or
  * dtype), bucket_map [2 radius + 1]: entries outside [0, num_buckets) add no bias; radius <= 1024.  Tq = 1 is decoding.
@@ -671,7 +675,7 @@ int dua_rel_attention_bwd(const dua_rel_attention_args* args_host, void* stream)
  *   logprob[i] = l[ids[i]] - lse[i] (an id outside [0, V), or ids NULL: 0 and no gradient), entropy[i] = -sum p log p, lse[i] = log sum e^l,
  *   top_ids / top_logprobs [rows][k]: the k largest, ties to the lowest index, NaN above every number; k <= 64.
  * Logits of -inf have probability 0; a row without a finite value gives logprob = lse = -inf, entropy 0 and no gradient; NaN or +inf: NaN.
- * stats [rows][4] is what the backward pass takes. */
+ * stats [rows][4] is what the backward pass takes.  dlogits is logits itself (one row stride) or does not overlap them. */
 typedef struct {
     const void* logits;
     int dtype;
