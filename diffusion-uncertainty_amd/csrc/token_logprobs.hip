@@ -346,10 +346,12 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return k == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((k >> 31) ? k & 0x7FFFFFFFu : ~k);
 }
 
-// log p of a value from the row's reference and log2 s (a masked value near the type's lowest has no log2 units in fp32's range: natural ones)
+// log p of a value from the row's reference and log2 s (a masked value near the type's lowest has no log2 units in fp32's range: natural ones).  Of a token
+// that decides its row the two cancel but for their roundings: not above 0 (NaN stays).
 __device__ __forceinline__ float value_lp(float x, float ref, float logs, bool huge, float t) {
-    if (huge) return (x - ref) * t - LN2 * logs;
-    return fabsf(x) > 1e30f ? x * t - LN2 * (ref + logs) : LN2 * (fmaf(x, t * LOG2E, -ref) - logs);
+    const float lp = huge ? (x - ref) * t - LN2 * logs
+                          : (fabsf(x) > 1e30f ? x * t - LN2 * (ref + logs) : LN2 * (fmaf(x, t * LOG2E, -ref) - logs));
+    return lp > 0.f ? 0.f : lp;
 }
 
 // A row without any finite value has no distribution: log probabilities -inf, entropy 0.
@@ -358,7 +360,8 @@ __device__ void finish_row(const LogpP& p, long r, Soft a, bool huge, const uint
     const float logs = a.s > 0.f || a.s != a.s ? log2f(a.s) : -INFINITY;
     const bool none = logs == -INFINITY;
     if (threadIdx.x == 0) {
-        const float H = none ? 0.f : LN2 * (logs - a.w / a.s);
+        float H = none ? 0.f : LN2 * (logs - a.w / a.s);
+        if (H < 0.f) H = 0.f;                                  // (the same rounding of a decided row)
         const int64_t id = p.ids ? p.ids[r] : -1;
         float lp = 0.f;
         if (id >= 0 && id < p.V) lp = none ? -INFINITY : value_lp((float)((const T*)p.x)[r * p.ld + id], a.ref, logs, huge, p.t);

@@ -737,6 +737,22 @@ def test_token_logprobs_temperature_and_masks(dt):
     logprob_case(x, ids, 0, t=1.7)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+def test_token_logprobs_of_decided_rows_keep_their_sign(dt):
+    """Rows that one token decides: no log probability above 0, no entropy below it (a square root or log(1 - p) of them would be NaN)."""
+    from diffusion_uncertainty_amd import ops
+    g = torch.Generator().manual_seed(14)
+    for V in (7, 1001, 40000):
+        x = rnd(g, 64, V, dtype=dt)
+        best = torch.randint(0, V, (64,), generator=g)
+        lead = torch.linspace(0, 40, 64)
+        x[torch.arange(64), best] = (x.float().max(1).values + lead + 5.0 * torch.rand(64, generator=g)).to(dt)
+        x[32:] = (x[32:].float() + 300.0 * torch.rand(32, 1, generator=g)).to(dt)
+        for t in (1.0, 0.7, 3.1):
+            o = logprob_case(x, best, min(V, 5), t=t, grads=False)
+            assert (o.logprob <= 0).all() and (o.top_logprobs <= 0).all() and (o.entropy >= 0).all(), (V, t, float(o.logprob.max()), float(o.entropy.min()))
+
+
 def test_token_logprobs_huge_offsets():
     g = torch.Generator().manual_seed(6)
     x = rnd(g, 4, 700) + torch.tensor([3e4, -3e4, 1e30, -2e38])[:, None]
