@@ -523,7 +523,7 @@ int check_common(const dua_token_logprobs_args* a, const char* who) {
     DUA_REQUIRE(dua_dtype_ok(a->dtype), "%s: dtype must be fp32, bf16 or fp16", who);
     DUA_REQUIRE(a->rows >= 0 && a->rows < (1L << 24) && a->V >= 1 && a->V < (1L << 30) && a->ld >= a->V, "%s: rows in [0, 2^24), V in [1, 2^30), ld >= V", who);
     DUA_REQUIRE(a->k >= 0 && a->k <= KMAX && a->k <= a->V, "%s: k must be in [0, %d] and at most V", who, KMAX);
-    DUA_REQUIRE(a->inv_temperature > 0.f && a->inv_temperature < INFINITY, "%s: inv_temperature must be positive and finite", who);
+    DUA_REQUIRE(a->inv_temperature > 0.f && a->inv_temperature * LOG2E < INFINITY, "%s: inv_temperature must be positive and finite, also times log2 e", who);
     DUA_REQUIRE(a->rows == 0 || (a->logits && a->stats && ((uintptr_t)a->stats & 15) == 0), "%s: null logits / stats, or stats not 16-byte aligned", who);
     return DUA_OK;
 }

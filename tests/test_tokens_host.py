@@ -186,3 +186,13 @@ def test_token_logprobs_parts_have_no_cliff():
     assert [parts(r, 65536, 0) for r in (255, 256, 512)] == [3, 4, 2]
     assert [parts(r, 65536, 2) for r in (255, 256, 512)] == [3, 0, 0]
     assert parts(4, 8191, 0) == 0 and parts(4, 8192, 0) == 2
+
+
+def test_token_logprobs_refuses_a_temperature_without_log2_units():
+    from diffusion_uncertainty_amd import _lib
+    L = _lib.lib()
+    P = 4096
+    for t, ok in ((3e38, False), (2.4e38, False), (1e38, True)):
+        a = _lib.TokenLogprobsArgs(logits=P, rows=0, V=100, ld=100, k=0, inv_temperature=t, logprob=P, entropy=P, lse=P, stats=P)
+        assert (L.dua_token_logprobs(ctypes.byref(a), None) == 0) == ok
+        assert ok or "inv_temperature" in L.dua_last_error().decode()
