@@ -165,7 +165,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_rel_attention(AttP p) {
 // through the wave's own LDS tile to be read transposed; workgroups split the keys further and k_rel_attention_join adds up.
 // The matrix unit waits for memory here, so P goes into its product with v twice, rounded and what the rounding left: the output is off by its own rounding
 // alone (bf16 1.66e-3 of its size against 2.3e-3, fp16 2.1e-4 against 2.9e-4; 48.1 -> 48.4 and 26.5 -> 27.0 us in the first two examples).
-// 32 sequences of 4096 keys, 4 kv heads of 128 bf16: 48 us, 5.6 TB/s; 2 of 30001 fp16: 25 + 4 us, 4.2 TB/s; 8 of 1000, 16 heads of 64: 11 + 4 us, where
+// 32 sequences of 4096 keys, 4 kv heads of 128 bf16: 48 us, 5.6 TB/s; 2 of 30001 fp16: 27 + 4 us, 3.9 TB/s; 8 of 1000, 16 heads of 64: 15 + 4 us, where
 // the launches and the dependent loads of three tiles count.
 template <typename T, int CHP>
 __global__ __launch_bounds__(NTHR, CHP > 64 ? 2 : 4) void k_rel_attention_few(AttP p) {
